@@ -39,6 +39,7 @@ extern "C" {
 /* element types */
 #define SB_F16 1
 #define SB_F32 2
+#define SB_BF16 3             /* the paged-cache operators only */
 #define SB_SCALE_F16 SB_F16
 #define SB_SCALE_F32 SB_F32
 
@@ -581,6 +582,60 @@ int sb_ple_gate_act(const float* pre, int ld_pre, int64_t plane, int nsplit, con
 /* out16[i] = f16(x[i]) (round to nearest even), i < n: the f16 A operand of a
  * prefill GEMM taken from an f32 residual stream. */
 int sb_cast_f16(const float* x, void* out16, int64_t n, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Serving several sequences over a paged key-value cache.  Pages hold
+ * page_size tokens (a power of two) of every kv head; page p, head g, token j
+ * starts at element p * page_stride + g * head_stride + j * token_stride of k
+ * and of v (head_dim values in f16 or bf16, on a 16-byte boundary), so both
+ * orders of heads and tokens inside a page are served.  A page table is device
+ * int32 [n_seqs][max_pages]: entry i of a row is the page of the sequence's
+ * positions i * page_size ...  An entry outside [0, n_pages) is no page: nothing
+ * is written there and its keys take no part.  Query head h reads kv head
+ * h / (n_heads / n_kv_heads).  No counterpart in the reference (one sequence,
+ * one contiguous cache).
+ * ------------------------------------------------------------------------- */
+typedef struct sb_paged_kv {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, token_stride; /* elements, multiples of 8 */
+  int32_t dtype;                                   /* SB_F16 or SB_BF16 */
+  int32_t n_pages, page_size, n_kv_heads, head_dim; /* head_dim in {64, 128, 256, 512} */
+} sb_paged_kv;
+
+/*
+ * Append t tokens: row i of qkv (f16, bf16 or f32, row stride ld) holds n_heads
+ * query heads, then n_kv_heads keys, then n_kv_heads values of head_dim.  Each
+ * q and k head is RMS-normalised when its weight is given (q_norm, k_norm
+ * [head_dim] f32; x / sqrt(mean(x^2) + eps) * w, v_norm != 0: v without a
+ * weight), then rotated at position pos[i]: values j and j + rot/2 pair up for
+ * j < rot/2, values from rot on pass through (rot a multiple of 16, 0 for no
+ * rotation; cos_t, sin_t f32 [max_pos][rot/2]).  q goes to q_out
+ * [t][n_heads][head_dim] in the cache's type (NULL: not wanted), k and v to
+ * position pos[i] of the sequence of page-table row seq[i] (seq NULL: row i).
+ * A token with pos[i] outside [0, max_pos) is padding: its q is zero and
+ * nothing is appended.  Two tokens of one call must not share a place.
+ */
+int sb_kv_append_paged(const sb_paged_kv* kv, const int32_t* page_table, int n_seqs, int max_pages, const void* qkv,
+                       int qkv_dtype, int64_t ld, int t, int n_heads, const int32_t* seq, const int32_t* pos,
+                       const float* q_norm, const float* k_norm, int v_norm, float eps, const float* cos_t,
+                       const float* sin_t, int rot, int max_pos, void* q_out, void* stream);
+
+/*
+ * Attention of one new token per sequence: out[i][h] = softmax(scale *
+ * q[i][h] . K) V over the cached keys at positions lo .. pos[i] of page-table
+ * row i, lo = 0, or pos[i] + 1 - window when window > 0; a row without a key
+ * (pos[i] < 0) gives zeros.  q [b] rows of [n_heads][head_dim] q_stride elements
+ * apart and out [b][n_heads][head_dim] are of the cache's type.
+ * workspace: device, 16-byte aligned, at least
+ * sb_attn_decode_paged_workspace_size bytes, zero before the first call; each
+ * call leaves it ready for the next, of the same or of smaller shape.  Calls that may
+ * overlap on the GPU need their own.
+ */
+int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_table, int max_pages, const int32_t* pos, int b,
+                         const void* q, int64_t q_stride, int n_heads, int window, float scale, void* out,
+                         void* workspace, size_t workspace_bytes, void* stream);
+size_t sb_attn_decode_paged_workspace_size(const sb_paged_kv* kv, int n_heads, int b);
 
 #ifdef __cplusplus
 }

@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(HERE, "libslang_b200.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "slang_b200.h")
 
 SB_OK, SB_ERR_ARG, SB_ERR_ALIGN, SB_ERR_CUDA, SB_ERR_TIMEOUT, SB_ERR_WORKSPACE = 0, 1, 2, 3, 4, 5
-SB_F16, SB_F32 = 1, 2
+SB_F16, SB_F32, SB_BF16 = 1, 2, 3
 
 _vp, _i, _f, _sz, _i64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_int64
 
@@ -78,7 +78,18 @@ SIGNATURES = {
     "sb_decode_step_fused": ([_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _f, _vp, _vp, _vp,
                               _vp, _i, _vp, _vp, _sz, _vp], _i),
     "sb_decode_step_fused_scratch_size": ([_i, _i, _i, _i, _i], _sz),
+    "sb_kv_append_paged": ([_vp, _vp, _i, _i, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _vp, _i, _f, _vp, _vp, _i, _i, _vp,
+                            _vp], _i),
+    "sb_attn_decode_paged": ([_vp, _vp, _i, _vp, _i, _vp, _i64, _i, _i, _f, _vp, _vp, _sz, _vp], _i),
+    "sb_attn_decode_paged_workspace_size": ([_vp, _i, _i], _sz),
 }
+
+
+class PagedKVDesc(C.Structure):
+    """``sb_paged_kv``."""
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("head_stride", _i64), ("token_stride", _i64),
+                ("dtype", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32)]
 
 
 class SlangError(RuntimeError):

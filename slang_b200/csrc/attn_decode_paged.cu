@@ -1,0 +1,521 @@
+// Attention of one new token per sequence over a paged key-value cache
+// (sb_attn_decode_paged): out[b, h] = softmax_t(scale q[b, h] . K_t) V over the
+// keys t in [lo, pos[b]] of the sequence's pages, lo = 0 or pos + 1 - window.
+//
+// Bound by reading K and V once.  The cached keys of every (sequence, kv head)
+// are cut into blocks of KB keys, the blocks of all of them are laid end to
+// end, and each CTA of one resident wave takes an equal run of blocks: the SMs
+// stay busy to the end whatever the lengths are, and the split needs no host
+// knowledge of them.  A (sequence, kv head) that ends up in several CTAs is
+// joined by the CTA that finishes it last (a counter, no waiting):
+//   out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c,   M = max m_c.
+//
+// A warp reads K and V straight into registers in the layout of the tensor
+// cores' operands (mma.sync m16n8k16): per CTA nothing is staged in shared
+// memory and no warp waits for another until the join.  With t = lane % 4 and
+// g = lane / 4:
+//   S = Q K^T   A = Q (rows = the kv head's query heads, at most 8 or 16),
+//               B = K: lane (g, t) loads 16 bytes of key g, dims 8 (t + 4 i) ...;
+//               the contraction runs over the same permutation of the dims
+//               on both sides, so whole vectors are the fragments.
+//   O^T = V^T P^T  B = P^T, which is S's accumulator layout as it stands;
+//               A = V^T: lane (g, t) loads 16 bytes (dims 64 c + 8 g ...) of keys
+//               2t, 2t+1, 2t+8, 2t+9 and pairs neighbouring keys with byte permutes.
+// The legacy tensor path suffices: 8 query heads per kv head need 51 TFLOP/s at
+// the full memory rate.
+//
+// p = 2^(s - m) is rounded to the cache's type for the second product (its
+// relative error is that of the output's own rounding); m, l, S and O are f32.
+// m only rises when a score passes it by 2^8, so O is rarely rescaled.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace {
+
+constexpr int W = 4;  // warps per CTA
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRise = 8.f;  // log2 units: p stays below 2^8
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                 uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct DecodeParams {
+  const void* q;
+  int64_t q_stride;  // elements between sequences
+  void* out;         // [b][nh][hd]
+  sbp::Pages pages;
+  const int32_t* pos;
+  unsigned int* count;  // [b * nkv * htiles], zero between calls
+  float* part;          // [grid][2][HT * (hd + 2)]
+  int b, nkv, group, htiles, window;  // htiles: tiles of HT query heads per kv head
+  float scale2;                       // scale * log2(e)
+};
+
+// Keys [lo, hi) of sequence b, hi clamped to what its pages hold.
+__device__ __forceinline__ void key_range(const DecodeParams& p, int b, int* lo, int* hi) {
+  const int pos = p.pos[b];
+  const int64_t held = static_cast<int64_t>(p.pages.max_pages) << p.pages.shift;
+  const int end = pos < 0 ? 0 : (pos < held ? pos + 1 : static_cast<int>(held));
+  *hi = end;
+  // the window ends at the token's own position, even when that lies past the pages
+  *lo = p.window > 0 && pos >= p.window ? (pos + 1 - p.window < end ? pos + 1 - p.window : end) : 0;
+}
+
+// HD: head_dim.  HS: warps that share a key tile, each with HD / HS of the dims.
+// NT: tiles of 8 query heads (HT = 8 NT heads per CTA).
+template <typename T, int HD, int HS, int NT>
+struct Shape {
+  static constexpr int HDW = HD / HS;
+  static constexpr int NS = 256 / HDW;     // 16-key subtiles per iteration: constant bytes in flight
+  static constexpr int TK = 16 * NS;       // keys per warp (team) and iteration
+  static constexpr int TEAMS = W / HS;
+  static constexpr int KB = TK * TEAMS;    // keys per block
+  static constexpr int HT = 8 * NT;
+  static constexpr int PART = HT * (HD + 2);       // a partial: O [HT][HD], m [HT], l [HT]
+  static constexpr int SM_O = TEAMS * HT * HD;     // each team's O
+  static constexpr int SM_F = SM_O + 2 * TEAMS * HT + (HS > 1 ? W * 32 * 4 * NS * NT : 0);
+};
+
+template <typename T, int HD, int HS, int NT>
+__global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const DecodeParams p) {
+  using C = Shape<T, HD, HS, NT>;
+  constexpr int HDW = C::HDW, NS = C::NS, TK = C::TK, TEAMS = C::TEAMS, KB = C::KB, HT = C::HT;
+  constexpr int KC = HDW / 32, VC = HDW / 64;  // 16-byte vectors of a key / of a value row per lane
+  extern __shared__ float sm[];
+  float* sm_o = sm;
+  float* sm_m = sm + C::SM_O;
+  float* sm_l = sm_m + TEAMS * HT;
+  float* sm_x = sm_l + TEAMS * HT;  // HS > 1: the teams' partial scores
+  __shared__ int sh_last;
+  __shared__ long long sh_scan[2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int team = warp / HS, half = warp % HS;
+  const int heads_per_seq = p.nkv * p.htiles;
+  sbd::griddep_launch_dependents();
+  sbd::griddep_wait();
+
+  // total blocks of all sequences, and this CTA's run of them [r0, r1)
+  auto blocks_of = [&](int b) {
+    int lo, hi;
+    key_range(p, b, &lo, &hi);
+    return static_cast<long long>((hi - lo + KB - 1) / KB) * heads_per_seq;
+  };
+  if (warp == 0) {
+    long long sum = 0;
+    for (int b = lane; b < p.b; b += 32) sum += blocks_of(b);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    // the sequence that holds this CTA's first block: scan 32 sequences at a time
+    const long long n = sum < gridDim.x ? sum : gridDim.x;
+    const long long r0 = n ? sum * blockIdx.x / n : 0;
+    long long before = 0;
+    int found = p.b;
+    long long found_before = sum;
+    if (blockIdx.x < n) {
+      for (int b0 = 0; b0 < p.b; b0 += 32) {
+        const long long own = b0 + lane < p.b ? blocks_of(b0 + lane) : 0;
+        long long inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+          if (lane >= o) inc += v;
+        }
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, before + inc > r0);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          found = b0 + l;
+          found_before = before + __shfl_sync(0xFFFFFFFFu, inc - own, l);
+          break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
+      }
+    }
+    if (lane == 0) {
+      sh_scan[0] = sum;
+      sh_scan[1] = found_before;
+      sh_last = found;
+    }
+  }
+  // sequences with no key at all: zero rows
+  for (int b = blockIdx.x; b < p.b; b += gridDim.x) {
+    int lo, hi;
+    key_range(p, b, &lo, &hi);
+    if (hi > lo) continue;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<int64_t>(b) * p.nkv * p.group * HD);
+    for (int i = threadIdx.x; i < p.nkv * p.group * HD / 8; i += W * 32) dst[i] = make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  const long long total = sh_scan[0];
+  long long seq_start = sh_scan[1];  // first block of sequence `b`
+  int b = sh_last;
+  // every CTA below n_cta holds at least one block, those from n_cta on hold none
+  const long long n_cta = total < gridDim.x ? total : gridDim.x;
+  const bool works = blockIdx.x < n_cta;
+  const long long r0 = works ? total * blockIdx.x / n_cta : 0, r1 = works ? total * (blockIdx.x + 1) / n_cta : 0;
+  const T* kbase = static_cast<const T*>(p.pages.k);
+  const T* vbase = static_cast<const T*>(p.pages.v);
+  const int pmask = (1 << p.pages.shift) - 1;
+
+  for (long long r = r0; r < r1;) {
+    int lo, hi;
+    key_range(p, b, &lo, &hi);
+    const int nblk = (hi - lo + KB - 1) / KB;
+    if (nblk == 0 || r >= seq_start + static_cast<long long>(nblk) * heads_per_seq) {
+      seq_start += static_cast<long long>(nblk) * heads_per_seq;
+      ++b;
+      continue;
+    }
+    const int hidx = static_cast<int>((r - seq_start) / nblk);  // (kv head, head tile)
+    const long long seg0 = seq_start + static_cast<long long>(hidx) * nblk, seg1 = seg0 + nblk;
+    const long long e = r1 < seg1 ? r1 : seg1;
+    const int kv = hidx / p.htiles, h0 = (hidx % p.htiles) * HT;  // query heads kv * group + h0 ...
+    const int nheads = min(HT, p.group - h0);
+    const int k_begin = lo + static_cast<int>(r - seg0) * KB;
+    const int k_end = min(hi, lo + static_cast<int>(e - seg0) * KB);
+    const int32_t* row = p.pages.table + static_cast<int64_t>(b) * p.pages.max_pages;
+
+    // Q fragments: vector i of lane (g, t) is dims half * HDW + 8 (t + 4 i) ... of heads g (and g + 8)
+    uint4 qf[NT][KC];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int h = g + 8 * n;
+      const T* qp = static_cast<const T*>(p.q) + b * p.q_stride + static_cast<int64_t>(kv * p.group + h0 + h) * HD + half * HDW + 8 * t;
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+        qf[n][i] = h < nheads ? *reinterpret_cast<const uint4*>(qp + 32 * i) : make_uint4(0, 0, 0, 0);
+    }
+    float o[4 * VC][NT][4];
+#pragma unroll
+    for (int i = 0; i < 4 * VC; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[i][n][x] = 0.f;
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n] = -INFINITY, l[n] = 0.f;
+
+    // page of key `key`, -1 for a key that takes no part
+    auto page_of = [&](int key) {
+      if (key >= k_end) return -1;
+      const int pg = row[key >> p.pages.shift];
+      return pg >= 0 && pg < p.pages.n_pages ? pg : -1;
+    };
+    // this lane holds the pages of keys base + lane (and + 32 when a tile has 64 keys)
+    constexpr int PL = TK > 32 ? 2 : 1;
+    int pg[PL], pg_next[PL];
+    auto fetch_pages = [&](int base, int (&d)[PL]) {
+#pragma unroll
+      for (int j = 0; j < PL; ++j) d[j] = lane + 32 * j < TK ? page_of(base + lane + 32 * j) : -1;
+    };
+    auto row_of = [&](const T* basep, int key, int page) {
+      return basep + page * p.pages.page_stride + kv * p.pages.head_stride + (key & pmask) * p.pages.token_stride;
+    };
+    uint4 kf[2 * NS][KC];
+    auto load_k = [&](int base, const int (&d)[PL]) {
+#pragma unroll
+      for (int j = 0; j < 2 * NS; ++j) {
+        const int in = 8 * j + g;
+        const int page = __shfl_sync(0xFFFFFFFFu, d[8 * j >= 32 ? PL - 1 : 0], in & 31);
+        const T* src = row_of(kbase, base + in, page) + half * HDW + 8 * t;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) kf[j][i] = page >= 0 ? sbd::ldg_nc_v4(src + 32 * i) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    int base = k_begin + team * TK;
+    fetch_pages(base, pg);
+    load_k(base, pg);
+    fetch_pages(base + KB, pg_next);
+    for (; base < k_end; base += KB) {
+      // V of this tile: keys 16 s + {2t, 2t+1, 2t+8, 2t+9}
+      uint4 vf[NS][4][VC];
+      uint32_t okmask = 0;  // bit 4 s + x: that key takes part
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int in = 16 * s + 2 * t + (x & 1) + 8 * (x >> 1);
+          const int page = __shfl_sync(0xFFFFFFFFu, pg[16 * s >= 32 ? PL - 1 : 0], in & 31);
+          const T* src = row_of(vbase, base + in, page) + half * HDW + 8 * g;
+          okmask |= page >= 0 ? 1u << (4 * s + x) : 0u;
+#pragma unroll
+          for (int c = 0; c < VC; ++c) vf[s][x][c] = page >= 0 ? sbd::ldg_nc_v4(src + 64 * c) : make_uint4(0, 0, 0, 0);
+        }
+      // S: rows = heads (g, g + 8), columns = keys 2t, 2t+1 of each 8-key tile
+      float sc[2 * NS][4];
+#pragma unroll
+      for (int j = 0; j < 2 * NS; ++j) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[j][x] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+          mma16816<T>(sc[j], qf[0][i].x, NT > 1 ? qf[NT - 1][i].x : 0u, qf[0][i].y, NT > 1 ? qf[NT - 1][i].y : 0u,
+                      kf[j][i].x, kf[j][i].y);
+          mma16816<T>(sc[j], qf[0][i].z, NT > 1 ? qf[NT - 1][i].z : 0u, qf[0][i].w, NT > 1 ? qf[NT - 1][i].w : 0u,
+                      kf[j][i].z, kf[j][i].w);
+        }
+      }
+      // the next tile's K while the softmax and the second product run
+      load_k(base + KB, pg_next);
+#pragma unroll
+      for (int j = 0; j < PL; ++j) pg[j] = pg_next[j];
+      fetch_pages(base + 2 * KB, pg_next);
+      if constexpr (HS > 1) {  // the sum of the team's shares of the dims, in one order for all of them
+        constexpr int N = 4 * NS * NT;
+        float* share = sm_x + (team * HS * 32 + lane) * N;
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j)
+#pragma unroll
+          for (int x = 0; x < 2 * NT; ++x) share[half * 32 * N + j * 2 * NT + x] = sc[j][x];
+        sbd::named_bar_sync(1 + team, HS * 32);
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j)
+#pragma unroll
+          for (int x = 0; x < 2 * NT; ++x) {
+            float sum = share[j * 2 * NT + x];
+#pragma unroll
+            for (int w = 1; w < HS; ++w) sum += share[w * 32 * N + j * 2 * NT + x];
+            sc[j][x] = sum;
+          }
+        sbd::named_bar_sync(1 + team, HS * 32);  // the buffer is free for the next tile
+      }
+      uint32_t pb[2 * NS][NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const bool ok = (okmask >> (4 * (j >> 1) + 2 * (j & 1) + x)) & 1u;
+            float& v = sc[j][2 * n + x];
+            v = ok ? v * p.scale2 : -INFINITY;
+            mx = fmaxf(mx, v);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+        const bool rise = mx > m[n] + kRise || (m[n] == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xFFFFFFFFu, rise)) {
+          const float alpha = rise ? (m[n] == -INFINITY ? 0.f : ex2(m[n] - mx)) : 1.f;
+          l[n] *= alpha;
+          if (rise) m[n] = mx;
+          const float a0 = __shfl_sync(0xFFFFFFFFu, alpha, 8 * t), a1 = __shfl_sync(0xFFFFFFFFu, alpha, 8 * t + 4);
+#pragma unroll
+          for (int i = 0; i < 4 * VC; ++i) {
+            o[i][n][0] *= a0, o[i][n][2] *= a0;
+            o[i][n][1] *= a1, o[i][n][3] *= a1;
+          }
+        }
+        const float mu = m[n] == -INFINITY ? 0.f : m[n];
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j) {
+          const float p0 = ex2(sc[j][2 * n] - mu), p1 = ex2(sc[j][2 * n + 1] - mu);
+          l[n] += p0 + p1;
+          pb[j][n] = sbp::pack2<T>(p0, p1);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          const uint32_t* r0v = reinterpret_cast<const uint32_t*>(&vf[s][0][c]);
+          const uint32_t* r1v = reinterpret_cast<const uint32_t*>(&vf[s][1][c]);
+          const uint32_t* r2v = reinterpret_cast<const uint32_t*>(&vf[s][2][c]);
+          const uint32_t* r3v = reinterpret_cast<const uint32_t*>(&vf[s][3][c]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t a0 = __byte_perm(r0v[w], r1v[w], 0x5410), a1 = __byte_perm(r0v[w], r1v[w], 0x7632);
+            const uint32_t a2 = __byte_perm(r2v[w], r3v[w], 0x5410), a3 = __byte_perm(r2v[w], r3v[w], 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<T>(o[4 * c + w][n], a0, a1, a2, a3, pb[2 * s][n], pb[2 * s + 1][n]);
+          }
+        }
+    }
+
+    // join the CTA's teams: every team's O, m, l in shared memory
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      l[n] += __shfl_xor_sync(0xFFFFFFFFu, l[n], 1);
+      l[n] += __shfl_xor_sync(0xFFFFFFFFu, l[n], 2);
+      if (half == 0 && t == 0) {
+        sm_m[team * HT + 8 * n + g] = m[n];
+        sm_l[team * HT + 8 * n + g] = l[n];
+      }
+      // lane (g, t): heads 8 n + 2t, + 1; dims half * HDW + 64 c + 8 g + 0..7
+#pragma unroll
+      for (int c = 0; c < VC; ++c)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          float* dst = sm_o + (team * HT + 8 * n + 2 * t + hh) * HD + half * HDW + 64 * c + 8 * g;
+          *reinterpret_cast<float4*>(dst) = make_float4(o[4 * c][n][hh], o[4 * c][n][2 + hh], o[4 * c + 1][n][hh], o[4 * c + 1][n][2 + hh]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(o[4 * c + 2][n][hh], o[4 * c + 2][n][2 + hh], o[4 * c + 3][n][hh], o[4 * c + 3][n][2 + hh]);
+        }
+    }
+    __syncthreads();
+    const bool whole = r == seg0 && e == seg1;
+    float* part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (r == r0 ? 0 : 1)) * C::PART;
+    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.nkv * p.group + kv * p.group + h0) * HD;
+    for (int i = threadIdx.x; i < nheads * (HD / 8); i += W * 32) {
+      const int h = i / (HD / 8), d = 8 * (i % (HD / 8));
+      float M = sm_m[h];
+#pragma unroll
+      for (int w = 1; w < TEAMS; ++w) M = fmaxf(M, sm_m[w * HT + h]);
+      const float mu = M == -INFINITY ? 0.f : M;
+      float L = 0.f, acc[8] = {};
+#pragma unroll
+      for (int w = 0; w < TEAMS; ++w) {
+        const float f = ex2(sm_m[w * HT + h] - mu);
+        L += f * sm_l[w * HT + h];
+        float v[8];
+        sbp::load8(sm_o + (w * HT + h) * HD + d, v);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) acc[x] += f * v[x];
+      }
+      if (whole) {
+        const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) acc[x] *= inv;
+        sbp::store8(out + h * HD + d, acc);
+      } else {
+        float4* dst = reinterpret_cast<float4*>(part + h * HD + d);
+        dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        if (d == 0) part[HT * HD + h] = M, part[HT * HD + HT + h] = L;
+      }
+    }
+    if (!whole) {
+      // the CTAs that hold blocks of this segment: [c0, c1]; the last to arrive joins them
+      const int c0 = static_cast<int>(((seg0 + 1) * n_cta - 1) / total), c1 = static_cast<int>((seg1 * n_cta - 1) / total);
+      unsigned int* cnt = p.count + static_cast<int64_t>(b) * heads_per_seq + hidx;
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const unsigned int seen = atomicAdd(cnt, 1u);
+        sh_last = seen == static_cast<unsigned int>(c1 - c0);
+        if (sh_last) *cnt = 0;
+      }
+      __syncthreads();
+      if (sh_last) {
+        __threadfence();
+        const bool first_aligned = total * c0 / n_cta == seg0;  // c0's run begins with this segment
+        for (int i = threadIdx.x; i < nheads * (HD / 8); i += W * 32) {
+          const int h = i / (HD / 8), d = 8 * (i % (HD / 8));
+          float M = -INFINITY, L = 0.f, acc[8] = {};
+          for (int c = c0; c <= c1; ++c) {
+            const float* src = p.part + (static_cast<int64_t>(c) * 2 + (c > c0 || first_aligned ? 0 : 1)) * C::PART;
+            const float mc = __ldcg(src + HT * HD + h), lc = __ldcg(src + HT * HD + HT + h);
+            const float4 v0 = __ldcg(reinterpret_cast<const float4*>(src + h * HD + d));
+            const float4 v1 = __ldcg(reinterpret_cast<const float4*>(src + h * HD + d + 4));
+            const float Mn = fmaxf(M, mc), mu = Mn == -INFINITY ? 0.f : Mn;
+            const float fo = ex2(M - mu), fn = ex2(mc - mu);
+            M = Mn;
+            L = L * fo + lc * fn;
+            const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+            for (int x = 0; x < 8; ++x) acc[x] = acc[x] * fo + v[x] * fn;
+          }
+          const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) acc[x] *= inv;
+          sbp::store8(out + h * HD + d, acc);
+        }
+      }
+    }
+    __syncthreads();  // shared memory is free for the next segment
+    r = e;
+  }
+}
+
+// CTAs of one resident wave, and the workspace's layout (counters, then partials).
+int grid_of() { return 2 * sb::num_sms(); }
+
+int head_tile(int group) { return group <= 8 ? 8 : 16; }
+
+size_t counter_bytes(const sb_paged_kv* kv, int n_heads, int b) {
+  const int group = n_heads / kv->n_kv_heads, ht = head_tile(group);
+  const size_t n = static_cast<size_t>(b) * kv->n_kv_heads * ((group + ht - 1) / ht);
+  return (n * 4 + 255) / 256 * 256;
+}
+
+template <typename T, int HD, int HS, int NT>
+int launch_decode(const DecodeParams& p, int grid, cudaStream_t stream) {
+  using C = Shape<T, HD, HS, NT>;
+  constexpr int smem = C::SM_F * 4;
+  static bool set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(attn_decode_paged_kernel<T, HD, HS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return sb::cuda_fail(e, "attn_decode_paged_kernel smem attribute");
+    if (dev >= 0 && dev < 64) set[dev] = true;
+  }
+  cudaError_t e = sb::launch_pdl(attn_decode_paged_kernel<T, HD, HS, NT>, dim3(grid), dim3(W * 32), smem, stream, p);
+  if (e != cudaSuccess) return sb::cuda_fail(e, "attn_decode_paged_kernel");
+  return sb::launch_status("attn_decode_paged_kernel");
+}
+
+template <typename T>
+int launch_decode_hd(int hd, int ht, const DecodeParams& p, int grid, cudaStream_t s) {
+  switch (hd) {
+    case 64: return ht == 8 ? launch_decode<T, 64, 1, 1>(p, grid, s) : launch_decode<T, 64, 1, 2>(p, grid, s);
+    case 128: return ht == 8 ? launch_decode<T, 128, 1, 1>(p, grid, s) : launch_decode<T, 128, 1, 2>(p, grid, s);
+    case 256: return ht == 8 ? launch_decode<T, 256, 1, 1>(p, grid, s) : launch_decode<T, 256, 2, 2>(p, grid, s);
+    default: return ht == 8 ? launch_decode<T, 512, 2, 1>(p, grid, s) : launch_decode<T, 512, 4, 2>(p, grid, s);
+  }
+}
+
+}  // namespace
+
+extern "C" size_t sb_attn_decode_paged_workspace_size(const sb_paged_kv* kv, int n_heads, int b) {
+  if (!kv || kv->n_kv_heads < 1 || n_heads < 1 || n_heads % kv->n_kv_heads || b < 1) return 0;
+  const int ht = head_tile(n_heads / kv->n_kv_heads);
+  return counter_bytes(kv, n_heads, b) + static_cast<size_t>(grid_of()) * 2 * ht * (kv->head_dim + 2) * sizeof(float);
+}
+
+extern "C" int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_table, int max_pages, const int32_t* pos,
+                                    int b, const void* q, int64_t q_stride, int n_heads, int window, float scale,
+                                    void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  DecodeParams p{};
+  int rc = sbp::check_pages("sb_attn_decode_paged", kv, page_table, max_pages, &p.pages);
+  if (rc) return rc;
+  SB_CHECK_ARG(b >= 0 && n_heads >= 1 && n_heads % kv->n_kv_heads == 0 && window >= 0,
+               "sb_attn_decode_paged: %d query heads over %d kv heads, or bad sizes", n_heads, kv->n_kv_heads);
+  SB_CHECK_ARG(b <= 1 || q_stride >= static_cast<int64_t>(n_heads) * kv->head_dim, "sb_attn_decode_paged: q_stride is shorter than a row");
+  if (b == 0) return SB_OK;
+  SB_CHECK_ARG(pos && q && out && workspace, "sb_attn_decode_paged: null pointer");
+  if (!sb::aligned(q, 16) || q_stride % 8 || !sb::aligned(out, 16) || !sb::aligned(workspace, 16))
+    return sb::fail(SB_ERR_ALIGN, "sb_attn_decode_paged: q rows, out and the workspace must start on 16-byte boundaries");
+  if (workspace_bytes < sb_attn_decode_paged_workspace_size(kv, n_heads, b))
+    return sb::fail(SB_ERR_WORKSPACE, "sb_attn_decode_paged: workspace of %zu bytes, %zu needed", workspace_bytes,
+                    sb_attn_decode_paged_workspace_size(kv, n_heads, b));
+  const int group = n_heads / kv->n_kv_heads, ht = head_tile(group);
+  p.q = q, p.q_stride = q_stride, p.out = out, p.pos = pos, p.b = b, p.nkv = kv->n_kv_heads, p.group = group;
+  p.htiles = (group + ht - 1) / ht, p.window = window, p.scale2 = scale * kLog2e;
+  p.count = static_cast<unsigned int*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + counter_bytes(kv, n_heads, b));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return kv->dtype == SB_F16 ? launch_decode_hd<__half>(kv->head_dim, ht, p, grid_of(), s)
+                             : launch_decode_hd<__nv_bfloat16>(kv->head_dim, ht, p, grid_of(), s);
+}

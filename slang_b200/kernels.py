@@ -7,10 +7,12 @@ theirs); wrappers only allocate an output when none is given.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
-from ._lib import SB_F16, SB_F32
+from ._lib import SB_BF16, SB_F16, SB_F32
 
 _DT = {torch.float16: SB_F16, torch.float32: SB_F32}
 
@@ -583,3 +585,142 @@ def _num_sms(dev) -> int:
     if key not in _SMS:
         _SMS[key] = torch.cuda.get_device_properties(dev).multi_processor_count
     return _SMS[key]
+
+
+# ---------------------------------------------------------------- paged-cache serving
+
+_DT_PAGED = {torch.float16: SB_F16, torch.bfloat16: SB_BF16}
+_DT_ALL = {torch.float16: SB_F16, torch.bfloat16: SB_BF16, torch.float32: SB_F32}
+
+
+def _int32(t: torch.Tensor, name: str, dim: int, dev) -> None:
+    """An int32 operand of the serving operators: contiguous, on the cache's GPU."""
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected torch.int32")
+    if t.dim() != dim or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must be a contiguous {dim}-dimensional tensor on {dev}")
+
+
+def _f32_vec(t: torch.Tensor | None, name: str, n: int, dev) -> None:
+    if t is None:
+        return
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected torch.float32")
+    if t.numel() != n or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must hold {n} contiguous values on {dev}")
+
+
+class PagedKV:
+    """One layer's paged key-value cache: ``k`` and ``v`` are f16 or bf16 tensors (or views)
+    [n_pages, n_kv_heads, page_size, head_dim] with the same strides and unit stride in
+    head_dim.  A cache laid out token by token inside a page, [n_pages, page_size,
+    n_kv_heads, head_dim], is passed as its ``transpose(1, 2)``."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        for t, name in ((k, "k"), (v, "v")):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise ValueError(f"{name} must be a CUDA tensor")
+            if t.dtype not in _DT_PAGED:
+                raise TypeError(f"{name} has dtype {t.dtype}, expected torch.float16 or torch.bfloat16")
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("k and v must be [n_pages, n_kv_heads, page_size, head_dim] of one type on one GPU")
+        if k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("k and v must have the same strides, with unit stride in head_dim")
+        self.k, self.v = k, v
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        self.desc = _lib.PagedKVDesc(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+                                     _DT_PAGED[k.dtype], self.n_pages, self.page_size, self.n_kv_heads, self.head_dim)
+        self.ptr = ctypes.addressof(self.desc)
+
+    @classmethod
+    def allocate(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=torch.float16,
+                 device="cuda") -> "PagedKV":
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+
+def kv_append_paged(qkv: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, pos: torch.Tensor,
+                    cos: torch.Tensor, sin: torch.Tensor, n_heads: int, seq: torch.Tensor | None = None,
+                    q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, v_norm: bool = False,
+                    eps: float = 1e-6, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Normalise (optionally), rotate and append new tokens to a paged cache
+    (``sb_kv_append_paged``); returns the rotated queries [t, n_heads, head_dim] in the
+    cache's type.
+
+    ``qkv`` [t, (n_heads + 2 n_kv_heads) head_dim] f16, bf16 or f32 (rows may be spaced);
+    ``page_table`` [n_seqs, max_pages] and ``pos`` [t] int32; ``seq`` [t] int32 is each
+    token's row of the page table (None: token i is sequence i, a decode step).
+    ``cos`` / ``sin`` [max_pos, rot/2] f32 rotate values j and j + rot/2 of every q and k
+    head.  A token whose position is negative or past the tables is padding."""
+    dev = cache.device
+    if qkv.dtype not in _DT_ALL:
+        raise TypeError(f"qkv has dtype {qkv.dtype}, expected f16, bf16 or f32")
+    hd = cache.head_dim
+    width = (n_heads + 2 * cache.n_kv_heads) * hd
+    if qkv.dim() != 2 or qkv.shape[1] != width or (qkv.stride(1) != 1) or qkv.device != dev:
+        raise ValueError(f"qkv must be [t, {width}] rows with unit column stride on {dev}")
+    t = qkv.shape[0]
+    _int32(page_table, "page_table", 2, dev)
+    _int32(pos, "pos", 1, dev)
+    if seq is not None:
+        _int32(seq, "seq", 1, dev)
+        if seq.shape[0] != t:
+            raise ValueError("seq must hold one page-table row per token")
+    if pos.shape[0] != t:
+        raise ValueError("pos must hold one position per token")
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise ValueError("cos and sin must be [max_pos, rot / 2]")
+    max_pos, half = cos.shape
+    _f32_vec(cos, "cos", max_pos * half, dev)
+    _f32_vec(sin, "sin", max_pos * half, dev)
+    _f32_vec(q_norm, "q_norm", hd, dev)
+    _f32_vec(k_norm, "k_norm", hd, dev)
+    if q_out is None:
+        q_out = torch.empty((t, n_heads, hd), dtype=cache.dtype, device=dev)
+    elif q_out.dtype != cache.dtype or q_out.shape != (t, n_heads, hd) or not q_out.is_contiguous() or q_out.device != dev:
+        raise ValueError(f"q_out must be a contiguous [{t}, {n_heads}, {hd}] tensor of the cache's type on {dev}")
+    _lib.call("sb_kv_append_paged", cache.ptr, page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
+              qkv.data_ptr(), _DT_ALL[qkv.dtype], qkv.stride(0) if t > 1 else width, t, n_heads, _ptr(seq), pos.data_ptr(), _ptr(q_norm),
+              _ptr(k_norm), int(v_norm), eps, cos.data_ptr(), sin.data_ptr(), 2 * half, max_pos, q_out.data_ptr(),
+              _stream())
+    return q_out
+
+
+def attn_decode_paged_workspace(cache: PagedKV, n_heads: int, batch: int) -> torch.Tensor:
+    """A zeroed workspace for :func:`attn_decode_paged` calls of up to ``batch`` sequences
+    that run one after another; calls that may overlap on the GPU need their own."""
+    n = int(_lib.load().sb_attn_decode_paged_workspace_size(cache.ptr, n_heads, batch))
+    return torch.zeros(max(n, 16), dtype=torch.uint8, device=cache.device)
+
+
+def attn_decode_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, pos: torch.Tensor,
+                      scale: float = 1.0, window: int = 0, out: torch.Tensor | None = None,
+                      workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence over the paged cache
+    (``sb_attn_decode_paged``): q [b, n_heads, head_dim] of the cache's type,
+    ``page_table`` [b, max_pages], ``pos`` [b] int32 = each sequence's last cached
+    position (negative: no key, a zero row); over keys 0..pos, or the last ``window``
+    of them.  ``workspace`` from :func:`attn_decode_paged_workspace`; without one a fresh
+    one is made for the call."""
+    dev = cache.device
+    if q.dtype != cache.dtype:
+        raise TypeError(f"q has dtype {q.dtype}, expected the cache's {cache.dtype}")
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.device != dev or q.stride(2) != 1 or \
+            (q.shape[1] > 1 and q.stride(1) != cache.head_dim):
+        raise ValueError(f"q must be [b, n_heads, {cache.head_dim}] with contiguous rows on {dev}")
+    b, nh, hd = q.shape
+    _int32(page_table, "page_table", 2, dev)
+    _int32(pos, "pos", 1, dev)
+    if page_table.shape[0] != b or pos.shape[0] != b:
+        raise ValueError("page_table and pos must hold one row per sequence")
+    if out is None:
+        out = torch.empty((b, nh, hd), dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != dev:
+        raise ValueError("out must be contiguous and match q")
+    if workspace is None:
+        workspace = attn_decode_paged_workspace(cache, nh, b)
+    _lib.call("sb_attn_decode_paged", cache.ptr, page_table.data_ptr(), page_table.shape[1], pos.data_ptr(), b,
+              q.data_ptr(), q.stride(0) if b > 1 else nh * hd, nh, window, scale, out.data_ptr(),
+              workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
+    return out
