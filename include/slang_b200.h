@@ -39,7 +39,7 @@ extern "C" {
 /* element types */
 #define SB_F16 1
 #define SB_F32 2
-#define SB_BF16 3             /* the paged-cache operators only */
+#define SB_BF16 3             /* the serving operators at the end of this file only */
 #define SB_SCALE_F16 SB_F16
 #define SB_SCALE_F32 SB_F32
 
@@ -636,6 +636,27 @@ int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_table, int m
                          const void* q, int64_t q_stride, int n_heads, int window, float scale, void* out,
                          void* workspace, size_t workspace_bytes, void* stream);
 size_t sb_attn_decode_paged_workspace_size(const sb_paged_kv* kv, int n_heads, int b);
+
+/*
+ * Draw the next token of each row of logits [rows][vocab] (f32, f16 or bf16, row
+ * stride ld; rows <= 65535, vocab <= 819200).  Per row r, each setting a device
+ * array or NULL for "off":
+ *   temperature[r] (off: 1)   w_i = exp((x_i - max x) / T); T <= 0: the largest logit
+ *   top_k[r]       (off: 0)   keep the k largest logits (k <= 0 or k >= vocab: all)
+ *   top_p[r]       (off: 1)   of those keep each whose larger ones sum to less than
+ *                             top_p of their total mass (>= 1: all, <= 0: the first)
+ *   min_p[r]       (off: 0)   of those keep w_i >= min_p (the largest always stays)
+ * Equal logits rank by index, lowest first.  The kept token with the smallest
+ * E_i / w_i is drawn (ties: lowest index), which is token i with probability
+ * w_i / sum of the kept w; E_i = -log(1 - u_i), u_i = (q_i + 1/2) 2^-32 at most
+ * 1 - 2^-24, q_i word i % 4 of Philox4x32-10 with key (low, high) of seeds[r] and
+ * counter (i / 4, pos[r], 0, 0): the same seed, position and logits always draw
+ * the same token, whatever else is in the batch.  NaN counts as -inf; tokens[r]
+ * = -1 when every logit is -inf.  No counterpart in the reference (greedy only).
+ */
+int sb_sample(const void* logits, int dtype, int64_t ld, int rows, int vocab, const int64_t* seeds,
+              const int32_t* pos, const float* temperature, const int32_t* top_k, const float* top_p,
+              const float* min_p, int32_t* tokens, void* stream);
 
 #ifdef __cplusplus
 }

@@ -724,3 +724,42 @@ def attn_decode_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
               q.data_ptr(), q.stride(0) if b > 1 else nh * hd, nh, window, scale, out.data_ptr(),
               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
     return out
+
+
+def sample(logits: torch.Tensor, seeds: torch.Tensor, pos: torch.Tensor, temperature: torch.Tensor | None = None,
+           top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
+           tokens: torch.Tensor | None = None) -> torch.Tensor:
+    """Draw one token per row of ``logits`` [rows, vocab] (``sb_sample``): temperature, then
+    top-k, then top-p, then min-p, each a per-row tensor on the device or None for off.
+    ``seeds`` [rows] int64 and ``pos`` [rows] int32 decide the draw: the same seed,
+    position and logits give the same token.  Returns int32 tokens, -1 for a row whose
+    logits are all -inf."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor")
+    if logits.dtype not in _DT_ALL:
+        raise TypeError(f"logits has dtype {logits.dtype}, expected f16, bf16 or f32")
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [rows, vocab] with unit column stride")
+    dev = logits.device
+    rows, vocab = logits.shape
+    if seeds.dtype != torch.int64 or seeds.shape != (rows,) or not seeds.is_contiguous() or seeds.device != dev:
+        raise ValueError(f"seeds must hold {rows} contiguous int64 values on {dev}")
+    _int32(pos, "pos", 1, dev)
+    if top_k is not None:
+        _int32(top_k, "top_k", 1, dev)
+    for t, name in ((pos, "pos"), (top_k, "top_k")):
+        if t is not None and t.shape[0] != rows:
+            raise ValueError(f"{name} must hold one value per row")
+    _f32_vec(temperature, "temperature", rows, dev)
+    _f32_vec(top_p, "top_p", rows, dev)
+    _f32_vec(min_p, "min_p", rows, dev)
+    if tokens is None:
+        tokens = torch.empty(rows, dtype=torch.int32, device=dev)
+    else:
+        _int32(tokens, "tokens", 1, dev)
+        if tokens.shape[0] != rows:
+            raise ValueError("tokens must hold one value per row")
+    _lib.call("sb_sample", logits.data_ptr(), _DT_ALL[logits.dtype], logits.stride(0) if rows > 1 else vocab, rows,
+              vocab, seeds.data_ptr(), pos.data_ptr(), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+              tokens.data_ptr(), _stream())
+    return tokens
