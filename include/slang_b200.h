@@ -638,6 +638,28 @@ int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_table, int m
 size_t sb_attn_decode_paged_workspace_size(const sb_paged_kv* kv, int n_heads, int b);
 
 /*
+ * Causal attention of packed prompts on tcgen05: sequence i has q_lens[i] rows of
+ * q and out and kv_lens[i] rows of k and v, the sequences end to end.  Its query
+ * j stands at position kv_lens[i] - q_lens[i] + j and sees the keys up to its own
+ * position, the last `window` of them when window > 0; a query that sees none
+ * gives zeros.  out = softmax(scale * q . K) V, scale > 0; f16 or bf16, head_dim in
+ * {64, 128, 256}, any number of query heads per kv head up to 128.  q [t_q][n_heads],
+ * k and v [t_k][n_kv_heads] and out [t_q][n_heads] rows of head_dim lie *_token and
+ * *_head elements apart (multiples of 8, k and v alike).  What lies in rows of
+ * other sequences, NaN included, changes nothing.
+ * tiles: device copy of what sb_attn_packed_plan wrote for the same lengths, head
+ * counts and head_dim (host arrays; tiles NULL: the count alone; kv_lens NULL: as
+ * q_lens; 8 int32 per tile; `window` only orders them, longest first).  A plan
+ * serves every layer of the batch.
+ */
+int sb_attn_packed_plan(const int32_t* q_lens, const int32_t* kv_lens, int n, int n_heads, int n_kv_heads,
+                        int head_dim, int window, int32_t* tiles, int max_tiles, int* n_tiles);
+int sb_attn_prefill_packed(const void* q, int64_t q_token, int64_t q_head, const void* k, const void* v,
+                           int64_t k_token, int64_t k_head, void* out, int64_t out_token, int64_t out_head, int dtype,
+                           int t_q, int t_k, int n_heads, int n_kv_heads, int head_dim, int window, float scale,
+                           const int32_t* tiles, int n_tiles, void* stream);
+
+/*
  * Draw the next token of each row of logits [rows][vocab] (f32, f16 or bf16, row
  * stride ld; rows <= 65535, vocab <= 819200).  Per row r, each setting a device
  * array or NULL for "off":

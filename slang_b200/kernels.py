@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -724,6 +725,60 @@ def attn_decode_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
               q.data_ptr(), q.stride(0) if b > 1 else nh * hd, nh, window, scale, out.data_ptr(),
               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
     return out
+
+
+class PackedPlan:
+    """The query tiles of a packed batch of prompts for :func:`attn_prefill_packed`, made
+    once per batch (host lengths) and shared by its layers.  ``kv_lens`` longer than
+    ``q_lens``: the sequences' first keys come from a cached prefix."""
+
+    def __init__(self, q_lens, n_heads: int, n_kv_heads: int, head_dim: int, kv_lens=None, window: int = 0,
+                 device="cuda"):
+        q = np.ascontiguousarray(q_lens, dtype=np.int32)
+        k = q if kv_lens is None else np.ascontiguousarray(kv_lens, dtype=np.int32)
+        if q.ndim != 1 or k.shape != q.shape:
+            raise ValueError("q_lens and kv_lens must be lists of the same length")
+        n = ctypes.c_int(0)
+        args = (q.ctypes.data, k.ctypes.data, q.size, n_heads, n_kv_heads, head_dim, window)
+        _lib.call("sb_attn_packed_plan", *args, None, 0, ctypes.addressof(n))
+        tiles = np.zeros((n.value, 8), dtype=np.int32)
+        _lib.call("sb_attn_packed_plan", *args, tiles.ctypes.data, n.value, ctypes.addressof(n))
+        self.n_tiles = n.value
+        self.tiles = torch.from_numpy(tiles).to(device)
+        self.total_q, self.total_k = int(q.sum()), int(k.sum())
+        self.n_heads, self.n_kv_heads, self.head_dim, self.window = n_heads, n_kv_heads, head_dim, window
+
+
+def attn_prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan, scale: float = 1.0,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed prompts (``sb_attn_prefill_packed``): q [total_q, n_heads,
+    head_dim], k, v [total_k, n_kv_heads, head_dim] f16 or bf16, each sequence's queries
+    aligned with the end of its keys, the plan's window; returns [total_q, n_heads,
+    head_dim].  Tokens and heads may be spaced."""
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise ValueError("q must be a CUDA tensor")
+    if q.dtype not in _DT_PAGED or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must all be f16 or all be bf16")
+    dev, nh, nkv, hd = q.device, plan.n_heads, plan.n_kv_heads, plan.head_dim
+    if q.shape != (plan.total_q, nh, hd) or q.stride(2) != 1:
+        raise ValueError(f"q must be [{plan.total_q}, {nh}, {hd}] with unit stride in head_dim")
+    if k.shape != (plan.total_k, nkv, hd) or v.shape != k.shape or k.stride() != v.stride() or k.stride(2) != 1:
+        raise ValueError(f"k and v must be [{plan.total_k}, {nkv}, {hd}] with the same strides, unit in head_dim")
+    if k.device != dev or v.device != dev or plan.tiles.device != dev:
+        raise ValueError(f"k, v and the plan must be on {dev}")
+    if out is None:
+        out = torch.empty((plan.total_q, nh, hd), dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.device != dev:
+        raise ValueError("out must match q, with unit stride in head_dim")
+    _lib.call("sb_attn_prefill_packed", q.data_ptr(), _step(q, 0), _step(q, 1), k.data_ptr(), v.data_ptr(), _step(k, 0),
+              _step(k, 1), out.data_ptr(), _step(out, 0), _step(out, 1), _DT_PAGED[q.dtype], plan.total_q, plan.total_k,
+              nh, nkv, hd, plan.window, scale, plan.tiles.data_ptr(), plan.n_tiles, _stream())
+    return out
+
+
+def _step(t: torch.Tensor, dim: int) -> int:
+    """Stride of a dimension; that of a dimension of one says nothing, so the rows' own width stands in."""
+    return t.stride(dim) if t.shape[dim] > 1 else t.shape[2]
 
 
 def sample(logits: torch.Tensor, seeds: torch.Tensor, pos: torch.Tensor, temperature: torch.Tensor | None = None,
