@@ -18,7 +18,15 @@
 // Bound by reading the logits once.  A row belongs to one thread-block cluster
 // that holds it in shared memory, a slice per CTA; every later pass reads the
 // slices, and the CTAs exchange a few words each through distributed shared
-// memory.
+// memory.  What the passes cost is kept small by working on short lists:
+//   min-p, top-p  a token below w = min_p is out, and so is one below (1 - p) / V of
+//                 the total: all such tokens together weigh less than 1 - p, so
+//                 the prefix above them already holds the nucleus.
+//   top-k         the k-th largest of the threads' own maxima is a lower bound of
+//                 the k-th largest value; what reaches it (a little more than
+//                 k tokens) is sorted by one CTA, which finishes the row alone.
+// Masses are added as integers (w in units of 2^-40), so no order of addition
+// shows in the result.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -28,6 +36,11 @@ namespace {
 constexpr int NT = 512;       // threads per CTA
 constexpr int MAX_CS = 16;    // CTAs per row
 constexpr int MAX_SLICE = 51200;  // values per CTA: 200 KB
+constexpr int BINS = 256;     // of the threads' maxima, 1/8 octave of w each
+constexpr int SORT = 1024;    // candidates of a top-k row that one CTA sorts
+constexpr int LIST = 4608;    // candidates per CTA of other rows (16-bit offsets into the slice)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kUnit = 1099511627776.f;  // 2^40
 
 struct SampleParams {
   const void* x;
@@ -49,20 +62,32 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// What the CTAs of a cluster exchange in one step.
+// What the CTAs of a cluster exchange in one step: a sum, the smallest key with
+// a value that goes with it, and a count with the part that lower ranks hold.
 struct Word {
-  double sum;
-  unsigned long long key;
-  unsigned int count, pad;
+  unsigned long long sum, key;
+  unsigned int aux, count;
 };
 
 struct Shared {
-  Word slot[3];        // this CTA's contribution, in turn
+  Word slot[2];        // this CTA's contribution, in turn
   Word warp[NT / 32];
   Word all;
+  unsigned int lower;  // the count in CTAs of lower rank
+  unsigned int n;      // entries of this CTA's list
+  int bin;
+  unsigned int hist[BINS];
+  union {
+    uint16_t list[LIST];
+    struct {
+      unsigned long long keys[SORT];  // of the whole row, in the CTA of rank 0
+      uint16_t mine[SORT / 2];
+    } top;
+  };
 };
+static_assert(sizeof(Shared) <= 11 * 1024, "three CTAs of 64 KB slices per SM");
 
-// One counter word quadruple of Philox4x32-10.
+// One counter's four words of Philox4x32-10.
 __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t k0, uint32_t k1) {
   uint32_t c2 = 0, c3 = 0;
 #pragma unroll
@@ -78,199 +103,357 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t k0, u
   return make_uint4(c0, c1, c2, c3);
 }
 
-// Adds sums and counts and takes the smallest key over the cluster.  `turn`
-// counts the calls: three slots in turn, so that one barrier per call is
-// enough (a CTA can be at most one call ahead of another's reads).
-__device__ Word reduce(Shared& sh, double sum, unsigned long long key, unsigned int count, int cs, int& turn) {
+__device__ __forceinline__ void join(Word& w, const Word& o) {
+  w.sum += o.sum;
+  if (o.key < w.key) w.key = o.key, w.aux = o.aux;
+  w.count += o.count;
+}
+__device__ __forceinline__ Word shfl(const Word& w, int o) {
+  return Word{__shfl_xor_sync(0xFFFFFFFFu, w.sum, o), __shfl_xor_sync(0xFFFFFFFFu, w.key, o),
+              __shfl_xor_sync(0xFFFFFFFFu, w.aux, o), __shfl_xor_sync(0xFFFFFFFFu, w.count, o)};
+}
+
+// Joins the words of all threads of the cluster (keys differ, or are ~0).  Two
+// slots in turn: a CTA writes one again only after a barrier that every other
+// CTA reaches once it has read it.
+__device__ Word reduce(Shared& sh, Word w, int cs, int& turn) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    const unsigned long long k = __shfl_xor_sync(0xFFFFFFFFu, key, o);
-    key = k < key ? k : key;
-    count += __shfl_xor_sync(0xFFFFFFFFu, count, o);
-  }
-  if (lane == 0) sh.warp[warp] = Word{sum, key, count, 0};
+  for (int o = 16; o >= 1; o >>= 1) join(w, shfl(w, o));
+  if (lane == 0) sh.warp[warp] = w;
   __syncthreads();
   if (warp == 0) {
-    Word w = lane < NT / 32 ? sh.warp[lane] : Word{0.0, ~0ull, 0u, 0u};
+    w = lane < NT / 32 ? sh.warp[lane] : Word{0, ~0ull, 0, 0};
 #pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) {
-      w.sum += __shfl_xor_sync(0xFFFFFFFFu, w.sum, o);
-      const unsigned long long k = __shfl_xor_sync(0xFFFFFFFFu, w.key, o);
-      w.key = k < w.key ? k : w.key;
-      w.count += __shfl_xor_sync(0xFFFFFFFFu, w.count, o);
+    for (int o = 8; o >= 1; o >>= 1) join(w, shfl(w, o));
+    if (lane == 0) {
+      (cs > 1 ? sh.slot[turn] : sh.all) = w;
+      sh.lower = 0;
     }
-    if (lane == 0) (cs > 1 ? sh.slot[turn] : sh.all) = w;
   }
   if (cs > 1) {
     sbd::cluster_sync_all();
     if (warp == 0) {
-      Word w{0.0, ~0ull, 0u, 0u};
+      w = Word{0, ~0ull, 0, 0};
       if (lane < cs) {
         const uint32_t a = sbd::mapa_shared(sbd::smem_u32(&sh.slot[turn]), lane);
-        uint32_t lo, hi;
-        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(w.sum) : "r"(a) : "memory");
-        asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(lo), "=r"(hi) : "r"(a + 8) : "memory");
-        w.key = static_cast<unsigned long long>(hi) << 32 | lo;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w.count) : "r"(a + 16) : "memory");
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(w.sum) : "r"(a) : "memory");
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(w.key) : "r"(a + 8) : "memory");
+        asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(w.aux), "=r"(w.count) : "r"(a + 16) : "memory");
       }
+      unsigned int lower = lane < static_cast<int>(sbd::cluster_ctarank()) ? w.count : 0;
 #pragma unroll
-      for (int o = 8; o >= 1; o >>= 1) {  // every CTA adds in the same order
-        w.sum += __shfl_xor_sync(0xFFFFFFFFu, w.sum, o);
-        const unsigned long long k = __shfl_xor_sync(0xFFFFFFFFu, w.key, o);
-        w.key = k < w.key ? k : w.key;
-        w.count += __shfl_xor_sync(0xFFFFFFFFu, w.count, o);
+      for (int o = 8; o >= 1; o >>= 1) {
+        join(w, shfl(w, o));
+        lower += __shfl_xor_sync(0xFFFFFFFFu, lower, o);
       }
-      if (lane == 0) sh.all = w;
+      if (lane == 0) sh.all = w, sh.lower = lower;
     }
-    turn = turn == 2 ? 0 : turn + 1;
+    turn ^= 1;
   }
   __syncthreads();
   return sh.all;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
-  extern __shared__ float xs[];  // this CTA's slice of the row, NaN as -inf, padded with -inf to a multiple of 4
+__global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
+  extern __shared__ __align__(16) float xs[];  // this CTA's slice of the row, NaN as -inf, padded with -inf to a multiple of 4
   __shared__ Shared sh;
   const int cs = gridDim.x, rank = blockIdx.x, row = blockIdx.y;  // a cluster spans the x axis
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   sbd::griddep_launch_dependents();
+  if (threadIdx.x < BINS) sh.hist[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.n = 0;
   sbd::griddep_wait();
+  const float temp = p.temperature ? p.temperature[row] : 1.f;
+  const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
+  const int top_k = p.top_k ? p.top_k[row] : 0;
   const int first = rank * p.slice, n = max(0, min(p.slice, p.v - first)), n4 = (n + 3) / 4;
   const T* src = static_cast<const T*>(p.x) + row * p.ld + first;
   int turn = 0;
 
-  // ---- the slice into shared memory; the largest value, ties to the lowest index
-  unsigned long long best = ~0ull;
-  for (int i = threadIdx.x; i < n4; i += NT) {
-    float v[4];
-    if (p.vec && 4 * i + 4 <= n) {
-      if constexpr (sizeof(T) == 4) {
-        const uint4 r = sbd::ldg_nc_v4(src + 4 * i);
-        v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
-      } else {
-        const uint2 r = __ldg(reinterpret_cast<const uint2*>(src + 4 * i));
-        const float2 a = sbp::unpack2<T>(r.x), b = sbp::unpack2<T>(r.y);
-        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = 4 * i + e < n ? static_cast<float>(src[4 * i + e]) : -INFINITY;
-    }
+  // ---- the slice into shared memory; this thread's largest value, ties to the lowest index
+  float tmax = -INFINITY;
+  int tidx = -1;
+  auto take = [&](int i, float4 f) {
+    float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = v[e] != v[e] ? -INFINITY : v[e] + 0.f;  // -0 ranks with 0
-      const unsigned long long key = static_cast<unsigned long long>(~sbd::orderable(v[e])) << 32 | static_cast<uint32_t>(first + 4 * i + e);
-      best = 4 * i + e < n && key < best ? key : best;
+      if (v[e] > tmax) tmax = v[e], tidx = 4 * i + e;
     }
     *reinterpret_cast<float4*>(xs + 4 * i) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-  best = reduce(sh, 0.0, best, 0, cs, turn).key;
-  const uint32_t mx_bits = ~static_cast<uint32_t>(best >> 32);
-  const float mx = __uint_as_float(mx_bits & 0x80000000u ? mx_bits & 0x7FFFFFFFu : ~mx_bits);
-  const float temp = p.temperature ? p.temperature[row] : 1.f;
-  const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
-  const int top_k = p.top_k ? p.top_k[row] : 0;
-  int token;
-  if (mx == -INFINITY) {
-    token = -1;  // no token may be drawn
-  } else if (!(temp > 0.f) || top_p <= 0.f || top_k == 1) {
-    token = static_cast<int>(best & 0xFFFFFFFFu);
-  } else {
-    // distance below the maximum in units of the temperature (0 for the maximum itself, whatever its size)
-    auto z_of = [&](float x) { return x == mx ? 0.f : (x - mx) / temp; };
-    constexpr float kLog2e = 1.4426950408889634f;
-    const float inv = kLog2e / temp;
-    auto w_fast = [&](float x) { return x == mx ? 1.f : ex2((x - mx) * inv); };
-
-    // ---- top-k: the rank's last member (xk, ik); a token is in when it does not rank behind it
-    uint32_t xk = 0;  // orderable bits
-    int ik = p.v;
-    if (top_k > 0 && top_k < p.v) {
-      // the largest key that at least top_k values reach, bit by bit
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = xk | 1u << bit;
-        unsigned int cnt = 0;
-        for (int i = threadIdx.x; i < n; i += NT) cnt += sbd::orderable(xs[i]) >= c;
-        if (reduce(sh, 0.0, ~0ull, cnt, cs, turn).count >= static_cast<unsigned int>(top_k)) xk = c;
-      }
-      unsigned int cnt = 0;
-      for (int i = threadIdx.x; i < n; i += NT) cnt += sbd::orderable(xs[i]) > xk;
-      const unsigned int above = reduce(sh, 0.0, ~0ull, cnt, cs, turn).count;
-      // of those equal to it the lowest indices: the smallest index bound that lets enough of them in
-      int lo = 0, hi = p.v - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        cnt = 0;
-        for (int i = threadIdx.x; i < n && first + i <= mid; i += NT) cnt += sbd::orderable(xs[i]) == xk;
-        if (above + reduce(sh, 0.0, ~0ull, cnt, cs, turn).count >= static_cast<unsigned int>(top_k)) hi = mid;
-        else lo = mid + 1;
-      }
-      ik = lo;
+  };
+  auto quad = [&](int i) {
+    if constexpr (sizeof(T) == 4) {
+      const uint4 r = sbd::ldg_nc_v4(src + 4 * i);
+      return make_float4(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), __uint_as_float(r.w));
+    } else {
+      const uint2 r = __ldg(reinterpret_cast<const uint2*>(src + 4 * i));
+      const float2 a = sbp::unpack2<T>(r.x), b = sbp::unpack2<T>(r.y);
+      return make_float4(a.x, a.y, b.x, b.y);
     }
-    auto before = [](uint32_t a, int ia, uint32_t b, int ib) { return a > b || (a == b && ia < ib); };
+  };
+  int i0 = threadIdx.x;
+  if (p.vec) {
+    constexpr int U = 8;  // vectors in flight per thread
+    for (; i0 + (U - 1) * NT < n / 4; i0 += U * NT) {
+      float4 f[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) f[u] = quad(i0 + u * NT);
+#pragma unroll
+      for (int u = 0; u < U; ++u) take(i0 + u * NT, f[u]);
+    }
+    for (; i0 < n / 4; i0 += NT) take(i0, quad(i0));
+  }
+  for (; i0 < n4; i0 += NT) {
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = 4 * i0 + e < n ? static_cast<float>(src[4 * i0 + e]) : -INFINITY;
+    take(i0, make_float4(v[0], v[1], v[2], v[3]));
+  }
+  Word w0{0, ~0ull, 0, 0};
+  if (tidx >= 0) w0.key = static_cast<unsigned long long>(~sbd::orderable(tmax)) << 32 | static_cast<uint32_t>(first + tidx), w0.aux = __float_as_uint(tmax);
+  w0 = reduce(sh, w0, cs, turn);
+  int token = static_cast<int>(w0.key & 0xFFFFFFFFu);  // -1 when no value is above -inf
+  const float mx = __uint_as_float(w0.aux);
+  if (w0.key == ~0ull || !(temp > 0.f) || top_p <= 0.f || top_k == 1) {
+    if (rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
+    if (cs > 1) sbd::cluster_sync_all();  // no CTA leaves while another may read its slot
+    return;
+  }
+  const uint32_t k0 = static_cast<uint32_t>(p.seeds[row]), k1 = static_cast<uint32_t>(p.seeds[row] >> 32);
+  const uint32_t c1 = static_cast<uint32_t>(p.pos[row]);
+  // log2 of w, and w; the maximum has 0 and 1 whatever its size
+  const float inv = kLog2e / temp;
+  auto z2_of = [&](float x) { return x == mx ? 0.f : (x - mx) * inv; };
+  // race key of a token with random word q: its waiting time over its rate, then its index; ~0 below min_p
+  auto race = [&](float x, int idx, uint32_t q) {
+    const float wx = expf(x == mx ? 0.f : (x - mx) / temp);
+    if (!(wx >= min_p && wx > 0.f) && x != mx) return ~0ull;
+    const float u = fminf((__uint2float_rn(q) + 0.5f) * 2.3283064365386963e-10f, 0.99999994f);
+    return static_cast<unsigned long long>(__float_as_uint(-log1pf(-u) / wx)) << 32 | static_cast<uint32_t>(idx);
+  };
+  auto word_of = [&](int idx) {
+    const uint4 r = philox(static_cast<uint32_t>(idx) >> 2, c1, k0, k1);
+    const uint32_t lo = idx & 1 ? r.y : r.x, hi = idx & 1 ? r.w : r.z;
+    return idx & 2 ? hi : lo;
+  };
+  // offsets of this CTA's values that `in` holds for into list[cap]; sh.n counts them all
+  auto collect = [&](uint16_t* list, int cap, auto in) {
+    for (int i = threadIdx.x - lane; i < n; i += NT) {  // whole warps
+      const bool hit = i + lane < n && in(xs[i + lane], i + lane);
+      const unsigned vote = __ballot_sync(0xFFFFFFFFu, hit);
+      if (!vote) continue;
+      unsigned base = 0;
+      if (lane == 0) base = atomicAdd(&sh.n, static_cast<unsigned>(__popc(vote)));
+      base = __shfl_sync(0xFFFFFFFFu, base, 0) + __popc(vote & ((1u << lane) - 1));
+      if (hit && base < static_cast<unsigned>(cap)) list[base] = static_cast<uint16_t>(i + lane);
+    }
+    __syncthreads();
+  };
 
-    // ---- the race among (x, i) up to and including (xl, il) in rank, and the mass before or up to it
-    uint32_t xl = xk;
-    int il = ik;
-    double total = 0.0;
-    const uint32_t k0 = static_cast<uint32_t>(p.seeds[row]), k1 = static_cast<uint32_t>(p.seeds[row] >> 32);
-    const uint32_t c1 = static_cast<uint32_t>(p.pos[row]);
-    for (int round = 0;; ++round) {
+  uint32_t xl = 0;  // the race is among tokens that rank before (xl, il): orderable value, index
+  int il = p.v;
+  if (top_k > 0 && top_k < p.v) {
+    // ---- top-k: the bin of the threads' maxima that reaches k; every value in it or above is a candidate
+    auto bin_of = [&](float x) { return static_cast<int>(fminf(-8.f * z2_of(x), static_cast<float>(BINS - 1))); };
+    if (tidx >= 0) atomicAdd(&sh.hist[bin_of(tmax)], 1u);
+    __syncthreads();
+    if (cs > 1) sbd::cluster_sync_all();
+    unsigned cnt = 0;
+    if (threadIdx.x < BINS) {
+      if (cs > 1) {
+        for (int r = 0; r < cs; ++r) {
+          unsigned c;
+          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(sbd::mapa_shared(sbd::smem_u32(&sh.hist[threadIdx.x]), r)) : "memory");
+          cnt += c;
+        }
+      } else {
+        cnt = sh.hist[threadIdx.x];
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned c = __shfl_up_sync(0xFFFFFFFFu, cnt, o);
+        if (lane >= o) cnt += c;
+      }
+      if (lane == 31) sh.warp[warp].count = cnt;
+    }
+    if (threadIdx.x == 0) sh.bin = BINS - 1;  // too few maxima: everything
+    __syncthreads();
+    if (threadIdx.x < BINS) {
+      unsigned before = 0;
+      for (int x = 0; x < warp; ++x) before += sh.warp[x].count;
+      const unsigned up = __shfl_up_sync(0xFFFFFFFFu, cnt, 1);
+      const unsigned k = static_cast<unsigned>(top_k);
+      if (before + cnt >= k && (lane ? before + up : before) < k) sh.bin = threadIdx.x;
+    }
+    __syncthreads();
+    const int bin = sh.bin;
+    collect(sh.top.mine, SORT / 2, [&](float x, int) { return bin == BINS - 1 || bin_of(x) <= bin; });
+    const unsigned mine = sh.n;  // a list that does not fit counts as too many candidates
+    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : mine > SORT / 2 ? SORT + 1u : mine}, cs, turn).count;
+    if (total <= SORT) {
+      auto key_of = [&](int i) { return static_cast<unsigned long long>(~sbd::orderable(xs[i])) << 32 | static_cast<uint32_t>(first + i); };
+      const unsigned at = sh.lower;
+      if (cs > 1) {
+        const uint32_t dst = sbd::mapa_shared(sbd::smem_u32(sh.top.keys), 0);
+        for (unsigned i = threadIdx.x; i < mine; i += NT)
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst + 8 * (at + i)), "l"(key_of(sh.top.mine[i])) : "memory");
+        sbd::cluster_sync_all();
+        if (rank) return;  // from here on nobody reads this CTA's memory
+      } else {
+        for (unsigned i = threadIdx.x; i < mine; i += NT) sh.top.keys[i] = key_of(sh.top.mine[i]);
+      }
+      unsigned size = 2;
+      while (size < total) size *= 2;
+      for (unsigned i = total + threadIdx.x; i < size; i += NT) sh.top.keys[i] = ~0ull;
+      __syncthreads();
+      unsigned long long* key = sh.top.keys;
+      for (unsigned k = 2; k <= size; k *= 2)  // bitonic
+        for (unsigned j = k / 2; j; j /= 2) {
+          if (threadIdx.x < size / 2) {
+            const unsigned a = 2 * j * (threadIdx.x / j) + threadIdx.x % j, b = a + j;
+            const unsigned long long ka = key[a], kb = key[b];
+            if ((ka > kb) == !(a & k)) key[a] = kb, key[b] = ka;
+          }
+          __syncthreads();
+        }
+      // ranks 2 t and 2 t + 1 are this thread's; the mass before each
+      float x[2] = {-INFINITY, -INFINITY};
+      int idx[2] = {0, 0};
+      unsigned long long mass[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned r = 2 * threadIdx.x + e;
+        if (r < total && r < static_cast<unsigned>(top_k)) {
+          const uint32_t o = ~static_cast<uint32_t>(key[r] >> 32);
+          x[e] = __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+          idx[e] = static_cast<int>(key[r] & 0xFFFFFFFFu);
+          mass[e] = __float2ull_rn(ex2(z2_of(x[e])) * kUnit);
+        }
+      }
+      unsigned long long inc = mass[0] + mass[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) sh.warp[warp].sum = inc;
+      __syncthreads();
+      unsigned long long before = inc - mass[0] - mass[1], all = 0;
+      for (int r = 0; r < NT / 32; ++r) {
+        const unsigned long long v = sh.warp[r].sum;
+        before += r < warp ? v : 0;
+        all += v;
+      }
+      __syncthreads();
+      const double limit = static_cast<double>(top_p) * static_cast<double>(all);
+      Word best{0, ~0ull, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (x[e] > -INFINITY && (top_p >= 1.f || static_cast<double>(before) < limit)) best.key = min(best.key, race(x[e], idx[e], word_of(idx[e])));
+        before += mass[e];
+      }
+      int none = 0;
+      best = reduce(sh, best, 1, none);
+      if (threadIdx.x == 0) p.tokens[row] = static_cast<int>(best.key & 0xFFFFFFFFu);
+      return;
+    }
+    // more candidates than one CTA sorts (a large k, or thousands of equal values): the largest value that at
+    // least top_k values reach, bit by bit, then the index up to which those equal to it are in
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t c = xl | 1u << bit;
+      unsigned cnt = 0;
+      for (int i = threadIdx.x; i < n; i += NT) cnt += sbd::orderable(xs[i]) >= c;
+      if (reduce(sh, Word{0, ~0ull, 0, cnt}, cs, turn).count >= static_cast<unsigned>(top_k)) xl = c;
+    }
+    unsigned above = 0;
+    for (int i = threadIdx.x; i < n; i += NT) above += sbd::orderable(xs[i]) > xl;
+    above = reduce(sh, Word{0, ~0ull, 0, above}, cs, turn).count;
+    int lo = 0, hi = p.v - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      unsigned cnt = 0;
+      for (int i = threadIdx.x; i < n && first + i <= mid; i += NT) cnt += sbd::orderable(xs[i]) == xl;
+      if (above + reduce(sh, Word{0, ~0ull, 0, cnt}, cs, turn).count >= static_cast<unsigned>(top_k)) hi = mid;
+      else lo = mid + 1;
+    }
+    il = lo + 1;  // ranks before (xl, il): the k in
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+  }
+
+  // ---- the race among the tokens that rank before (xl, il)
+  auto in = [&](float x, int idx) {
+    const uint32_t o = sbd::orderable(x);
+    return o > xl || (o == xl && idx < il);
+  };
+  // log2 of the smallest w that can be kept (see above; the margin covers the arithmetic of both sides)
+  float cut = min_p > 0.f ? __log2f(min_p) - 0.01f : -INFINITY;
+  if (top_p < 1.f) cut = fmaxf(cut, __log2f((1.f - top_p) / static_cast<float>(p.v)) - 0.01f);
+  bool listed = false;
+  Word w{0, ~0ull, 0, 0};
+  if (cut > -INFINITY) {
+    float sum = 0.f;
+    collect(sh.list, LIST, [&](float x, int i) {
+      const float z = z2_of(x);
+      const bool ok = in(x, first + i);
+      sum += ok ? ex2(z) : 0.f;
+      return ok && z >= cut;
+    });
+    w.sum = __float2ull_rn(sum * kUnit);
+    listed = sh.n <= LIST;
+  }
+  double mass = 0.0;
+  for (int round = 0;; ++round) {
+    if (listed) {
+      const unsigned m = sh.n;
+      for (unsigned i = threadIdx.x; i < m; i += NT) {
+        const int at = sh.list[i], idx = first + at;
+        const float x = xs[at];
+        if (round && !in(x, idx)) continue;
+        if (round) w.sum += __float2ull_rn(ex2(z2_of(x)) * kUnit);
+        const unsigned long long k = race(x, idx, word_of(idx));
+        if (k < w.key) w.key = k, w.aux = sbd::orderable(x);
+      }
+    } else {
       float sum = 0.f;
-      unsigned long long win = ~0ull;
       for (int i = threadIdx.x; i < n4; i += NT) {
         const float4 f = *reinterpret_cast<const float4*>(xs + 4 * i);
         const float v[4] = {f.x, f.y, f.z, f.w};
-        bool in[4], any = false;
+        bool run[4], any = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t o = sbd::orderable(v[e]);
-          const int idx = first + 4 * i + e;
-          in[e] = 4 * i + e < n && (before(o, idx, xl, il) || (round == 0 && o == xl && idx == il));
-          const float w = in[e] ? w_fast(v[e]) : 0.f;
-          sum += w;
-          in[e] = in[e] && w > 0.f;
-          any |= in[e];
+          const float z = z2_of(v[e]);
+          run[e] = v[e] > -INFINITY && in(v[e], first + 4 * i + e);
+          sum += run[e] ? ex2(z) : 0.f;
+          run[e] = run[e] && z >= cut;
+          any |= run[e];
         }
         if (!any) continue;
         const uint4 r = philox(static_cast<uint32_t>(first / 4 + i), c1, k0, k1);
-        const uint32_t word[4] = {r.x, r.y, r.z, r.w};
+        const uint32_t q[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (!in[e]) continue;
-          const float w = expf(z_of(v[e]));
-          if (!(w >= min_p) && v[e] != mx) continue;  // min-p never drops the maximum
-          const float u = fminf((__uint2float_rn(word[e]) + 0.5f) * 2.3283064365386963e-10f, 0.99999994f);
-          const float t = -log1pf(-u) / w;
-          const unsigned long long key = static_cast<unsigned long long>(__float_as_uint(t)) << 32 | static_cast<uint32_t>(first + 4 * i + e);
-          win = key < win ? key : win;
+          if (!run[e]) continue;
+          const unsigned long long k = race(v[e], first + 4 * i + e, q[e]);
+          if (k < w.key) w.key = k, w.aux = sbd::orderable(v[e]);
         }
       }
-      const Word all = reduce(sh, static_cast<double>(sum), win, 0, cs, turn);
-      if (round == 0) {
-        total = all.sum;
-      } else if (all.sum < static_cast<double>(top_p) * total || all.key == ~0ull) {
-        token = il;  // the mass before the last winner is below p of the total: it stands
-        break;
-      }
-      // the winner of this round becomes the bound of the next
-      il = static_cast<int>(all.key & 0xFFFFFFFFu);
-      if (top_p >= 1.f) {
-        token = il;
-        break;
-      }
-      // its value, from the CTA that holds it
-      {
-        const bool mine = threadIdx.x == 0 && il >= first && il < first + n;
-        const unsigned long long bits = mine ? sbd::orderable(xs[il - first]) : ~0ull;
-        xl = static_cast<uint32_t>(reduce(sh, 0.0, bits, 0, cs, turn).key);
-      }
+      if (round) w.sum = __float2ull_rn(sum * kUnit);
     }
+    w = reduce(sh, w, cs, turn);
+    if (round && (w.key == ~0ull || static_cast<double>(w.sum) < static_cast<double>(top_p) * mass)) break;  // the last winner stands
+    token = static_cast<int>(w.key & 0xFFFFFFFFu);
+    if (top_p >= 1.f) break;
+    if (!round) mass = static_cast<double>(w.sum);
+    // next: what ranks before the winner, its mass and the winner among it
+    xl = w.aux, il = token;
+    w = Word{0, ~0ull, 0, 0};
   }
   if (rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
-  if (cs > 1) sbd::cluster_sync_all();  // no CTA leaves while another may read its slots
+  if (cs > 1) sbd::cluster_sync_all();  // no CTA leaves while another may read its slot
 }
 
 template <typename T>
