@@ -38,8 +38,13 @@ constexpr int MAX_CS = 16;    // CTAs per row
 constexpr int MAX_SLICE = 51200;  // values per CTA: 200 KB
 constexpr int BINS = 256;     // of the threads' maxima, 1/8 octave of w each
 constexpr int SORT = 1024;    // candidates of a top-k row that one CTA sorts
-constexpr int LIST = 4608;    // candidates per CTA of other rows (16-bit offsets into the slice)
+constexpr int MINE = 512;     // of those in one slice
+// Candidates per CTA of other rows (16-bit offsets into the slice).  Beyond this
+// many of a 16384-value slice a pass over all of it costs no more: one Philox call
+// serves four values there, one here.
+constexpr int LIST = 3072;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLargest = 3.402823466e38f;  // bounds stay finite: -inf (banned, padding) is below them
 constexpr float kUnit = 1099511627776.f;  // 2^40
 
 struct SampleParams {
@@ -62,6 +67,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Ranking bits of a value; -0 ranks with 0.
+__device__ __forceinline__ uint32_t order_of(float x) { return sbd::orderable(x + 0.f); }
+
 // What the CTAs of a cluster exchange in one step: a sum, the smallest key with
 // a value that goes with it, and a count with the part that lower ranks hold.
 struct Word {
@@ -81,7 +89,7 @@ struct Shared {
     uint16_t list[LIST];
     struct {
       unsigned long long keys[SORT];  // of the whole row, in the CTA of rank 0
-      uint16_t mine[SORT / 2];
+      uint16_t mine[MINE];
     } top;
   };
 };
@@ -103,14 +111,20 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t k0, u
   return make_uint4(c0, c1, c2, c3);
 }
 
-__device__ __forceinline__ void join(Word& w, const Word& o) {
-  w.sum += o.sum;
-  if (o.key < w.key) w.key = o.key, w.aux = o.aux;
-  w.count += o.count;
-}
-__device__ __forceinline__ Word shfl(const Word& w, int o) {
-  return Word{__shfl_xor_sync(0xFFFFFFFFu, w.sum, o), __shfl_xor_sync(0xFFFFFFFFu, w.key, o),
-              __shfl_xor_sync(0xFFFFFFFFu, w.aux, o), __shfl_xor_sync(0xFFFFFFFFu, w.count, o)};
+// The join of a warp's words, in every lane: the 64-bit parts in pieces that the
+// 32-bit warp reductions take (sums below 2^60 in pieces of 20 bits).
+__device__ __forceinline__ Word warp_join(Word w) {
+  constexpr unsigned kAll = 0xFFFFFFFFu;
+  Word r;
+  r.sum = __reduce_add_sync(kAll, static_cast<unsigned>(w.sum & 0xFFFFFu)) +
+          (static_cast<unsigned long long>(__reduce_add_sync(kAll, static_cast<unsigned>(w.sum >> 20 & 0xFFFFFu))) << 20) +
+          (static_cast<unsigned long long>(__reduce_add_sync(kAll, static_cast<unsigned>(w.sum >> 40))) << 40);
+  const unsigned hi = __reduce_min_sync(kAll, static_cast<unsigned>(w.key >> 32));
+  const unsigned lo = __reduce_min_sync(kAll, static_cast<unsigned>(w.key >> 32) == hi ? static_cast<unsigned>(w.key) : ~0u);
+  r.key = static_cast<unsigned long long>(hi) << 32 | lo;
+  r.aux = __shfl_sync(kAll, w.aux, __ffs(__ballot_sync(kAll, w.key == r.key)) - 1);
+  r.count = __reduce_add_sync(kAll, w.count);
+  return r;
 }
 
 // Joins the words of all threads of the cluster (keys differ, or are ~0).  Two
@@ -118,14 +132,11 @@ __device__ __forceinline__ Word shfl(const Word& w, int o) {
 // CTA reaches once it has read it.
 __device__ Word reduce(Shared& sh, Word w, int cs, int& turn) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) join(w, shfl(w, o));
+  w = warp_join(w);
   if (lane == 0) sh.warp[warp] = w;
   __syncthreads();
   if (warp == 0) {
-    w = lane < NT / 32 ? sh.warp[lane] : Word{0, ~0ull, 0, 0};
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) join(w, shfl(w, o));
+    w = warp_join(lane < NT / 32 ? sh.warp[lane] : Word{0, ~0ull, 0, 0});
     if (lane == 0) {
       (cs > 1 ? sh.slot[turn] : sh.all) = w;
       sh.lower = 0;
@@ -141,12 +152,8 @@ __device__ Word reduce(Shared& sh, Word w, int cs, int& turn) {
         asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(w.key) : "r"(a + 8) : "memory");
         asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(w.aux), "=r"(w.count) : "r"(a + 16) : "memory");
       }
-      unsigned int lower = lane < static_cast<int>(sbd::cluster_ctarank()) ? w.count : 0;
-#pragma unroll
-      for (int o = 8; o >= 1; o >>= 1) {
-        join(w, shfl(w, o));
-        lower += __shfl_xor_sync(0xFFFFFFFFu, lower, o);
-      }
+      const unsigned lower = __reduce_add_sync(0xFFFFFFFFu, lane < static_cast<int>(sbd::cluster_ctarank()) ? w.count : 0u);
+      w = warp_join(w);
       if (lane == 0) sh.all = w, sh.lower = lower;
     }
     turn ^= 1;
@@ -168,21 +175,20 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
   const float temp = p.temperature ? p.temperature[row] : 1.f;
   const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
   const int top_k = p.top_k ? p.top_k[row] : 0;
+  const uint32_t k0 = static_cast<uint32_t>(p.seeds[row]), k1 = static_cast<uint32_t>(p.seeds[row] >> 32);
+  const uint32_t c1 = static_cast<uint32_t>(p.pos[row]);
   const int first = rank * p.slice, n = max(0, min(p.slice, p.v - first)), n4 = (n + 3) / 4;
   const T* src = static_cast<const T*>(p.x) + row * p.ld + first;
   int turn = 0;
 
   // ---- the slice into shared memory; this thread's largest value, ties to the lowest index
   float tmax = -INFINITY;
-  int tidx = -1;
+  int tquad = -1;
   auto take = [&](int i, float4 f) {
-    float v[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = v[e] != v[e] ? -INFINITY : v[e] + 0.f;  // -0 ranks with 0
-      if (v[e] > tmax) tmax = v[e], tidx = 4 * i + e;
-    }
-    *reinterpret_cast<float4*>(xs + 4 * i) = make_float4(v[0], v[1], v[2], v[3]);
+    f.x = fmaxf(f.x, -INFINITY), f.y = fmaxf(f.y, -INFINITY), f.z = fmaxf(f.z, -INFINITY), f.w = fmaxf(f.w, -INFINITY);  // NaN
+    const float m = fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w));
+    if (m > tmax) tmax = m, tquad = i;
+    *reinterpret_cast<float4*>(xs + 4 * i) = f;
   };
   auto quad = [&](int i) {
     if constexpr (sizeof(T) == 4) {
@@ -213,7 +219,11 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     take(i0, make_float4(v[0], v[1], v[2], v[3]));
   }
   Word w0{0, ~0ull, 0, 0};
-  if (tidx >= 0) w0.key = static_cast<unsigned long long>(~sbd::orderable(tmax)) << 32 | static_cast<uint32_t>(first + tidx), w0.aux = __float_as_uint(tmax);
+  if (tquad >= 0) {
+    const float4 f = *reinterpret_cast<const float4*>(xs + 4 * tquad);  // this thread's own store
+    const int idx = first + 4 * tquad + (f.x == tmax ? 0 : f.y == tmax ? 1 : f.z == tmax ? 2 : 3);
+    w0.key = static_cast<unsigned long long>(~order_of(tmax)) << 32 | static_cast<uint32_t>(idx), w0.aux = __float_as_uint(tmax);
+  }
   w0 = reduce(sh, w0, cs, turn);
   int token = static_cast<int>(w0.key & 0xFFFFFFFFu);  // -1 when no value is above -inf
   const float mx = __uint_as_float(w0.aux);
@@ -222,11 +232,9 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     if (cs > 1) sbd::cluster_sync_all();  // no CTA leaves while another may read its slot
     return;
   }
-  const uint32_t k0 = static_cast<uint32_t>(p.seeds[row]), k1 = static_cast<uint32_t>(p.seeds[row] >> 32);
-  const uint32_t c1 = static_cast<uint32_t>(p.pos[row]);
-  // log2 of w, and w; the maximum has 0 and 1 whatever its size
-  const float inv = kLog2e / temp;
-  auto z2_of = [&](float x) { return x == mx ? 0.f : (x - mx) * inv; };
+  // log2 of w; fminf gives the maximum itself 0 even where it is infinite (inf - inf)
+  const float inv = fmaxf(kLog2e / temp, 1e-37f);  // above zero, so that -inf stays -inf
+  auto z2_of = [&](float x) { return fminf((x - mx) * inv, 0.f); };
   // race key of a token with random word q: its waiting time over its rate, then its index; ~0 below min_p
   auto race = [&](float x, int idx, uint32_t q) {
     const float wx = expf(x == mx ? 0.f : (x - mx) / temp);
@@ -239,16 +247,41 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     const uint32_t lo = idx & 1 ? r.y : r.x, hi = idx & 1 ? r.w : r.z;
     return idx & 2 ? hi : lo;
   };
-  // offsets of this CTA's values that `in` holds for into list[cap]; sh.n counts them all
-  auto collect = [&](uint16_t* list, int cap, auto in) {
-    for (int i = threadIdx.x - lane; i < n; i += NT) {  // whole warps
-      const bool hit = i + lane < n && in(xs[i + lane], i + lane);
-      const unsigned vote = __ballot_sync(0xFFFFFFFFu, hit);
-      if (!vote) continue;
+  // a value below every x with log2 w >= c, whatever the rounding on either side
+  auto floor_of = [&](float c) { return mx == INFINITY ? kLargest : fmaxf(mx + (c - 0.01f) / inv - fabsf(mx) * 0x1p-21f, -kLargest); };
+  // offsets of this CTA's values of at least `least` into list[cap]; sh.n counts them all.  Up to 32 values
+  // per thread become a bit mask, so that a warp takes its places in the list with one atomic.
+  auto collect = [&](uint16_t* list, int cap, float least, auto also) {
+    for (int i0 = 0; i0 < n4; i0 += 8 * NT) {
+      uint32_t hits = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = i0 + j * NT + threadIdx.x;
+        if (i < n4) {
+          const float4 f = *reinterpret_cast<const float4*>(xs + 4 * i);
+          const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            hits |= v[e] >= least ? 1u << (4 * j + e) : 0u;
+            also(v[e], 4 * i + e);
+          }
+        }
+      }
+      const unsigned mine = __popc(hits);
+      unsigned inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += v;
+      }
       unsigned base = 0;
-      if (lane == 0) base = atomicAdd(&sh.n, static_cast<unsigned>(__popc(vote)));
-      base = __shfl_sync(0xFFFFFFFFu, base, 0) + __popc(vote & ((1u << lane) - 1));
-      if (hit && base < static_cast<unsigned>(cap)) list[base] = static_cast<uint16_t>(i + lane);
+      if (lane == 31 && inc) base = atomicAdd(&sh.n, inc);
+      base = __shfl_sync(0xFFFFFFFFu, base, 31) + inc - mine;
+      if (base + mine > static_cast<unsigned>(cap)) hits = 0;  // the list will not be used
+      for (; hits; hits &= hits - 1, ++base) {
+        const int bit = __ffs(hits) - 1;
+        list[base] = static_cast<uint16_t>(4 * (i0 + (bit >> 2) * NT + threadIdx.x) + (bit & 3));
+      }
     }
     __syncthreads();
   };
@@ -258,7 +291,7 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
   if (top_k > 0 && top_k < p.v) {
     // ---- top-k: the bin of the threads' maxima that reaches k; every value in it or above is a candidate
     auto bin_of = [&](float x) { return static_cast<int>(fminf(-8.f * z2_of(x), static_cast<float>(BINS - 1))); };
-    if (tidx >= 0) atomicAdd(&sh.hist[bin_of(tmax)], 1u);
+    if (tquad >= 0) atomicAdd(&sh.hist[bin_of(tmax)], 1u);
     __syncthreads();
     if (cs > 1) sbd::cluster_sync_all();
     unsigned cnt = 0;
@@ -290,11 +323,11 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     }
     __syncthreads();
     const int bin = sh.bin;
-    collect(sh.top.mine, SORT / 2, [&](float x, int) { return bin == BINS - 1 || bin_of(x) <= bin; });
+    collect(sh.top.mine, MINE, bin == BINS - 1 ? -kLargest : floor_of(-0.125f * (bin + 1)), [](float, int) {});
     const unsigned mine = sh.n;  // a list that does not fit counts as too many candidates
-    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : mine > SORT / 2 ? SORT + 1u : mine}, cs, turn).count;
+    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : mine > MINE ? SORT + 1u : mine}, cs, turn).count;
     if (total <= SORT) {
-      auto key_of = [&](int i) { return static_cast<unsigned long long>(~sbd::orderable(xs[i])) << 32 | static_cast<uint32_t>(first + i); };
+      auto key_of = [&](int i) { return static_cast<unsigned long long>(~order_of(xs[i])) << 32 | static_cast<uint32_t>(first + i); };
       const unsigned at = sh.lower;
       if (cs > 1) {
         const uint32_t dst = sbd::mapa_shared(sbd::smem_u32(sh.top.keys), 0);
@@ -365,17 +398,17 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t c = xl | 1u << bit;
       unsigned cnt = 0;
-      for (int i = threadIdx.x; i < n; i += NT) cnt += sbd::orderable(xs[i]) >= c;
+      for (int i = threadIdx.x; i < n; i += NT) cnt += order_of(xs[i]) >= c;
       if (reduce(sh, Word{0, ~0ull, 0, cnt}, cs, turn).count >= static_cast<unsigned>(top_k)) xl = c;
     }
     unsigned above = 0;
-    for (int i = threadIdx.x; i < n; i += NT) above += sbd::orderable(xs[i]) > xl;
+    for (int i = threadIdx.x; i < n; i += NT) above += order_of(xs[i]) > xl;
     above = reduce(sh, Word{0, ~0ull, 0, above}, cs, turn).count;
     int lo = 0, hi = p.v - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       unsigned cnt = 0;
-      for (int i = threadIdx.x; i < n && first + i <= mid; i += NT) cnt += sbd::orderable(xs[i]) == xl;
+      for (int i = threadIdx.x; i < n && first + i <= mid; i += NT) cnt += order_of(xs[i]) == xl;
       if (above + reduce(sh, Word{0, ~0ull, 0, cnt}, cs, turn).count >= static_cast<unsigned>(top_k)) hi = mid;
       else lo = mid + 1;
     }
@@ -385,61 +418,70 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
   }
 
   // ---- the race among the tokens that rank before (xl, il)
+  bool all = xl == 0;  // every token does
   auto in = [&](float x, int idx) {
-    const uint32_t o = sbd::orderable(x);
+    const uint32_t o = order_of(x);
     return o > xl || (o == xl && idx < il);
   };
-  // log2 of the smallest w that can be kept (see above; the margin covers the arithmetic of both sides)
-  float cut = min_p > 0.f ? __log2f(min_p) - 0.01f : -INFINITY;
-  if (top_p < 1.f) cut = fmaxf(cut, __log2f((1.f - top_p) / static_cast<float>(p.v)) - 0.01f);
+  // log2 of the smallest w that can be kept (see above)
+  float cut = min_p > 0.f ? __log2f(min_p) : -INFINITY;
+  if (top_p < 1.f) cut = fmaxf(cut, __log2f((1.f - top_p) / static_cast<float>(p.v)));
   bool listed = false;
   Word w{0, ~0ull, 0, 0};
   if (cut > -INFINITY) {
     float sum = 0.f;
-    collect(sh.list, LIST, [&](float x, int i) {
-      const float z = z2_of(x);
-      const bool ok = in(x, first + i);
-      sum += ok ? ex2(z) : 0.f;
-      return ok && z >= cut;
-    });
+    const float least = floor_of(cut);
+    if (top_p >= 1.f) collect(sh.list, LIST, least, [](float, int) {});
+    else if (all) collect(sh.list, LIST, least, [&](float x, int) { sum += ex2(z2_of(x)); });
+    else collect(sh.list, LIST, least, [&](float x, int i) { sum += in(x, first + i) ? ex2(z2_of(x)) : 0.f; });
     w.sum = __float2ull_rn(sum * kUnit);
     listed = sh.n <= LIST;
   }
+  // The largest logit's own time bounds the winner's: it is in every race that is not empty.  A token can
+  // only win when E / w <= bound; E >= u, so nearly all are out by u > bound w, two operations and an ex2 (with
+  // a margin over what those are off); the logarithm, the exponential and the division are for the rest.
+  const float bound = __uint_as_float(static_cast<uint32_t>(race(mx, token, word_of(token)) >> 32));
+  const float reach = __log2f(bound) + 32.01f;
+  auto loses = [&](float z2, uint32_t q) { return __uint2float_rn(q) > ex2(z2 + reach); };
   double mass = 0.0;
   for (int round = 0;; ++round) {
+    auto run = [&](float x, int idx, uint32_t q) {
+      const unsigned long long k = race(x, idx, q);
+      if (k < w.key) w.key = k, w.aux = order_of(x);
+    };
     if (listed) {
       const unsigned m = sh.n;
       for (unsigned i = threadIdx.x; i < m; i += NT) {
         const int at = sh.list[i], idx = first + at;
-        const float x = xs[at];
-        if (round && !in(x, idx)) continue;
-        if (round) w.sum += __float2ull_rn(ex2(z2_of(x)) * kUnit);
-        const unsigned long long k = race(x, idx, word_of(idx));
-        if (k < w.key) w.key = k, w.aux = sbd::orderable(x);
+        const float x = xs[at], z = z2_of(x);
+        if (!all) {
+          if (!in(x, idx)) continue;
+          if (round) w.sum += __float2ull_rn(ex2(z) * kUnit);
+        }
+        const uint32_t q = word_of(idx);
+        if (!loses(z, q)) run(x, idx, q);
       }
     } else {
       float sum = 0.f;
       for (int i = threadIdx.x; i < n4; i += NT) {
         const float4 f = *reinterpret_cast<const float4*>(xs + 4 * i);
         const float v[4] = {f.x, f.y, f.z, f.w};
-        bool run[4], any = false;
+        float z[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float z = z2_of(v[e]);
-          run[e] = v[e] > -INFINITY && in(v[e], first + 4 * i + e);
-          sum += run[e] ? ex2(z) : 0.f;
-          run[e] = run[e] && z >= cut;
-          any |= run[e];
+        for (int e = 0; e < 4; ++e) z[e] = z2_of(v[e]);
+        if (!all) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            z[e] = in(v[e], first + 4 * i + e) ? z[e] : -INFINITY;
+            sum += ex2(z[e]);
+          }
+          if (fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])) == -INFINITY) continue;
         }
-        if (!any) continue;
         const uint4 r = philox(static_cast<uint32_t>(first / 4 + i), c1, k0, k1);
         const uint32_t q[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (!run[e]) continue;
-          const unsigned long long k = race(v[e], first + 4 * i + e, q[e]);
-          if (k < w.key) w.key = k, w.aux = sbd::orderable(v[e]);
-        }
+        for (int e = 0; e < 4; ++e)
+          if (!loses(z[e], q[e]) && z[e] > -INFINITY) run(v[e], first + 4 * i + e, q[e]);
       }
       if (round) w.sum = __float2ull_rn(sum * kUnit);
     }
@@ -449,7 +491,7 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     if (top_p >= 1.f) break;
     if (!round) mass = static_cast<double>(w.sum);
     // next: what ranks before the winner, its mass and the winner among it
-    xl = w.aux, il = token;
+    xl = w.aux, il = token, all = false;
     w = Word{0, ~0ull, 0, 0};
   }
   if (rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
