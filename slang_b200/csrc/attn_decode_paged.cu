@@ -34,6 +34,8 @@
 namespace {
 
 constexpr int W = 4;  // warps per CTA
+constexpr int JOIN = 24;  // partials one CTA joins: more than the square root of the grid
+constexpr int MIN_KEYS = 64;  // of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRise = 8.f;  // log2 units: p stays below 2^8
 
@@ -67,7 +69,8 @@ struct DecodeParams {
   void* out;         // [b][nh][hd]
   sbp::Pages pages;
   const int32_t* pos;
-  unsigned int* count;  // [b * nkv * htiles], zero between calls
+  unsigned int* group_count;  // [grid / JOIN + 1][2], zero between calls
+  unsigned int* count;        // [b * nkv * htiles], zero between calls
   float* part;          // [grid][2][HT * (hd + 2)]
   int b, nkv, group, htiles, window;  // htiles: tiles of HT query heads per kv head
   float scale2;                       // scale * log2(e)
@@ -88,13 +91,14 @@ __device__ __forceinline__ void key_range(const DecodeParams& p, int b, int* lo,
 template <typename T, int HD, int HS, int NT>
 struct Shape {
   static constexpr int HDW = HD / HS;
-  static constexpr int NS = 256 / HDW;     // 16-key subtiles per iteration: constant bytes in flight
+  static constexpr int NS = 256 / HDW;     // 16-key subtiles per iteration: 8 KB of K and of V in flight per warp
   static constexpr int TK = 16 * NS;       // keys per warp (team) and iteration
   static constexpr int TEAMS = W / HS;
   static constexpr int KB = TK * TEAMS;    // keys per block
   static constexpr int HT = 8 * NT;
   static constexpr int PART = HT * (HD + 2);       // a partial: O [HT][HD], m [HT], l [HT]
   static constexpr int SM_O = TEAMS * HT * HD;     // each team's O
+  static_assert(SM_O >= (2 * JOIN + 2) * HT, "the join's weights and sums lie there too");
   static constexpr int SM_F = SM_O + 2 * TEAMS * HT + (HS > 1 ? W * 32 * 4 * NS * NT : 0);
 };
 
@@ -109,54 +113,50 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
   float* sm_l = sm_m + TEAMS * HT;
   float* sm_x = sm_l + TEAMS * HT;  // HS > 1: the teams' partial scores
   __shared__ int sh_last;
-  __shared__ long long sh_scan[2];
+  __shared__ long long sh_scan[W], sh_first;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int team = warp / HS, half = warp % HS;
   const int heads_per_seq = p.nkv * p.htiles;
   sbd::griddep_launch_dependents();
   sbd::griddep_wait();
 
-  // total blocks of all sequences, and this CTA's run of them [r0, r1)
+  // total blocks of all sequences, this CTA's run of them [r0, r1) and the sequence that holds r0: each
+  // thread counts a few neighbouring sequences, whose loads are one latency
   auto blocks_of = [&](int b) {
     int lo, hi;
     key_range(p, b, &lo, &hi);
     return static_cast<long long>((hi - lo + KB - 1) / KB) * heads_per_seq;
   };
-  if (warp == 0) {
-    long long sum = 0;
-    for (int b = lane; b < p.b; b += 32) sum += blocks_of(b);
+  const int per = (p.b + W * 32 - 1) / (W * 32), b0 = threadIdx.x * per, b1 = min(b0 + per, p.b);
+  long long own = 0;
+#pragma unroll 4
+  for (int b = b0; b < b1; ++b) own += blocks_of(b);
+  long long inc = own;
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    // the sequence that holds this CTA's first block: scan 32 sequences at a time
-    const long long n = sum < gridDim.x ? sum : gridDim.x;
-    const long long r0 = n ? sum * blockIdx.x / n : 0;
-    long long before = 0;
-    int found = p.b;
-    long long found_before = sum;
-    if (blockIdx.x < n) {
-      for (int b0 = 0; b0 < p.b; b0 += 32) {
-        const long long own = b0 + lane < p.b ? blocks_of(b0 + lane) : 0;
-        long long inc = own;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) sh_scan[warp] = inc;
+  __syncthreads();
+  long long total = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-          if (lane >= o) inc += v;
-        }
-        const unsigned hit = __ballot_sync(0xFFFFFFFFu, before + inc > r0);
-        if (hit) {
-          const int l = __ffs(hit) - 1;
-          found = b0 + l;
-          found_before = before + __shfl_sync(0xFFFFFFFFu, inc - own, l);
-          break;
-        }
-        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
-      }
-    }
-    if (lane == 0) {
-      sh_scan[0] = sum;
-      sh_scan[1] = found_before;
-      sh_last = found;
-    }
+  for (int w = 0; w < W; ++w) {
+    if (w == warp) inc += total;
+    total += sh_scan[w];
+  }
+  // CTAs that work: each has at least MIN_KEYS keys to itself, so that joining does not cost more than it saves;
+  // every one of them holds at least one block
+  constexpr int MIN_BLOCKS = MIN_KEYS > KB ? MIN_KEYS / KB : 1;
+  const long long n_cta = min(static_cast<long long>(gridDim.x), (total + MIN_BLOCKS - 1) / MIN_BLOCKS);
+  const bool works = blockIdx.x < n_cta;
+  const long long r0 = works ? total * blockIdx.x / n_cta : 0, r1 = works ? total * (blockIdx.x + 1) / n_cta : 0;
+  if (works && inc - own <= r0 && r0 < inc) {
+    long long at = inc - own;
+    int b = b0;
+    for (long long n; (n = blocks_of(b)) <= r0 - at; ++b) at += n;
+    sh_first = at;
+    sh_last = b;
   }
   // sequences with no key at all: zero rows
   for (int b = blockIdx.x; b < p.b; b += gridDim.x) {
@@ -167,13 +167,8 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
     for (int i = threadIdx.x; i < p.nkv * p.group * HD / 8; i += W * 32) dst[i] = make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
-  const long long total = sh_scan[0];
-  long long seq_start = sh_scan[1];  // first block of sequence `b`
+  long long seq_start = sh_first;  // first block of sequence `b`
   int b = sh_last;
-  // every CTA below n_cta holds at least one block, those from n_cta on hold none
-  const long long n_cta = total < gridDim.x ? total : gridDim.x;
-  const bool works = blockIdx.x < n_cta;
-  const long long r0 = works ? total * blockIdx.x / n_cta : 0, r1 = works ? total * (blockIdx.x + 1) / n_cta : 0;
   const T* kbase = static_cast<const T*>(p.pages.k);
   const T* vbase = static_cast<const T*>(p.pages.v);
   const int pmask = (1 << p.pages.shift) - 1;
@@ -224,30 +219,30 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
       return pg >= 0 && pg < p.pages.n_pages ? pg : -1;
     };
     // this lane holds the pages of keys base + lane (and + 32 when a tile has 64 keys)
-    constexpr int PL = TK > 32 ? 2 : 1;
-    int pg[PL], pg_next[PL];
-    auto fetch_pages = [&](int base, int (&d)[PL]) {
-#pragma unroll
-      for (int j = 0; j < PL; ++j) d[j] = lane + 32 * j < TK ? page_of(base + lane + 32 * j) : -1;
+    struct Held {
+      int a, b;
+    };
+    auto fetch_page = [&](int base) {
+      return Held{lane < TK ? page_of(base + lane) : -1, lane + 32 < TK ? page_of(base + lane + 32) : -1};
     };
     auto row_of = [&](const T* basep, int key, int page) {
       return basep + page * p.pages.page_stride + kv * p.pages.head_stride + (key & pmask) * p.pages.token_stride;
     };
     uint4 kf[2 * NS][KC];
-    auto load_k = [&](int base, const int (&d)[PL]) {
+    auto load_k = [&](int base, const Held& pages) {
 #pragma unroll
       for (int j = 0; j < 2 * NS; ++j) {
         const int in = 8 * j + g;
-        const int page = __shfl_sync(0xFFFFFFFFu, d[8 * j >= 32 ? PL - 1 : 0], in & 31);
+        const int page = __shfl_sync(0xFFFFFFFFu, 8 * j >= 32 ? pages.b : pages.a, in & 31);
         const T* src = row_of(kbase, base + in, page) + half * HDW + 8 * t;
 #pragma unroll
         for (int i = 0; i < KC; ++i) kf[j][i] = page >= 0 ? sbd::ldg_nc_v4(src + 32 * i) : make_uint4(0, 0, 0, 0);
       }
     };
     int base = k_begin + team * TK;
-    fetch_pages(base, pg);
+    Held pg = fetch_page(base);
     load_k(base, pg);
-    fetch_pages(base + KB, pg_next);
+    Held pg_next = fetch_page(base + KB);
     for (; base < k_end; base += KB) {
       // V of this tile: keys 16 s + {2t, 2t+1, 2t+8, 2t+9}
       uint4 vf[NS][4][VC];
@@ -257,7 +252,7 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int in = 16 * s + 2 * t + (x & 1) + 8 * (x >> 1);
-          const int page = __shfl_sync(0xFFFFFFFFu, pg[16 * s >= 32 ? PL - 1 : 0], in & 31);
+          const int page = __shfl_sync(0xFFFFFFFFu, 16 * s >= 32 ? pg.b : pg.a, in & 31);
           const T* src = row_of(vbase, base + in, page) + half * HDW + 8 * g;
           okmask |= page >= 0 ? 1u << (4 * s + x) : 0u;
 #pragma unroll
@@ -279,9 +274,8 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
       }
       // the next tile's K while the softmax and the second product run
       load_k(base + KB, pg_next);
-#pragma unroll
-      for (int j = 0; j < PL; ++j) pg[j] = pg_next[j];
-      fetch_pages(base + 2 * KB, pg_next);
+      pg = pg_next;
+      pg_next = fetch_page(base + 2 * KB);
       if constexpr (HS > 1) {  // the sum of the team's shares of the dims, in one order for all of them
         constexpr int N = 4 * NS * NT;
         float* share = sm_x + (team * HS * 32 + lane) * N;
@@ -406,40 +400,78 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
       }
     }
     if (!whole) {
-      // the CTAs that hold blocks of this segment: [c0, c1]; the last to arrive joins them
+      // the CTAs that hold blocks of this segment: [c0, c1]
       const int c0 = static_cast<int>(((seg0 + 1) * n_cta - 1) / total), c1 = static_cast<int>((seg1 * n_cta - 1) / total);
-      unsigned int* cnt = p.count + static_cast<int64_t>(b) * heads_per_seq + hidx;
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const unsigned int seen = atomicAdd(cnt, 1u);
-        sh_last = seen == static_cast<unsigned int>(c1 - c0);
-        if (sh_last) *cnt = 0;
-      }
-      __syncthreads();
-      if (sh_last) {
+      const bool first_aligned = total * c0 / n_cta == seg0;  // c0's run begins with this segment
+      auto slot = [&](int c) { return p.part + (static_cast<int64_t>(c) * 2 + (c > c0 || first_aligned ? 0 : 1)) * C::PART; };
+      // true in the last of `n` CTAs to arrive at a counter; everything they wrote before is visible to it
+      auto last_of = [&](unsigned int* cnt, int n) {
         __threadfence();
-        const bool first_aligned = total * c0 / n_cta == seg0;  // c0's run begins with this segment
-        for (int i = threadIdx.x; i < nheads * (HD / 8); i += W * 32) {
-          const int h = i / (HD / 8), d = 8 * (i % (HD / 8));
-          float M = -INFINITY, L = 0.f, acc[8] = {};
-          for (int c = c0; c <= c1; ++c) {
-            const float* src = p.part + (static_cast<int64_t>(c) * 2 + (c > c0 || first_aligned ? 0 : 1)) * C::PART;
-            const float mc = __ldcg(src + HT * HD + h), lc = __ldcg(src + HT * HD + HT + h);
-            const float4 v0 = __ldcg(reinterpret_cast<const float4*>(src + h * HD + d));
-            const float4 v1 = __ldcg(reinterpret_cast<const float4*>(src + h * HD + d + 4));
-            const float Mn = fmaxf(M, mc), mu = Mn == -INFINITY ? 0.f : Mn;
-            const float fo = ex2(M - mu), fn = ex2(mc - mu);
-            M = Mn;
-            L = L * fo + lc * fn;
-            const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-            for (int x = 0; x < 8; ++x) acc[x] = acc[x] * fo + v[x] * fn;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          sh_last = atomicAdd(cnt, 1u) == static_cast<unsigned int>(n - 1);
+          if (sh_last) *cnt = 0;  // ready for the next call
+          __threadfence();
+        }
+        __syncthreads();
+        return sh_last != 0;
+      };
+      // joins the partials of n CTAs (at most JOIN), the i-th in slot(of(i)): into the output, or into the first one's slot
+      auto join = [&](int n, auto of, bool final) {
+        float* wgt = sm_o;  // [n][HT] weights, then [HT] sums; the teams' O is no longer needed
+        float* ls = wgt + (JOIN + 2) * HT;
+        for (int i = threadIdx.x; i < n * HT; i += W * 32) {
+          const float* src = slot(of(i / HT)) + HT * HD + i % HT;
+          wgt[i] = __ldcg(src);
+          ls[i] = __ldcg(src + HT);
+        }
+        __syncthreads();
+        if (threadIdx.x < nheads) {
+          const int h = threadIdx.x;
+          float M = -INFINITY, L = 0.f;
+          for (int i = 0; i < n; ++i) M = fmaxf(M, wgt[i * HT + h]);
+          const float mu = M == -INFINITY ? 0.f : M;
+          for (int i = 0; i < n; ++i) {
+            const float f = ex2(wgt[i * HT + h] - mu);
+            wgt[i * HT + h] = f;
+            L += f * ls[i * HT + h];
           }
-          const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) acc[x] *= inv;
-          sbp::store8(out + h * HD + d, acc);
+          wgt[n * HT + h] = L;
+          wgt[(n + 1) * HT + h] = M;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < nheads * (HD / 4); i += W * 32) {
+          const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int x = 0; x < n; ++x) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(of(x)) + h * HD + d));
+            const float f = wgt[x * HT + h];
+            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+          }
+          const float L = wgt[n * HT + h];
+          if (final) {
+            const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+            *reinterpret_cast<uint2*>(out + h * HD + d) =
+                make_uint2(sbp::pack2<T>(acc.x * inv, acc.y * inv), sbp::pack2<T>(acc.z * inv, acc.w * inv));
+          } else {
+            float* dst = slot(of(0));
+            *reinterpret_cast<float4*>(dst + h * HD + d) = acc;
+            if (d == 0) dst[HT * HD + h] = wgt[(n + 1) * HT + h], dst[HT * HD + HT + h] = L;
+          }
+        }
+      };
+      unsigned int* cnt = p.count + static_cast<int64_t>(b) * heads_per_seq + hidx;
+      if (c1 - c0 < JOIN) {
+        if (last_of(cnt, c1 - c0 + 1)) join(c1 - c0 + 1, [&](int i) { return c0 + i; }, true);
+      } else {
+        // a long segment: CTAs of each group of JOIN neighbours join first, so that no CTA reads them all.  A
+        // group touches two long segments at most: one from its left, one that starts in it.
+        const int grp = static_cast<int>(blockIdx.x) / JOIN, g0 = max(c0, grp * JOIN), g1 = min(c1, grp * JOIN + JOIN - 1);
+        if (last_of(p.group_count + 2 * grp + (c0 < grp * JOIN ? 0 : 1), g1 - g0 + 1)) {
+          join(g1 - g0 + 1, [&](int i) { return g0 + i; }, false);
+          const int first = c0 / JOIN, n = c1 / JOIN - first + 1;
+          if (last_of(cnt, n)) join(n, [&](int i) { return max(c0, (first + i) * JOIN); }, true);
         }
       }
     }
@@ -448,15 +480,17 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
   }
 }
 
-// CTAs of one resident wave, and the workspace's layout (counters, then partials).
-int grid_of() { return 2 * sb::num_sms(); }
-
 int head_tile(int group) { return group <= 8 ? 8 : 16; }
 
+// CTAs of one resident wave.
+int grid_of() { return 2 * sb::num_sms(); }
+
+// The workspace: counters of the groups and of the segments, then the partials.
+size_t group_bytes(int grid) { return (static_cast<size_t>(grid) / JOIN + 1) * 8; }
 size_t counter_bytes(const sb_paged_kv* kv, int n_heads, int b) {
   const int group = n_heads / kv->n_kv_heads, ht = head_tile(group);
   const size_t n = static_cast<size_t>(b) * kv->n_kv_heads * ((group + ht - 1) / ht);
-  return (n * 4 + 255) / 256 * 256;
+  return (group_bytes(grid_of()) + n * 4 + 255) / 256 * 256;
 }
 
 template <typename T, int HD, int HS, int NT>
@@ -513,9 +547,11 @@ extern "C" int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_t
   const int group = n_heads / kv->n_kv_heads, ht = head_tile(group);
   p.q = q, p.q_stride = q_stride, p.out = out, p.pos = pos, p.b = b, p.nkv = kv->n_kv_heads, p.group = group;
   p.htiles = (group + ht - 1) / ht, p.window = window, p.scale2 = scale * kLog2e;
-  p.count = static_cast<unsigned int*>(workspace);
+  const int grid = grid_of();
+  p.group_count = static_cast<unsigned int*>(workspace);
+  p.count = p.group_count + group_bytes(grid) / 4;
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + counter_bytes(kv, n_heads, b));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return kv->dtype == SB_F16 ? launch_decode_hd<__half>(kv->head_dim, ht, p, grid_of(), s)
-                             : launch_decode_hd<__nv_bfloat16>(kv->head_dim, ht, p, grid_of(), s);
+  return kv->dtype == SB_F16 ? launch_decode_hd<__half>(kv->head_dim, ht, p, grid, s)
+                             : launch_decode_hd<__nv_bfloat16>(kv->head_dim, ht, p, grid, s);
 }
