@@ -97,7 +97,8 @@ struct Shape {
   static constexpr int KB = TK * TEAMS;    // keys per block
   static constexpr int HT = 8 * NT;
   static constexpr int PART = HT * (HD + 2);       // a partial: O [HT][HD], m [HT], l [HT]
-  static constexpr int SM_O = TEAMS * HT * HD;     // each team's O
+  static constexpr int HP = HD + 4;                // a head's row in shared memory: neighbouring heads in other banks
+  static constexpr int SM_O = TEAMS * HT * HP;     // each team's O
   static_assert(SM_O >= (2 * JOIN + 2) * HT, "the join's weights and sums lie there too");
   static constexpr int SM_F = SM_O + 2 * TEAMS * HT + (HS > 1 ? W * 32 * 4 * NS * NT : 0);
 };
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
   float* sm_l = sm_m + TEAMS * HT;
   float* sm_x = sm_l + TEAMS * HT;  // HS > 1: the teams' partial scores
   __shared__ int sh_last;
-  __shared__ long long sh_scan[W], sh_first;
+  __shared__ int sh_scan[W], sh_first[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int team = warp / HS, half = warp % HS;
   const int heads_per_seq = p.nkv * p.htiles;
@@ -121,74 +122,68 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
   sbd::griddep_wait();
 
   // total blocks of all sequences, this CTA's run of them [r0, r1) and the sequence that holds r0: each
-  // thread counts a few neighbouring sequences, whose loads are one latency
-  auto blocks_of = [&](int b) {
+  // thread counts a few neighbouring sequences, whose loads are one latency (blocks of 16 keys or more of
+  // a cache that fits a GPU number far below 2^31)
+  auto blocks_of = [&](int lo, int hi) { return (hi - lo + KB - 1) / KB * heads_per_seq; };
+  const int per = (p.b + W * 32 - 1) / (W * 32), b0 = threadIdx.x * per, b1 = min(b0 + per, p.b);
+  int own = 0;
+#pragma unroll 4
+  for (int b = b0; b < b1; ++b) {
     int lo, hi;
     key_range(p, b, &lo, &hi);
-    return static_cast<long long>((hi - lo + KB - 1) / KB) * heads_per_seq;
-  };
-  const int per = (p.b + W * 32 - 1) / (W * 32), b0 = threadIdx.x * per, b1 = min(b0 + per, p.b);
-  long long own = 0;
-#pragma unroll 4
-  for (int b = b0; b < b1; ++b) own += blocks_of(b);
-  long long inc = own;
+    own += blocks_of(lo, hi);
+  }
+  int inc = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
     if (lane >= o) inc += v;
   }
   if (lane == 31) sh_scan[warp] = inc;
   __syncthreads();
-  long long total = 0;
+  int total = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     if (w == warp) inc += total;
     total += sh_scan[w];
   }
   // CTAs that work: each has at least MIN_KEYS keys to itself, so that joining does not cost more than it saves;
-  // every one of them holds at least one block
+  // the first `more` of them hold `share` + 1 blocks, the others `share`
   constexpr int MIN_BLOCKS = MIN_KEYS > KB ? MIN_KEYS / KB : 1;
-  const long long n_cta = min(static_cast<long long>(gridDim.x), (total + MIN_BLOCKS - 1) / MIN_BLOCKS);
-  const bool works = blockIdx.x < n_cta;
-  const long long r0 = works ? total * blockIdx.x / n_cta : 0, r1 = works ? total * (blockIdx.x + 1) / n_cta : 0;
+  const int n_cta = min(static_cast<int>(gridDim.x), (total + MIN_BLOCKS - 1) / MIN_BLOCKS);
+  const int share = n_cta ? total / n_cta : 0, more = total - share * n_cta;
+  auto start_of = [&](int c) { return c * share + min(c, more); };
+  auto cta_of = [&](int r) { return r < more * (share + 1) ? r / (share + 1) : more + (r - more * (share + 1)) / share; };
+  const bool works = static_cast<int>(blockIdx.x) < n_cta;
+  const int r0 = works ? start_of(blockIdx.x) : 0, r1 = works ? start_of(blockIdx.x + 1) : 0;
   if (works && inc - own <= r0 && r0 < inc) {
-    long long at = inc - own;
-    int b = b0;
-    for (long long n; (n = blocks_of(b)) <= r0 - at; ++b) at += n;
-    sh_first = at;
-    sh_last = b;
-  }
-  // sequences with no key at all: zero rows
-  for (int b = blockIdx.x; b < p.b; b += gridDim.x) {
-    int lo, hi;
-    key_range(p, b, &lo, &hi);
-    if (hi > lo) continue;
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<int64_t>(b) * p.nkv * p.group * HD);
-    for (int i = threadIdx.x; i < p.nkv * p.group * HD / 8; i += W * 32) dst[i] = make_uint4(0, 0, 0, 0);
+    int at = inc - own, b = b0, lo, hi;
+    for (;; ++b) {
+      key_range(p, b, &lo, &hi);
+      if (r0 < at + blocks_of(lo, hi)) break;
+      at += blocks_of(lo, hi);
+    }
+    sh_first[0] = b, sh_first[1] = at, sh_first[2] = lo, sh_first[3] = hi;
   }
   __syncthreads();
-  long long seq_start = sh_first;  // first block of sequence `b`
-  int b = sh_last;
+  int b = sh_first[0], seq_start = sh_first[1], lo = sh_first[2], hi = sh_first[3];  // seq_start: its first block
   const T* kbase = static_cast<const T*>(p.pages.k);
   const T* vbase = static_cast<const T*>(p.pages.v);
   const int pmask = (1 << p.pages.shift) - 1;
 
-  for (long long r = r0; r < r1;) {
-    int lo, hi;
-    key_range(p, b, &lo, &hi);
+  for (int r = r0; r < r1;) {
     const int nblk = (hi - lo + KB - 1) / KB;
-    if (nblk == 0 || r >= seq_start + static_cast<long long>(nblk) * heads_per_seq) {
-      seq_start += static_cast<long long>(nblk) * heads_per_seq;
-      ++b;
+    if (r >= seq_start + nblk * heads_per_seq) {
+      seq_start += nblk * heads_per_seq;
+      key_range(p, ++b, &lo, &hi);
       continue;
     }
-    const int hidx = static_cast<int>((r - seq_start) / nblk);  // (kv head, head tile)
-    const long long seg0 = seq_start + static_cast<long long>(hidx) * nblk, seg1 = seg0 + nblk;
-    const long long e = r1 < seg1 ? r1 : seg1;
+    const int hidx = (r - seq_start) / nblk;  // (kv head, head tile)
+    const int seg0 = seq_start + hidx * nblk, seg1 = seg0 + nblk;
+    const int e = min(r1, seg1);
     const int kv = hidx / p.htiles, h0 = (hidx % p.htiles) * HT;  // query heads kv * group + h0 ...
     const int nheads = min(HT, p.group - h0);
-    const int k_begin = lo + static_cast<int>(r - seg0) * KB;
-    const int k_end = min(hi, lo + static_cast<int>(e - seg0) * KB);
+    const int k_begin = lo + (r - seg0) * KB, k_end = min(hi, lo + (e - seg0) * KB);
     const int32_t* row = p.pages.table + static_cast<int64_t>(b) * p.pages.max_pages;
 
     // Q fragments: vector i of lane (g, t) is dims half * HDW + 8 (t + 4 i) ... of heads g (and g + 8)
@@ -362,7 +357,7 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
       for (int c = 0; c < VC; ++c)
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          float* dst = sm_o + (team * HT + 8 * n + 2 * t + hh) * HD + half * HDW + 64 * c + 8 * g;
+          float* dst = sm_o + (team * HT + 8 * n + 2 * t + hh) * C::HP + half * HDW + 64 * c + 8 * g;
           *reinterpret_cast<float4*>(dst) = make_float4(o[4 * c][n][hh], o[4 * c][n][2 + hh], o[4 * c + 1][n][hh], o[4 * c + 1][n][2 + hh]);
           *reinterpret_cast<float4*>(dst + 4) = make_float4(o[4 * c + 2][n][hh], o[4 * c + 2][n][2 + hh], o[4 * c + 3][n][hh], o[4 * c + 3][n][2 + hh]);
         }
@@ -383,7 +378,7 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
         const float f = ex2(sm_m[w * HT + h] - mu);
         L += f * sm_l[w * HT + h];
         float v[8];
-        sbp::load8(sm_o + (w * HT + h) * HD + d, v);
+        sbp::load8(sm_o + (w * HT + h) * C::HP + d, v);
 #pragma unroll
         for (int x = 0; x < 8; ++x) acc[x] += f * v[x];
       }
@@ -401,17 +396,17 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
     }
     if (!whole) {
       // the CTAs that hold blocks of this segment: [c0, c1]
-      const int c0 = static_cast<int>(((seg0 + 1) * n_cta - 1) / total), c1 = static_cast<int>((seg1 * n_cta - 1) / total);
-      const bool first_aligned = total * c0 / n_cta == seg0;  // c0's run begins with this segment
+      const int c0 = cta_of(seg0), c1 = cta_of(seg1 - 1);
+      const bool first_aligned = start_of(c0) == seg0;  // c0's run begins with this segment
       auto slot = [&](int c) { return p.part + (static_cast<int64_t>(c) * 2 + (c > c0 || first_aligned ? 0 : 1)) * C::PART; };
       // true in the last of `n` CTAs to arrive at a counter; everything they wrote before is visible to it
       auto last_of = [&](unsigned int* cnt, int n) {
-        __threadfence();
         __syncthreads();
-        if (threadIdx.x == 0) {
-          sh_last = atomicAdd(cnt, 1u) == static_cast<unsigned int>(n - 1);
+        if (threadIdx.x == 0) {  // one release / acquire for the CTA, around whose barriers its threads' accesses stand
+          unsigned int seen;
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(seen) : "l"(cnt) : "memory");
+          sh_last = seen == static_cast<unsigned int>(n - 1);
           if (sh_last) *cnt = 0;  // ready for the next call
-          __threadfence();
         }
         __syncthreads();
         return sh_last != 0;
@@ -426,13 +421,13 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
           ls[i] = __ldcg(src + HT);
         }
         __syncthreads();
-        if (threadIdx.x < nheads) {
+        if (threadIdx.x < HT) {  // rows of heads that are not there hold anything: no weight
           const int h = threadIdx.x;
           float M = -INFINITY, L = 0.f;
           for (int i = 0; i < n; ++i) M = fmaxf(M, wgt[i * HT + h]);
           const float mu = M == -INFINITY ? 0.f : M;
           for (int i = 0; i < n; ++i) {
-            const float f = ex2(wgt[i * HT + h] - mu);
+            const float f = h < nheads ? ex2(wgt[i * HT + h] - mu) : 0.f;
             wgt[i * HT + h] = f;
             L += f * ls[i * HT + h];
           }
@@ -440,23 +435,40 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
           wgt[(n + 1) * HT + h] = M;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < nheads * (HD / 4); i += W * 32) {
-          const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int x = 0; x < n; ++x) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(of(x)) + h * HD + d));
-            const float f = wgt[x * HT + h];
-            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+        // every thread has the loads of several parts of its vectors in flight at once
+        constexpr int VPT = HT * HD / 4 / (W * 32), UX = VPT >= 16 ? 2 : 32 / VPT > 8 ? 8 : 32 / VPT;
+        float4 acc[VPT];
+#pragma unroll
+        for (int u = 0; u < VPT; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int x = 0; x < n; x += UX) {
+          float4 v[UX][VPT];
+#pragma unroll
+          for (int y = 0; y < UX; ++y) {
+            const float4* src = reinterpret_cast<const float4*>(slot(of(min(x + y, n - 1)))) + threadIdx.x;
+#pragma unroll
+            for (int u = 0; u < VPT; ++u) v[y][u] = __ldcg(src + u * W * 32);
           }
+#pragma unroll
+          for (int y = 0; y < UX; ++y)
+#pragma unroll
+            for (int u = 0; u < VPT; ++u) {
+              const float f = x + y < n ? wgt[(x + y) * HT + (threadIdx.x + u * W * 32) / (HD / 4)] : 0.f;
+              if (f == 0.f) continue;  // a part without weight, or of a head that is not there
+              acc[u].x += f * v[y][u].x, acc[u].y += f * v[y][u].y, acc[u].z += f * v[y][u].z, acc[u].w += f * v[y][u].w;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < VPT; ++u) {
+          const int i = threadIdx.x + u * W * 32, h = i / (HD / 4), d = 4 * (i % (HD / 4));
+          if (h >= nheads) continue;
           const float L = wgt[n * HT + h];
           if (final) {
             const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
             *reinterpret_cast<uint2*>(out + h * HD + d) =
-                make_uint2(sbp::pack2<T>(acc.x * inv, acc.y * inv), sbp::pack2<T>(acc.z * inv, acc.w * inv));
+                make_uint2(sbp::pack2<T>(acc[u].x * inv, acc[u].y * inv), sbp::pack2<T>(acc[u].z * inv, acc[u].w * inv));
           } else {
             float* dst = slot(of(0));
-            *reinterpret_cast<float4*>(dst + h * HD + d) = acc;
+            *reinterpret_cast<float4*>(dst + h * HD + d) = acc[u];
             if (d == 0) dst[HT * HD + h] = wgt[(n + 1) * HT + h], dst[HT * HD + HT + h] = L;
           }
         }
@@ -477,6 +489,13 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
     }
     __syncthreads();  // shared memory is free for the next segment
     r = e;
+  }
+  // sequences with no key at all: zero rows
+  for (int b = blockIdx.x; b < p.b; b += gridDim.x) {
+    key_range(p, b, &lo, &hi);
+    if (hi > lo) continue;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<int64_t>(b) * p.nkv * p.group * HD);
+    for (int i = threadIdx.x; i < p.nkv * p.group * HD / 8; i += W * 32) dst[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
