@@ -6,11 +6,11 @@
 // row pos % page_size.
 //
 // Every value is read and written once: bound by memory for many tokens and by
-// launch latency for a few.  A lane holds eight neighbouring values (one
-// 16-byte vector in 16 bits), so a head takes head_dim / 8 lanes and a warp
-// holds 256 / head_dim heads (or one head of 512 as two vectors per lane); the
-// rotation's partner value sits r / 8 lanes away and comes by shuffle, which
-// keeps every load and store a full vector whatever rot is.
+// launch latency for a few.  A lane holds the two vectors of eight values that the
+// rotation pairs, v and v + r / 8 (past the rotated part any two), so a pair
+// shares its angles, nothing is exchanged between lanes but the norm's sum, and
+// every load and store is a full vector whatever rot is.  A head takes
+// head_dim / 16 lanes, a warp holds 512 / head_dim heads.
 #include "paged.cuh"
 
 namespace {
@@ -22,127 +22,127 @@ struct AppendParams {
   const float *q_norm, *k_norm, *cos_t, *sin_t;
   const int32_t *seq, *pos;
   sbp::Pages pages;
-  int t, n_seqs, nh, nkv, rot, max_pos, v_norm, units;  // units: warp-wide pieces of a token's row
+  int t, n_seqs, nh, nkv, rot, max_pos, v_norm, units;  // units: warps per token
   float eps;
 };
 
-// VPT: vectors of eight per lane (2 for head_dim 512, else 1).
-template <int HD, typename S, typename D>
-__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p) {
-  constexpr int VPT = HD > 256 ? 2 : 1;
-  constexpr int LPH = HD / (8 * VPT);  // lanes per head
-  constexpr int HPW = 32 / LPH;        // heads per warp
+// R: pieces of 512 values of one token per warp, whose loads are all in flight at
+// once and share the angles and the page.
+template <int HD, int R, typename S, typename D>
+__global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendParams p) {
+  constexpr int LPH = HD / 16;   // lanes per head
+  constexpr int HPW = 32 / LPH;  // heads per piece
   sbd::griddep_launch_dependents();
-  sbd::griddep_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int tok = static_cast<int>(unit / p.units);
-  if (tok >= p.t) return;  // whole warps
+  const unsigned warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int tok = static_cast<int>(warp / static_cast<unsigned>(p.units));
   const int heads = p.nh + 2 * p.nkv;
-  const int head = static_cast<int>(unit - static_cast<int64_t>(tok) * p.units) * HPW + lane / LPH;
-  const int sub = lane % LPH;  // vector j of this lane covers values 8 * (sub + j * LPH) ...
-  const bool live = head < heads;
+  const int head0 = (static_cast<int>(warp) - tok * p.units) * R * HPW + lane / LPH;  // piece r: head0 + r * HPW
+  // this lane's pair of vectors: i and i + rot/2 for i < rot/2; past rot the halves of the rest
+  const int sub = lane % LPH, hv = p.rot >> 4;
+  const bool turns = sub < hv;
+  const int at0 = 8 * (turns ? sub : sub + hv), at1 = 8 * (turns ? sub + hv : sub + LPH);
+  sbd::griddep_wait();
+  if (tok >= p.t) return;  // whole warps
+
+  const S* src = static_cast<const S*>(p.qkv) + tok * p.ld;
+  float x[R][2][8];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int head = min(head0 + r * HPW, heads - 1);  // a head past the last loads it again and stores nothing
+    sbp::load8(src + head * HD + at0, x[r][0]);
+    sbp::load8(src + head * HD + at1, x[r][1]);
+  }
   const int pos = p.pos[tok];
   const int seq = p.seq ? p.seq[tok] : tok;
-  const bool place = pos >= 0 && pos < p.max_pos;
-
-  float x[VPT][8];
+  D* q_row = static_cast<D*>(p.q_out) + static_cast<int64_t>(tok) * p.nh * HD;
+  if (pos < 0 || pos >= p.max_pos) {  // padding (the whole warp): its q is zero, nothing is appended
+    const float zero[8] = {};
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    if (live) {
-      sbp::load8(static_cast<const S*>(p.qkv) + tok * p.ld + static_cast<int64_t>(head) * HD + 8 * (sub + j * LPH), x[j]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[j][e] = 0.f;
-    }
-  }
-  const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
-  const float* w = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
-  if (p.q_norm || p.k_norm || p.v_norm) {  // uniform over the warp: the shuffles below meet every lane
-    float ss = 0.f;
-#pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss += x[j][e] * x[j][e];
-#pragma unroll
-    for (int o = LPH / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-    const float rd = 1.0f / sqrtf(ss / HD + p.eps);
-    if (w || (is_v && p.v_norm)) {
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        float wv[8];
-        if (w) sbp::load8(w + 8 * (sub + j * LPH), wv);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[j][e] *= w ? rd * wv[e] : rd;
-      }
-    }
-  }
-  // rotation: value i < rot/2 pairs with i + rot/2, a whole number of vectors away
-  const int hv = p.rot >> 4;  // vectors in half the rotated part
-  float y[VPT][8];
-#pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int vec = sub + j * LPH;
-    const bool rotates = vec < 2 * hv, low = vec < hv;
-    const int other = rotates ? (low ? vec + hv : vec - hv) : vec;  // the partner's vector
-    const int src = (lane - sub) + other % LPH;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float o = __shfl_sync(0xFFFFFFFFu, x[0][e], src);
-      if constexpr (VPT == 2) {
-        const float o1 = __shfl_sync(0xFFFFFFFFu, x[1][e], src);
-        o = other >= LPH ? o1 : o;
-      }
-      y[j][e] = o;
-    }
-    if (rotates && live && !is_v && place) {
-      const size_t at = static_cast<size_t>(pos) * (p.rot >> 1) + 8 * (low ? vec : other);
-      float c[8], s[8];
-      sbp::load8(p.cos_t + at, c);
-      sbp::load8(p.sin_t + at, s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[j][e] = low ? x[j][e] * c[e] - y[j][e] * s[e] : x[j][e] * c[e] + y[j][e] * s[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[j][e] = x[j][e];
-    }
-  }
-  if (!live) return;
-  if (is_q) {
-    if (!p.q_out) return;
-    D* dst = static_cast<D*>(p.q_out) + (static_cast<int64_t>(tok) * p.nh + head) * HD;
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      if (!place) {  // a padding token's q is zero
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[j][e] = 0.f;
-      }
-      sbp::store8(dst + 8 * (sub + j * LPH), y[j]);
+    for (int r = 0; r < R; ++r) {
+      if (!p.q_out || head0 + r * HPW >= p.nh) continue;
+      sbp::store8(q_row + (head0 + r * HPW) * HD + at0, zero);
+      sbp::store8(q_row + (head0 + r * HPW) * HD + at1, zero);
     }
     return;
   }
-  // a token out of place, a sequence without the page, or a page the cache does not have: nothing is written
-  if (!place || seq < 0 || seq >= p.n_seqs || (pos >> p.pages.shift) >= p.pages.max_pages) return;
-  const int page = p.pages.table[static_cast<int64_t>(seq) * p.pages.max_pages + (pos >> p.pages.shift)];
-  if (page < 0 || page >= p.pages.n_pages) return;
-  const int g = head - p.nh - (is_v ? p.nkv : 0);
-  D* dst = static_cast<D*>(const_cast<void*>(is_v ? p.pages.v : p.pages.k)) + page * p.pages.page_stride +
-           g * p.pages.head_stride + (pos & ((1 << p.pages.shift) - 1)) * p.pages.token_stride;
+  // the page of the token, -1 for a sequence without it or a page the cache does not have
+  int page = -1;
+  if (seq >= 0 && seq < p.n_seqs && (pos >> p.pages.shift) < p.pages.max_pages)
+    page = p.pages.table[static_cast<int64_t>(seq) * p.pages.max_pages + (pos >> p.pages.shift)];
+  if (page >= p.pages.n_pages) page = -1;
+  float c[8], sn[8];
+  if (turns) {
+    const size_t at = static_cast<size_t>(pos) * (p.rot >> 1) + at0;
+    sbp::load8(p.cos_t + at, c);
+    sbp::load8(p.sin_t + at, sn);
+  } else {
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) sbp::store8(dst + 8 * (sub + j * LPH), y[j]);
+    for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f;
+  }
+  const int64_t kv_row = page * p.pages.page_stride + (pos & ((1 << p.pages.shift) - 1)) * p.pages.token_stride;
+  const bool norms = p.q_norm || p.k_norm || p.v_norm;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int head = head0 + r * HPW;
+    const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+    if (norms) {  // uniform over the warp: the shuffles meet every lane
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += x[r][0][e] * x[r][0][e] + x[r][1][e] * x[r][1][e];
+#pragma unroll
+      for (int o = LPH / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+      const float rd = 1.0f / sqrtf(ss / HD + p.eps);
+      const float* w = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
+      if (w) {
+        float w0[8], w1[8];
+        sbp::load8(w + at0, w0);
+        sbp::load8(w + at1, w1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[r][0][e] *= rd * w0[e], x[r][1][e] *= rd * w1[e];
+      } else if (is_v && p.v_norm) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[r][0][e] *= rd, x[r][1][e] *= rd;
+      }
+    }
+    if (!is_v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = x[r][0][e], b = x[r][1][e];
+        x[r][0][e] = a * c[e] - b * sn[e];
+        x[r][1][e] = b * c[e] + a * sn[e];
+      }
+    }
+    // nothing is stored for a head past the last, a q that is not wanted, a key or value without a page
+    if (head >= heads || (is_q ? !p.q_out : page < 0)) continue;
+    D* dst = is_q ? q_row + head * HD
+                  : static_cast<D*>(const_cast<void*>(is_v ? p.pages.v : p.pages.k)) + kv_row +
+                        (head - p.nh - (is_v ? p.nkv : 0)) * p.pages.head_stride;
+    sbp::store8(dst + at0, x[r][0]);
+    sbp::store8(dst + at1, x[r][1]);
+  }
 }
 
-template <int HD, typename S, typename D>
-int launch_append(AppendParams& p, cudaStream_t stream) {
-  constexpr int HPW = HD > 256 ? 1 : 256 / HD;
-  const int heads = p.nh + 2 * p.nkv;
-  p.units = (heads + HPW - 1) / HPW;
-  const int64_t warps = static_cast<int64_t>(p.t) * p.units;
-  const int64_t blocks = (warps + 7) / 8;
-  SB_CHECK_ARG(blocks < (1ll << 31), "sb_kv_append_paged: too many tokens");
-  cudaError_t e = sb::launch_pdl(kv_append_kernel<HD, S, D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
+template <int HD, int R, typename S, typename D>
+int launch_append_r(AppendParams& p, int pieces, cudaStream_t stream) {
+  p.units = (pieces + R - 1) / R;
+  const int64_t blocks = (static_cast<int64_t>(p.t) * p.units + 7) / 8;
+  SB_CHECK_ARG(blocks < (1ll << 28), "sb_kv_append_paged: too many tokens");
+  cudaError_t e = sb::launch_pdl(kv_append_kernel<HD, R, S, D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
   if (e != cudaSuccess) return sb::cuda_fail(e, "kv_append_kernel");
   return sb::launch_status("kv_append_kernel");
+}
+
+// A piece per warp while they fit two full waves (the shortest chain of loads);
+// beyond that three, which keep more bytes in flight.  16133 tokens of 48 heads of
+// 128 in bf16 (398 MB): 86 us with one piece, 78 with two, 70.5 with three (5.6
+// TB/s), 73 with four, whose registers leave one block less per SM.
+template <int HD, typename S, typename D>
+int launch_append(AppendParams& p, cudaStream_t stream) {
+  constexpr int HPW = 512 / HD;
+  const int pieces = (p.nh + 2 * p.nkv + HPW - 1) / HPW;
+  if (static_cast<int64_t>(p.t) * pieces <= 64ll * 2 * sb::num_sms()) return launch_append_r<HD, 1, S, D>(p, pieces, stream);
+  return launch_append_r<HD, 3, S, D>(p, pieces, stream);
 }
 
 template <typename S, typename D>
