@@ -661,8 +661,9 @@ int sb_attn_prefill_packed(const void* q, int64_t q_token, int64_t q_head, const
 
 /*
  * Draw the next token of each row of logits [rows][vocab] (f32, f16 or bf16, row
- * stride ld; rows <= 65535, vocab <= 819200).  Per row r, each setting a device
- * array or NULL for "off":
+ * stride ld; rows <= 65535, vocab <= 819200).  softcap > 0: logits are first capped,
+ * x = softcap * tanh(x / softcap), -inf excepted (the model's final_logit_softcapping,
+ * gemma4/reference.py:179).  Per row r, each setting a device array or NULL for "off":
  *   temperature[r] (off: 1)   w_i = exp((x_i - max x) / T); T <= 0: the largest logit
  *   top_k[r]       (off: 0)   keep the k largest logits (k <= 0 or k >= vocab: all)
  *   top_p[r]       (off: 1)   of those keep each whose larger ones sum to less than
@@ -678,7 +679,7 @@ int sb_attn_prefill_packed(const void* q, int64_t q_token, int64_t q_head, const
  */
 int sb_sample(const void* logits, int dtype, int64_t ld, int rows, int vocab, const int64_t* seeds,
               const int32_t* pos, const float* temperature, const int32_t* top_k, const float* top_p,
-              const float* min_p, int32_t* tokens, void* stream);
+              const float* min_p, float softcap, int32_t* tokens, void* stream);
 
 #ifdef __cplusplus
 }

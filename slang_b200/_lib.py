@@ -85,7 +85,7 @@ SIGNATURES = {
     "sb_attn_packed_plan": ([_vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp], _i),
     "sb_attn_prefill_packed": ([_vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _i, _i, _i, _f,
                                 _vp, _i, _vp], _i),
-    "sb_sample": ([_vp, _i, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i),
+    "sb_sample": ([_vp, _i, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp], _i),
 }
 
 

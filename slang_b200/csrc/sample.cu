@@ -15,43 +15,49 @@
 //   those before it
 // ends with the nucleus' own winner, after 1 / p rounds or so.
 //
-// Bound by reading the logits once.  A row belongs to one thread-block cluster
-// that holds it in shared memory, a slice per CTA; every later pass reads the
-// slices, and the CTAs exchange a few words each through distributed shared
-// memory.  What the passes cost is kept small by working on short lists:
-//   min-p, top-p  a token below w = min_p is out, and so is one below (1 - p) / V of
-//                 the total: all such tokens together weigh less than 1 - p, so
-//                 the prefix above them already holds the nucleus.
-//   top-k         the k-th largest of the threads' own maxima is a lower bound of
+// Bound by reading the logits once.  A row is cut into segments of 1024 values, a
+// warp takes whole segments, and a row's CTAs (one, or a thread-block cluster when
+// the rows are few) exchange a few words through distributed shared memory.  The
+// one pass over the row leaves each lane's maximum of its 32 values of a segment
+// and each segment's mass in shared memory; what follows reads again only the
+// lanes whose maximum can matter, mostly from the L2 cache, and keeps short lists:
+//   min-p         a token below w = min_p is out.
+//   top-p         a token below w = c is out when all such tokens together weigh no more
+//                 than 1 - p of the total: the prefix above them already holds the
+//                 nucleus.  A lane's 32 values weigh at most 32 min(c, w of its maximum)
+//                 there, so a histogram of the maxima gives a good c.
+//   top-k         the k-th largest of the lanes' maxima is a lower bound of
 //                 the k-th largest value; what reaches it (a little more than
 //                 k tokens) is sorted by one CTA, which finishes the row alone.
-// Masses are added as integers (w in units of 2^-40), so no order of addition
-// shows in the result.
+// Masses are added as integers, those of a segment in one order, so neither the
+// order of arrival nor the number of CTAs shows in the result.
 #include <algorithm>
 
 #include "paged.cuh"
 
 namespace {
 
-constexpr int NT = 512;       // threads per CTA
-constexpr int MAX_CS = 16;    // CTAs per row
-constexpr int MAX_SLICE = 51200;  // values per CTA: 200 KB
-constexpr int BINS = 256;     // of the threads' maxima, 1/8 octave of w each
-constexpr int SORT = 1024;    // candidates of a top-k row that one CTA sorts
-constexpr int MINE = 512;     // of those in one slice
-// Candidates per CTA of other rows (16-bit offsets into the slice).  Beyond this
-// many of a 16384-value slice a pass over all of it costs no more: one Philox call
-// serves four values there, one here.
+constexpr int NT = 256;         // threads per CTA
+constexpr int CTAS = 3;         // CTAs per SM
+constexpr int NW = NT / 32;
+constexpr int MAX_CS = 16;      // CTAs per row
+constexpr int SEG = 1024;       // values per segment: 32 per lane, in 8 vectors
+constexpr int MAX_V = 800 * SEG;  // 25600 lane maxima: 100 KB in one CTA
+constexpr int BINS = 256;       // of maxima, 1/8 octave of w each
+constexpr int SORT = 1024;      // candidates of a top-k row that one CTA sorts
+// Candidates per CTA of other rows.  Beyond this many a pass over all values costs
+// no more: one Philox call serves four values there, one here.
 constexpr int LIST = 3072;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLargest = 3.402823466e38f;  // bounds stay finite: -inf (banned, padding) is below them
-constexpr float kUnit = 1099511627776.f;  // 2^40
+constexpr float kUnit = 2147483648.f;        // masses in units of 2^-31 of the largest token's
 
 struct SampleParams {
   const void* x;
   int64_t ld;
-  int v, slice;  // slice: values per CTA, a multiple of 4
+  int v, segs;   // segs: segments of a row
   int vec;       // rows start on a 4-value boundary
+  float softcap; // 0: off
   const int64_t* seeds;
   const int32_t* pos;
   const float* temperature;
@@ -79,37 +85,38 @@ struct Word {
 
 struct Shared {
   Word slot[2];        // this CTA's contribution, in turn
-  Word warp[NT / 32];
+  Word warp[NW];
   Word all;
   unsigned int lower;  // the count in CTAs of lower rank
   unsigned int n;      // entries of this CTA's list
   int bin;
   unsigned int hist[BINS];
-  union {
-    uint16_t list[LIST];
-    struct {
-      unsigned long long keys[SORT];  // of the whole row, in the CTA of rank 0
-      uint16_t mine[MINE];
-    } top;
-  };
+  unsigned long long list[LIST];  // (inverted ranking bits, index): smaller ranks before
+  unsigned long long keys[SORT];  // a top-k row's, in the CTA of rank 0
 };
-static_assert(sizeof(Shared) <= 11 * 1024, "three CTAs of 64 KB slices per SM");
 
-// One counter's four words of Philox4x32-10.
-__device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t k0, uint32_t k1) {
-  uint32_t c2 = 0, c3 = 0;
+// Philox4x32-10 under one key: the keys of its ten rounds are kept, a call is
+// twenty 64-bit products and as many three-way exclusive ors.
+struct Philox {
+  uint32_t k0[10], k1[10], c1;
+  __device__ __forceinline__ Philox(uint64_t seed, uint32_t pos) : c1(pos) {
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u, b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
-    c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
-    c3 = static_cast<uint32_t>(a);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+    for (int r = 0; r < 10; ++r) {
+      k0[r] = static_cast<uint32_t>(seed) + r * 0x9E3779B9u;
+      k1[r] = static_cast<uint32_t>(seed >> 32) + r * 0xBB67AE85u;
+    }
   }
-  return make_uint4(c0, c1, c2, c3);
-}
+  __device__ __forceinline__ uint4 operator()(uint32_t c0) const {
+    uint4 c = make_uint4(c0, c1, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+      const uint64_t a = static_cast<uint64_t>(c.x) * 0xD2511F53u, b = static_cast<uint64_t>(c.z) * 0xCD9E8D57u;
+      c = make_uint4(static_cast<uint32_t>(b >> 32) ^ c.y ^ k0[r], static_cast<uint32_t>(b),
+                     static_cast<uint32_t>(a >> 32) ^ c.w ^ k1[r], static_cast<uint32_t>(a));
+    }
+    return c;
+  }
+};
 
 // The join of a warp's words, in every lane: the 64-bit parts in pieces that the
 // 32-bit warp reductions take (sums below 2^60 in pieces of 20 bits).
@@ -136,7 +143,7 @@ __device__ Word reduce(Shared& sh, Word w, int cs, int& turn) {
   if (lane == 0) sh.warp[warp] = w;
   __syncthreads();
   if (warp == 0) {
-    w = warp_join(lane < NT / 32 ? sh.warp[lane] : Word{0, ~0ull, 0, 0});
+    w = warp_join(lane < NW ? sh.warp[lane] : Word{0, ~0ull, 0, 0});
     if (lane == 0) {
       (cs > 1 ? sh.slot[turn] : sh.all) = w;
       sh.lower = 0;
@@ -163,11 +170,14 @@ __device__ Word reduce(Shared& sh, Word w, int cs, int& turn) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
-  extern __shared__ __align__(16) float xs[];  // this CTA's slice of the row, NaN as -inf, padded with -inf to a multiple of 4
+__global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) {
+  extern __shared__ __align__(16) float lane_max[];  // [local segment][lane], then [local segment] {largest, mass}
   __shared__ Shared sh;
   const int cs = gridDim.x, rank = blockIdx.x, row = blockIdx.y;  // a cluster spans the x axis
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rounds = (p.segs + cs * NW - 1) / (cs * NW);  // segments per warp; local segment l = round * NW + warp
+  float2* seg_mass = reinterpret_cast<float2*>(lane_max + rounds * NW * 32);
+  auto seg_of = [&](int round) { return (round * cs + rank) * NW + warp; };
   sbd::griddep_launch_dependents();
   if (threadIdx.x < BINS) sh.hist[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.n = 0;
@@ -175,65 +185,95 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
   const float temp = p.temperature ? p.temperature[row] : 1.f;
   const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
   const int top_k = p.top_k ? p.top_k[row] : 0;
-  const uint32_t k0 = static_cast<uint32_t>(p.seeds[row]), k1 = static_cast<uint32_t>(p.seeds[row] >> 32);
-  const uint32_t c1 = static_cast<uint32_t>(p.pos[row]);
-  const int first = rank * p.slice, n = max(0, min(p.slice, p.v - first)), n4 = (n + 3) / 4;
-  const T* src = static_cast<const T*>(p.x) + row * p.ld + first;
+  const int64_t seed = p.seeds[row];
+  const int pos = p.pos[row];
+  const T* src = static_cast<const T*>(p.x) + row * p.ld;
+  const bool greedy = !(temp > 0.f) || top_p <= 0.f || top_k == 1;
+  const float inv = fmaxf(kLog2e / temp, 1e-37f);  // above zero, so that -inf stays -inf
   int turn = 0;
 
-  // ---- the slice into shared memory; this thread's largest value, ties to the lowest index
-  float tmax = -INFINITY;
-  int tquad = -1;
-  auto take = [&](int i, float4 f) {
-    f.x = fmaxf(f.x, -INFINITY), f.y = fmaxf(f.y, -INFINITY), f.z = fmaxf(f.z, -INFINITY), f.w = fmaxf(f.w, -INFINITY);  // NaN
-    const float m = fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w));
-    if (m > tmax) tmax = m, tquad = i;
-    *reinterpret_cast<float4*>(xs + 4 * i) = f;
-  };
-  auto quad = [&](int i) {
-    if constexpr (sizeof(T) == 4) {
-      const uint4 r = sbd::ldg_nc_v4(src + 4 * i);
-      return make_float4(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), __uint_as_float(r.w));
+  // This lane's values of a segment: v[4 j + e] is value seg * SEG + 128 j + 4 lane + e, -inf for NaN and past the end.
+  auto load = [&](int seg, float (&v)[32]) {
+    const int at = seg * SEG + 4 * lane;
+    if (p.vec && seg * SEG + SEG <= p.v) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          const uint4 r = sbd::ldg_nc_v4(src + at + 128 * j);
+          v[4 * j] = __uint_as_float(r.x), v[4 * j + 1] = __uint_as_float(r.y);
+          v[4 * j + 2] = __uint_as_float(r.z), v[4 * j + 3] = __uint_as_float(r.w);
+        } else {
+          const uint2 r = __ldg(reinterpret_cast<const uint2*>(src + at + 128 * j));
+          const float2 a = sbp::unpack2<T>(r.x), b = sbp::unpack2<T>(r.y);
+          v[4 * j] = a.x, v[4 * j + 1] = a.y, v[4 * j + 2] = b.x, v[4 * j + 3] = b.y;
+        }
+      }
     } else {
-      const uint2 r = __ldg(reinterpret_cast<const uint2*>(src + 4 * i));
-      const float2 a = sbp::unpack2<T>(r.x), b = sbp::unpack2<T>(r.y);
-      return make_float4(a.x, a.y, b.x, b.y);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int idx = at + 128 * (i >> 2) + (i & 3);
+        v[i] = idx < p.v ? static_cast<float>(src[idx]) : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = fmaxf(v[i], -INFINITY);  // NaN
+    if (p.softcap > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = v[i] == -INFINITY ? v[i] : p.softcap * tanhf(v[i] / p.softcap);
     }
   };
-  int i0 = threadIdx.x;
-  if (p.vec) {
-    constexpr int U = 8;  // vectors in flight per thread
-    for (; i0 + (U - 1) * NT < n / 4; i0 += U * NT) {
-      float4 f[U];
+  auto fetch = [&](int idx) {  // one of them, as `load` gives it
+    const float x = fmaxf(static_cast<float>(src[idx]), -INFINITY);
+    return p.softcap > 0.f && x > -INFINITY ? p.softcap * tanhf(x / p.softcap) : x;
+  };
+  auto index_of = [&](int seg, int i) { return seg * SEG + 128 * (i >> 2) + 4 * lane + (i & 3); };
+
+  // ---- the pass over the row: the largest value (ties: the lowest index), lane maxima, segment masses
+  float wmax = -INFINITY;  // this warp's, with its index
+  unsigned widx = ~0u;
+  for (int r = 0; r < rounds; ++r) {
+    const int seg = seg_of(r);
+    float m = -INFINITY, sm = -INFINITY, sum = 0.f;
+    if (seg < p.segs) {
+      float v[32];
+      load(seg, v);
 #pragma unroll
-      for (int u = 0; u < U; ++u) f[u] = quad(i0 + u * NT);
+      for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
+      sm = m;
 #pragma unroll
-      for (int u = 0; u < U; ++u) take(i0 + u * NT, f[u]);
+      for (int o = 16; o >= 1; o >>= 1) sm = fmaxf(sm, __shfl_xor_sync(0xFFFFFFFFu, sm, o));
+      if (sm > wmax) {  // segments come in rising order: an equal value later has a higher index
+        unsigned idx = ~0u;
+        if (m == sm) {
+#pragma unroll
+          for (int i = 31; i >= 0; --i) idx = v[i] == m ? index_of(seg, i) : idx;
+        }
+        wmax = sm;
+        widx = __reduce_min_sync(0xFFFFFFFFu, idx);
+      }
+      if (top_p < 1.f && !greedy && sm > -INFINITY) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 32; ++i) part[i & 3] += ex2(fminf((v[i] - sm) * inv, 0.f));
+        sum = (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      }
     }
-    for (; i0 < n / 4; i0 += NT) take(i0, quad(i0));
-  }
-  for (; i0 < n4; i0 += NT) {
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = 4 * i0 + e < n ? static_cast<float>(src[4 * i0 + e]) : -INFINITY;
-    take(i0, make_float4(v[0], v[1], v[2], v[3]));
+    lane_max[(r * NW + warp) * 32 + lane] = m;
+    if (lane == 0) seg_mass[r * NW + warp] = make_float2(sm, sum);
   }
   Word w0{0, ~0ull, 0, 0};
-  if (tquad >= 0) {
-    const float4 f = *reinterpret_cast<const float4*>(xs + 4 * tquad);  // this thread's own store
-    const int idx = first + 4 * tquad + (f.x == tmax ? 0 : f.y == tmax ? 1 : f.z == tmax ? 2 : 3);
-    w0.key = static_cast<unsigned long long>(~order_of(tmax)) << 32 | static_cast<uint32_t>(idx), w0.aux = __float_as_uint(tmax);
-  }
+  if (widx != ~0u && wmax > -INFINITY) w0.key = static_cast<unsigned long long>(~order_of(wmax)) << 32 | widx, w0.aux = __float_as_uint(wmax);
   w0 = reduce(sh, w0, cs, turn);
   int token = static_cast<int>(w0.key & 0xFFFFFFFFu);  // -1 when no value is above -inf
   const float mx = __uint_as_float(w0.aux);
-  if (w0.key == ~0ull || !(temp > 0.f) || top_p <= 0.f || top_k == 1) {
+  if (w0.key == ~0ull || greedy) {
     if (rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
     if (cs > 1) sbd::cluster_sync_all();  // no CTA leaves while another may read its slot
     return;
   }
   // log2 of w; fminf gives the maximum itself 0 even where it is infinite (inf - inf)
-  const float inv = fmaxf(kLog2e / temp, 1e-37f);  // above zero, so that -inf stays -inf
   auto z2_of = [&](float x) { return fminf((x - mx) * inv, 0.f); };
   // race key of a token with random word q: its waiting time over its rate, then its index; ~0 below min_p
   auto race = [&](float x, int idx, uint32_t q) {
@@ -242,151 +282,164 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     const float u = fminf((__uint2float_rn(q) + 0.5f) * 2.3283064365386963e-10f, 0.99999994f);
     return static_cast<unsigned long long>(__float_as_uint(-log1pf(-u) / wx)) << 32 | static_cast<uint32_t>(idx);
   };
+  const Philox philox(static_cast<uint64_t>(seed), static_cast<uint32_t>(pos));
   auto word_of = [&](int idx) {
-    const uint4 r = philox(static_cast<uint32_t>(idx) >> 2, c1, k0, k1);
+    const uint4 r = philox(static_cast<uint32_t>(idx) >> 2);
     const uint32_t lo = idx & 1 ? r.y : r.x, hi = idx & 1 ? r.w : r.z;
     return idx & 2 ? hi : lo;
   };
+  auto mass_of = [&](float z2) { return static_cast<unsigned long long>(__float2uint_rn(ex2(z2) * kUnit)); };
+  auto value_bits = [](uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); };
+  auto value_of = [&](unsigned long long key) { return value_bits(~static_cast<uint32_t>(key >> 32)); };
   // a value below every x with log2 w >= c, whatever the rounding on either side
   auto floor_of = [&](float c) { return mx == INFINITY ? kLargest : fmaxf(mx + (c - 0.01f) / inv - fabsf(mx) * 0x1p-21f, -kLargest); };
-  // offsets of this CTA's values of at least `least` into list[cap]; sh.n counts them all.  Up to 32 values
-  // per thread become a bit mask, so that a warp takes its places in the list with one atomic.
-  auto collect = [&](uint16_t* list, int cap, float least, auto also) {
-    for (int i0 = 0; i0 < n4; i0 += 8 * NT) {
+  // Calls f(seg, v) with the segments of this warp that hold a value of at least `least`; the values of
+  // lanes without one are -inf.
+  auto visit = [&](float least, auto f, unsigned limit = ~0u) {
+    for (int r = 0; r < rounds; ++r) {
+      // one read for the whole warp, whose lanes have to leave together
+      if (__shfl_sync(0xFFFFFFFFu, *static_cast<volatile unsigned*>(&sh.n), 0) > limit) break;
+      const int seg = seg_of(r);
+      const bool hit = lane_max[(r * NW + warp) * 32 + lane] >= least;  // -inf past the last segment
+      if (!__any_sync(0xFFFFFFFFu, hit)) continue;
+      float v[32];
+      if (hit) {
+        load(seg, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = -INFINITY;
+      }
+      f(seg, v);
+    }
+  };
+  // the keys of this CTA's values of at least `least` into sh.list, sh.n of them; beyond LIST it gives up.  A
+  // lane's hits become a bit mask, so that a warp takes its places with one atomic.
+  auto collect = [&](float least) {
+    visit(least, [&](int seg, float (&v)[32]) {
       uint32_t hits = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = i0 + j * NT + threadIdx.x;
-        if (i < n4) {
-          const float4 f = *reinterpret_cast<const float4*>(xs + 4 * i);
-          const float v[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            hits |= v[e] >= least ? 1u << (4 * j + e) : 0u;
-            also(v[e], 4 * i + e);
-          }
-        }
-      }
+      for (int i = 0; i < 32; ++i) hits |= v[i] >= least ? 1u << i : 0u;
       const unsigned mine = __popc(hits);
       unsigned inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const unsigned v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-        if (lane >= o) inc += v;
+        const unsigned c = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += c;
       }
       unsigned base = 0;
       if (lane == 31 && inc) base = atomicAdd(&sh.n, inc);
       base = __shfl_sync(0xFFFFFFFFu, base, 31) + inc - mine;
-      if (base + mine > static_cast<unsigned>(cap)) hits = 0;  // the list will not be used
-      for (; hits; hits &= hits - 1, ++base) {
-        const int bit = __ffs(hits) - 1;
-        list[base] = static_cast<uint16_t>(4 * (i0 + (bit >> 2) * NT + threadIdx.x) + (bit & 3));
-      }
-    }
+      if (base + mine > LIST) hits = 0;  // the list will not be used
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (hits >> i & 1) sh.list[base++] = static_cast<unsigned long long>(~order_of(v[i])) << 32 | static_cast<uint32_t>(index_of(seg, i));
+    }, LIST);
     __syncthreads();
   };
 
-  uint32_t xl = 0;  // the race is among tokens that rank before (xl, il): orderable value, index
+  auto bin_of = [&](float x) { return static_cast<int>(fminf(-8.f * z2_of(x), static_cast<float>(BINS - 1))); };
+  auto count_maxima = [&] {
+    for (int r = 0; r < rounds; ++r) {
+      const float m = lane_max[(r * NW + warp) * 32 + lane];
+      if (m > -INFINITY) atomicAdd(&sh.hist[bin_of(m)], 1u);
+    }
+  };
+  // after a barrier of the cluster: thread b < BINS gets the row's count of bin b
+  auto bin_count = [&] {
+    unsigned cnt = 0;
+    for (int r = 0; r < cs; ++r) {
+      unsigned c;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(sbd::mapa_shared(sbd::smem_u32(&sh.hist[threadIdx.x]), r)) : "memory");
+      cnt += c;
+    }
+    return cnt;
+  };
+  static_assert(BINS == NT, "a bin per thread");
+  // inclusive sum over the threads
+  auto scan = [&](unsigned long long v, unsigned long long* whole) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long c = __shfl_up_sync(0xFFFFFFFFu, v, o);
+      if (lane >= o) v += c;
+    }
+    if (lane == 31) sh.warp[warp].sum = v;
+    __syncthreads();
+    *whole = 0;
+    for (int w = 0; w < NW; ++w) {
+      const unsigned long long c = sh.warp[w].sum;
+      v += w < warp ? c : 0;
+      *whole += c;
+    }
+    __syncthreads();
+    return v;
+  };
+
+  uint32_t xl = 0;  // the race is among tokens that rank before (xl, il): ranking bits, index
   int il = p.v;
   if (top_k > 0 && top_k < p.v) {
-    // ---- top-k: the bin of the threads' maxima that reaches k; every value in it or above is a candidate
-    auto bin_of = [&](float x) { return static_cast<int>(fminf(-8.f * z2_of(x), static_cast<float>(BINS - 1))); };
-    if (tquad >= 0) atomicAdd(&sh.hist[bin_of(tmax)], 1u);
+    // ---- top-k: the bin of the lanes' maxima (of all values where the maxima are too few) that reaches k;
+    // every value in it or above is a candidate
+    if (top_k <= p.v / 64) {
+      count_maxima();
+    } else {
+      visit(-kLargest, [&](int, float (&v)[32]) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (v[i] > -INFINITY) atomicAdd(&sh.hist[bin_of(v[i])], 1u);
+      });
+    }
+    if (threadIdx.x == 0) sh.bin = BINS - 1;  // not reached (fewer than k finite values): everything
     __syncthreads();
     if (cs > 1) sbd::cluster_sync_all();
-    unsigned cnt = 0;
-    if (threadIdx.x < BINS) {
-      if (cs > 1) {
-        for (int r = 0; r < cs; ++r) {
-          unsigned c;
-          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(sbd::mapa_shared(sbd::smem_u32(&sh.hist[threadIdx.x]), r)) : "memory");
-          cnt += c;
-        }
-      } else {
-        cnt = sh.hist[threadIdx.x];
-      }
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned c = __shfl_up_sync(0xFFFFFFFFu, cnt, o);
-        if (lane >= o) cnt += c;
-      }
-      if (lane == 31) sh.warp[warp].count = cnt;
-    }
-    if (threadIdx.x == 0) sh.bin = BINS - 1;  // too few maxima: everything
-    __syncthreads();
-    if (threadIdx.x < BINS) {
-      unsigned before = 0;
-      for (int x = 0; x < warp; ++x) before += sh.warp[x].count;
-      const unsigned up = __shfl_up_sync(0xFFFFFFFFu, cnt, 1);
-      const unsigned k = static_cast<unsigned>(top_k);
-      if (before + cnt >= k && (lane ? before + up : before) < k) sh.bin = threadIdx.x;
-    }
+    const unsigned cnt = bin_count();
+    unsigned long long finite;
+    const unsigned upto = static_cast<unsigned>(scan(cnt, &finite)), k = static_cast<unsigned>(top_k);
+    if (upto >= k && upto - cnt < k) sh.bin = threadIdx.x;
     __syncthreads();
     const int bin = sh.bin;
-    collect(sh.top.mine, MINE, bin == BINS - 1 ? -kLargest : floor_of(-0.125f * (bin + 1)), [](float, int) {});
+    collect(bin == BINS - 1 ? -kLargest : floor_of(-0.125f * (bin + 1)));
     const unsigned mine = sh.n;  // a list that does not fit counts as too many candidates
-    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : mine > MINE ? SORT + 1u : mine}, cs, turn).count;
+    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : mine > LIST ? SORT + 1u : mine}, cs, turn).count;
     if (total <= SORT) {
-      auto key_of = [&](int i) { return static_cast<unsigned long long>(~order_of(xs[i])) << 32 | static_cast<uint32_t>(first + i); };
       const unsigned at = sh.lower;
       if (cs > 1) {
-        const uint32_t dst = sbd::mapa_shared(sbd::smem_u32(sh.top.keys), 0);
+        const uint32_t dst = sbd::mapa_shared(sbd::smem_u32(sh.keys), 0);
         for (unsigned i = threadIdx.x; i < mine; i += NT)
-          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst + 8 * (at + i)), "l"(key_of(sh.top.mine[i])) : "memory");
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst + 8 * (at + i)), "l"(sh.list[i]) : "memory");
         sbd::cluster_sync_all();
         if (rank) return;  // from here on nobody reads this CTA's memory
       } else {
-        for (unsigned i = threadIdx.x; i < mine; i += NT) sh.top.keys[i] = key_of(sh.top.mine[i]);
+        for (unsigned i = threadIdx.x; i < mine; i += NT) sh.keys[i] = sh.list[i];
       }
       unsigned size = 2;
       while (size < total) size *= 2;
-      for (unsigned i = total + threadIdx.x; i < size; i += NT) sh.top.keys[i] = ~0ull;
+      for (unsigned i = total + threadIdx.x; i < size; i += NT) sh.keys[i] = ~0ull;
       __syncthreads();
-      unsigned long long* key = sh.top.keys;
+      unsigned long long* key = sh.keys;
       for (unsigned k = 2; k <= size; k *= 2)  // bitonic
         for (unsigned j = k / 2; j; j /= 2) {
-          if (threadIdx.x < size / 2) {
-            const unsigned a = 2 * j * (threadIdx.x / j) + threadIdx.x % j, b = a + j;
+          for (unsigned t = threadIdx.x; t < size / 2; t += NT) {
+            const unsigned a = 2 * j * (t / j) + t % j, b = a + j;
             const unsigned long long ka = key[a], kb = key[b];
             if ((ka > kb) == !(a & k)) key[a] = kb, key[b] = ka;
           }
           __syncthreads();
         }
-      // ranks 2 t and 2 t + 1 are this thread's; the mass before each
-      float x[2] = {-INFINITY, -INFINITY};
-      int idx[2] = {0, 0};
-      unsigned long long mass[2] = {0, 0};
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned r = 2 * threadIdx.x + e;
-        if (r < total && r < static_cast<unsigned>(top_k)) {
-          const uint32_t o = ~static_cast<uint32_t>(key[r] >> 32);
-          x[e] = __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
-          idx[e] = static_cast<int>(key[r] & 0xFFFFFFFFu);
-          mass[e] = __float2ull_rn(ex2(z2_of(x[e])) * kUnit);
-        }
-      }
-      unsigned long long inc = mass[0] + mass[1];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      if (lane == 31) sh.warp[warp].sum = inc;
-      __syncthreads();
-      unsigned long long before = inc - mass[0] - mass[1], all = 0;
-      for (int r = 0; r < NT / 32; ++r) {
-        const unsigned long long v = sh.warp[r].sum;
-        before += r < warp ? v : 0;
-        all += v;
-      }
-      __syncthreads();
+      // E neighbouring ranks are this thread's; the mass before each
+      constexpr int E = SORT / NT;
+      const unsigned members = min(total, static_cast<unsigned>(top_k)), r0 = E * threadIdx.x, r1 = min(r0 + E, members);
+      unsigned long long own = 0, all;
+#pragma unroll 1
+      for (unsigned r = r0; r < r1; ++r) own += mass_of(z2_of(value_of(key[r])));
+      unsigned long long before = scan(own, &all) - own;
       const double limit = static_cast<double>(top_p) * static_cast<double>(all);
       Word best{0, ~0ull, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (x[e] > -INFINITY && (top_p >= 1.f || static_cast<double>(before) < limit)) best.key = min(best.key, race(x[e], idx[e], word_of(idx[e])));
-        before += mass[e];
+#pragma unroll 1
+      for (unsigned r = r0; r < r1; ++r) {
+        const float x = value_of(key[r]);
+        const int idx = static_cast<int>(key[r] & 0xFFFFFFFFu);
+        if (x > -INFINITY && (top_p >= 1.f || static_cast<double>(before) < limit)) best.key = min(best.key, race(x, idx, word_of(idx)));
+        before += mass_of(z2_of(x));
       }
       int none = 0;
       best = reduce(sh, best, 1, none);
@@ -395,21 +448,23 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     }
     // more candidates than one CTA sorts (a large k, or thousands of equal values): the largest value that at
     // least top_k values reach, bit by bit, then the index up to which those equal to it are in
+    auto count = [&](auto in) {
+      unsigned cnt = 0;
+      visit(-INFINITY, [&](int seg, float (&v)[32]) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) cnt += index_of(seg, i) < p.v && in(order_of(v[i]), index_of(seg, i));
+      });
+      return reduce(sh, Word{0, ~0ull, 0, cnt}, cs, turn).count;
+    };
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t c = xl | 1u << bit;
-      unsigned cnt = 0;
-      for (int i = threadIdx.x; i < n; i += NT) cnt += order_of(xs[i]) >= c;
-      if (reduce(sh, Word{0, ~0ull, 0, cnt}, cs, turn).count >= static_cast<unsigned>(top_k)) xl = c;
+      if (count([&](uint32_t o, int) { return o >= c; }) >= static_cast<unsigned>(top_k)) xl = c;
     }
-    unsigned above = 0;
-    for (int i = threadIdx.x; i < n; i += NT) above += order_of(xs[i]) > xl;
-    above = reduce(sh, Word{0, ~0ull, 0, above}, cs, turn).count;
+    const unsigned above = count([&](uint32_t o, int) { return o > xl; });
     int lo = 0, hi = p.v - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      unsigned cnt = 0;
-      for (int i = threadIdx.x; i < n && first + i <= mid; i += NT) cnt += order_of(xs[i]) == xl;
-      if (above + reduce(sh, Word{0, ~0ull, 0, cnt}, cs, turn).count >= static_cast<unsigned>(top_k)) hi = mid;
+      if (above + count([&](uint32_t o, int idx) { return o == xl && idx <= mid; }) >= static_cast<unsigned>(top_k)) hi = mid;
       else lo = mid + 1;
     }
     il = lo + 1;  // ranks before (xl, il): the k in
@@ -423,76 +478,121 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
     const uint32_t o = order_of(x);
     return o > xl || (o == xl && idx < il);
   };
-  // log2 of the smallest w that can be kept (see above)
-  float cut = min_p > 0.f ? __log2f(min_p) : -INFINITY;
-  if (top_p < 1.f) cut = fmaxf(cut, __log2f((1.f - top_p) / static_cast<float>(p.v)));
-  bool listed = false;
-  Word w{0, ~0ull, 0, 0};
-  if (cut > -INFINITY) {
-    float sum = 0.f;
-    const float least = floor_of(cut);
-    if (top_p >= 1.f) collect(sh.list, LIST, least, [](float, int) {});
-    else if (all) collect(sh.list, LIST, least, [&](float x, int) { sum += ex2(z2_of(x)); });
-    else collect(sh.list, LIST, least, [&](float x, int i) { sum += in(x, first + i) ? ex2(z2_of(x)) : 0.f; });
-    w.sum = __float2ull_rn(sum * kUnit);
+  double mass = 1.0;  // of the tokens that top-p sums: all from the segments, a top-k's in round 0 of the race
+  float cut = min_p > 0.f ? __log2f(min_p) : -INFINITY;  // log2 of the smallest w that can be kept
+  if (top_p < 1.f && all) {
+    unsigned long long part = 0;
+    for (int i = threadIdx.x; i < rounds * NW; i += NT) {
+      const float2 f = seg_mass[i];
+      if (f.x > -INFINITY) part += __float2ull_rn(f.y * ex2(z2_of(f.x)) * kUnit);
+    }
+    count_maxima();
+    if (threadIdx.x == 0) sh.bin = BINS;
+    mass = static_cast<double>(reduce(sh, Word{part, ~0ull, 0, 0}, cs, turn).sum);
+    // c = 2^(-b/8): lanes whose maximum lies in bin b or below weigh at most 32 * 2^(-bin/8) each, the others 32 c.
+    // The last bin holds all that is further down, of weight below 2^-31 each, and gives no cut.
+    const unsigned cnt = bin_count();
+    unsigned long long lanes, tail;
+    const unsigned long long above = scan(cnt, &lanes) - cnt;
+    const float edge = ex2(-0.125f * threadIdx.x);
+    const unsigned long long own = __float2ull_ru(32.f * cnt * edge * kUnit);
+    const unsigned long long upto = scan(own, &tail);
+    const double weight = static_cast<double>(tail - upto + own) + 32.0 * kUnit * static_cast<double>(above) * edge;
+    if (threadIdx.x < BINS - 1 && weight * 1.001 <= (1.0 - static_cast<double>(top_p)) * mass) atomicMin(&sh.bin, static_cast<int>(threadIdx.x));
+    __syncthreads();
+    if (sh.bin < BINS) cut = fmaxf(cut, -0.125f * sh.bin);
+  }
+  const float least = cut > -INFINITY ? floor_of(cut) : -kLargest;
+  bool listed = cut > -INFINITY && all;  // as far as this CTA can tell
+  if (listed) {
+    collect(least);
     listed = sh.n <= LIST;
   }
   // The largest logit's own time bounds the winner's: it is in every race that is not empty.  A token can
-  // only win when E / w <= bound; E >= u, so nearly all are out by u > bound w, two operations and an ex2 (with
-  // a margin over what those are off); the logarithm, the exponential and the division are for the rest.
+  // only win when E / w <= bound; E >= u, so nearly all are out by u > bound w: a product, an ex2 and a
+  // comparison (with a margin over what those are off); logarithm, exponential and division are for the rest.
   const float bound = __uint_as_float(static_cast<uint32_t>(race(mx, token, word_of(token)) >> 32));
-  const float reach = __log2f(bound) + 32.01f;
-  auto loses = [&](float z2, uint32_t q) { return __uint2float_rn(q) > ex2(z2 + reach); };
-  double mass = 0.0;
-  for (int round = 0;; ++round) {
-    auto run = [&](float x, int idx, uint32_t q) {
-      const unsigned long long k = race(x, idx, q);
-      if (k < w.key) w.key = k, w.aux = order_of(x);
-    };
-    if (listed) {
-      const unsigned m = sh.n;
-      for (unsigned i = threadIdx.x; i < m; i += NT) {
-        const int at = sh.list[i], idx = first + at;
-        const float x = xs[at], z = z2_of(x);
-        if (!all) {
-          if (!in(x, idx)) continue;
-          if (round) w.sum += __float2ull_rn(ex2(z) * kUnit);
-        }
-        const uint32_t q = word_of(idx);
-        if (!loses(z, q)) run(x, idx, q);
-      }
-    } else {
-      float sum = 0.f;
-      for (int i = threadIdx.x; i < n4; i += NT) {
-        const float4 f = *reinterpret_cast<const float4*>(xs + 4 * i);
-        const float v[4] = {f.x, f.y, f.z, f.w};
-        float z[4];
+  const float reach = __log2f(bound) + 32.01f - mx * inv + fabsf(mx * inv) * 0x1p-20f;
+  auto loses = [&](float x, uint32_t q) { return __uint2float_rn(q) > ex2(fmaf(x, inv, reach)); };  // an infinite mx: NaN, may win
+  Word w{0, ~0ull, 0, 0};
+  auto run = [&](float x, int idx, uint32_t q) {
+    const unsigned long long k = race(x, idx, q);
+    if (k < w.key) w.key = k, w.aux = order_of(x);
+  };
+  // the race among values of at least `from` that rank before (xl, il)
+  auto race_all = [&](float from) {
+    visit(from, [&](int seg, float (&v)[32]) {
+      uint32_t may = 0;  // the few that may win
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = z2_of(v[e]);
+      for (int j = 0; j < 8; ++j) {
+        const int idx = index_of(seg, 4 * j);
         if (!all) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            z[e] = in(v[e], first + 4 * i + e) ? z[e] : -INFINITY;
-            sum += ex2(z[e]);
-          }
-          if (fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])) == -INFINITY) continue;
+          for (int e = 0; e < 4; ++e) v[4 * j + e] = in(v[4 * j + e], idx + e) ? v[4 * j + e] : -INFINITY;
+          if (fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3])) == -INFINITY) continue;
         }
-        const uint4 r = philox(static_cast<uint32_t>(first / 4 + i), c1, k0, k1);
+        const uint4 r = philox(static_cast<uint32_t>(idx) >> 2);
         const uint32_t q[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!loses(z[e], q[e]) && z[e] > -INFINITY) run(v[e], first + 4 * i + e, q[e]);
+        for (int e = 0; e < 4; ++e) may |= v[4 * j + e] > -INFINITY && !loses(v[4 * j + e], q[e]) ? 1u << (4 * j + e) : 0u;
       }
-      if (round) w.sum = __float2ull_rn(sum * kUnit);
+      for (; may; may &= may - 1) {  // read again: this path is rare, and one copy of it keeps the loop above in the instruction cache
+        const int idx = index_of(seg, __ffs(may) - 1);
+        run(fetch(idx), idx, word_of(idx));
+      }
+    });
+  };
+  // the mass of what ranks before (xl, il); lanes below it are not read again
+  auto mass_all = [&] {
+    visit(fmaxf(-kLargest, value_bits(xl)), [&](int seg, float (&v)[32]) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (in(v[i], index_of(seg, i))) w.sum += mass_of(z2_of(v[i]));
+    });
+  };
+  // from the list both at once
+  auto race_list = [&] {
+    const unsigned m = sh.n;
+    for (unsigned i = threadIdx.x; i < m; i += NT) {
+      const unsigned long long key = sh.list[i];
+      const int idx = static_cast<int>(key & 0xFFFFFFFFu);
+      const float x = value_of(key);
+      if (!all) {
+        if (!in(x, idx)) continue;
+        w.sum += mass_of(z2_of(x));
+      }
+      const uint32_t q = word_of(idx);
+      if (!loses(x, q)) run(x, idx, q);
     }
-    w = reduce(sh, w, cs, turn);
-    if (round && (w.key == ~0ull || static_cast<double>(w.sum) < static_cast<double>(top_p) * mass)) break;  // the last winner stands
-    token = static_cast<int>(w.key & 0xFFFFFFFFu);
-    if (top_p >= 1.f) break;
-    if (!round) mass = static_cast<double>(w.sum);
-    // next: what ranks before the winner, its mass and the winner among it
+  };
+  const Word none{0, ~0ull, 0, 0};
+  if (listed) {
+    race_list();
+  } else {
+    if (top_p < 1.f && !all) mass_all();  // of a top-k
+    race_all(least);
+  }
+  // the steps below are the same in all CTAs of the cluster: from lists only if every CTA's candidates fit one
+  w.count = threadIdx.x == 0 && !listed ? 1u : 0u;
+  w = reduce(sh, w, cs, turn);
+  listed = w.count == 0;
+  if (!all) mass = static_cast<double>(w.sum);
+  token = static_cast<int>(w.key & 0xFFFFFFFFu);
+  while (top_p < 1.f) {
+    // the mass before the winner; below p of the whole it stands, else the race goes on among what ranks before it
     xl = w.aux, il = token, all = false;
-    w = Word{0, ~0ull, 0, 0};
+    w = none;
+    if (listed) race_list();
+    else mass_all();
+    w = reduce(sh, w, cs, turn);
+    if (static_cast<double>(w.sum) < static_cast<double>(top_p) * mass) break;
+    if (!listed) {
+      w = none;
+      race_all(fmaxf(least, value_bits(xl)));
+      w = reduce(sh, w, cs, turn);
+    }
+    if (w.key == ~0ull) break;  // nothing before it
+    token = static_cast<int>(w.key & 0xFFFFFFFFu);
   }
   if (rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
   if (cs > 1) sbd::cluster_sync_all();  // no CTA leaves while another may read its slot
@@ -500,12 +600,13 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams p) {
 
 template <typename T>
 int launch_sample(SampleParams& p, int rows, int cs, cudaStream_t stream) {
-  const int smem = p.slice * 4;
+  const int local = (p.segs + cs * NW - 1) / (cs * NW) * NW;  // segments of a CTA
+  const int smem = local * (32 * 4 + 8);
   static bool set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SLICE * 4);
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_V / SEG * (32 * 4 + 8));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return sb::cuda_fail(e, "sample_kernel attributes");
     if (dev >= 0 && dev < 64) set[dev] = true;
@@ -533,10 +634,11 @@ int launch_sample(SampleParams& p, int rows, int cs, cudaStream_t stream) {
 
 extern "C" int sb_sample(const void* logits, int dtype, int64_t ld, int rows, int vocab, const int64_t* seeds,
                          const int32_t* pos, const float* temperature, const int32_t* top_k, const float* top_p,
-                         const float* min_p, int32_t* tokens, void* stream) {
+                         const float* min_p, float softcap, int32_t* tokens, void* stream) {
   SB_CHECK_ARG(dtype == SB_F16 || dtype == SB_BF16 || dtype == SB_F32, "sb_sample: bad logits dtype");
-  SB_CHECK_ARG(rows >= 0 && rows <= 65535 && vocab >= 1 && vocab <= MAX_CS * MAX_SLICE,
-               "sb_sample: %d rows of %d logits (at most 65535 rows, %d logits)", rows, vocab, MAX_CS * MAX_SLICE);
+  SB_CHECK_ARG(rows >= 0 && rows <= 65535 && vocab >= 1 && vocab <= MAX_V,
+               "sb_sample: %d rows of %d logits (at most 65535 rows, %d logits)", rows, vocab, MAX_V);
+  SB_CHECK_ARG(softcap >= 0.f && softcap <= kLargest, "sb_sample: softcap must be 0 (off) or positive and finite");
   SB_CHECK_ARG(rows <= 1 || ld >= vocab, "sb_sample: ld is shorter than a row");
   if (rows == 0) return SB_OK;
   SB_CHECK_ARG(logits && seeds && pos && tokens, "sb_sample: null pointer");
@@ -546,10 +648,12 @@ extern "C" int sb_sample(const void* logits, int dtype, int64_t ld, int rows, in
   p.x = logits, p.ld = ld, p.v = vocab, p.seeds = seeds, p.pos = pos, p.temperature = temperature, p.top_k = top_k;
   p.top_p = top_p, p.min_p = min_p, p.tokens = tokens;
   p.vec = sb::aligned(logits, 4 * size) && (rows == 1 || ld % 4 == 0);
-  // CTAs per row: as many as leave 1024 values or more to each, up to 16
+  p.segs = (vocab + SEG - 1) / SEG;
+  p.softcap = softcap;
+  // CTAs per row: four segments per warp, so that rows that need every random word spread over several SMs;
+  // fewer segments, down to one, while the CTAs do not fill the GPU
   int cs = 1;
-  while (cs < MAX_CS && vocab > cs * 1024) cs *= 2;
-  p.slice = ((vocab + cs - 1) / cs + 3) / 4 * 4;
+  while (cs < MAX_CS && p.segs >= cs * 2 * NW * (static_cast<int64_t>(rows) * cs * 2 <= CTAS * sb::num_sms() ? 1 : 4)) cs *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == SB_F32) return launch_sample<float>(p, rows, cs, s);
   if (dtype == SB_F16) return launch_sample<__half>(p, rows, cs, s);

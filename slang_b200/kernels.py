@@ -800,9 +800,10 @@ def _step(t: torch.Tensor, dim: int) -> int:
 
 def sample(logits: torch.Tensor, seeds: torch.Tensor, pos: torch.Tensor, temperature: torch.Tensor | None = None,
            top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
-           tokens: torch.Tensor | None = None) -> torch.Tensor:
+           softcap: float = 0.0, tokens: torch.Tensor | None = None) -> torch.Tensor:
     """Draw one token per row of ``logits`` [rows, vocab] (``sb_sample``): temperature, then
     top-k, then top-p, then min-p, each a per-row tensor on the device or None for off.
+    ``softcap`` > 0 caps the logits first (softcap * tanh(x / softcap)).
     ``seeds`` [rows] int64 and ``pos`` [rows] int32 decide the draw: the same seed,
     position and logits give the same token.  Returns int32 tokens, -1 for a row whose
     logits are all -inf."""
@@ -818,6 +819,6 @@ def sample(logits: torch.Tensor, seeds: torch.Tensor, pos: torch.Tensor, tempera
     _lib.call("sb_sample", logits.data_ptr(), dtype, logits.stride(0) if rows > 1 else vocab, rows, vocab,
               _vec(seeds, "seeds", _I64, rows, gpu), _vec(pos, "pos", _I32, rows, gpu),
               _vec(temperature, "temperature", _F32T, rows, gpu), _vec(top_k, "top_k", _I32, rows, gpu),
-              _vec(top_p, "top_p", _F32T, rows, gpu), _vec(min_p, "min_p", _F32T, rows, gpu),
+              _vec(top_p, "top_p", _F32T, rows, gpu), _vec(min_p, "min_p", _F32T, rows, gpu), softcap,
               _vec(tokens, "tokens", _I32, rows, gpu), _raw_stream(gpu))
     return tokens
