@@ -20,12 +20,15 @@
 // the rows are few) exchange a few words through distributed shared memory.  The
 // one pass over the row leaves each lane's maximum of its 32 values of a segment
 // and each segment's mass in shared memory; what follows reads again only the
-// lanes whose maximum can matter, mostly from the L2 cache, and keeps short lists:
+// lanes whose maximum can matter, mostly from the L2 cache:
+//   the race      needs every token's random word, but no logit: a token can win only
+//                 if u <= t w, where t is a time already reached and w at most
+//                 that of its lane's maximum, one integer comparison per word.
+//                 Only the few that pass are read and get their logarithm.
+//   top-p         one pass sums what ranks before the winner.  A token below (1 - p) / V of
+//                 the total is out from the start: all such tokens together
+//                 weigh less than 1 - p, so the prefix above them holds the nucleus.
 //   min-p         a token below w = min_p is out.
-//   top-p         a token below w = c is out when all such tokens together weigh no more
-//                 than 1 - p of the total: the prefix above them already holds the
-//                 nucleus.  A lane's 32 values weigh at most 32 min(c, w of its maximum)
-//                 there, so a histogram of the maxima gives a good c.
 //   top-k         the k-th largest of the lanes' maxima is a lower bound of
 //                 the k-th largest value; what reaches it (a little more than
 //                 k tokens) is sorted by one CTA, which finishes the row alone.
@@ -45,9 +48,6 @@ constexpr int SEG = 1024;       // values per segment: 32 per lane, in 8 vectors
 constexpr int MAX_V = 800 * SEG;  // 25600 lane maxima: 100 KB in one CTA
 constexpr int BINS = 256;       // of maxima, 1/8 octave of w each
 constexpr int SORT = 1024;      // candidates of a top-k row that one CTA sorts
-// Candidates per CTA of other rows.  Beyond this many a pass over all values costs
-// no more: one Philox call serves four values there, one here.
-constexpr int LIST = 3072;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLargest = 3.402823466e38f;  // bounds stay finite: -inf (banned, padding) is below them
 constexpr float kUnit = 2147483648.f;        // masses in units of 2^-31 of the largest token's
@@ -91,7 +91,7 @@ struct Shared {
   unsigned int n;      // entries of this CTA's list
   int bin;
   unsigned int hist[BINS];
-  unsigned long long list[LIST];  // (inverted ranking bits, index): smaller ranks before
+  unsigned long long list[SORT];  // candidates here: (inverted ranking bits, index), smaller ranks before
   unsigned long long keys[SORT];  // a top-k row's, in the CTA of rank 0
 };
 
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
       f(seg, v);
     }
   };
-  // the keys of this CTA's values of at least `least` into sh.list, sh.n of them; beyond LIST it gives up.  A
+  // the keys of this CTA's values of at least `least` into sh.list, sh.n of them; beyond SORT it gives up.  A
   // lane's hits become a bit mask, so that a warp takes its places with one atomic.
   auto collect = [&](float least) {
     visit(least, [&](int seg, float (&v)[32]) {
@@ -329,11 +329,11 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
       unsigned base = 0;
       if (lane == 31 && inc) base = atomicAdd(&sh.n, inc);
       base = __shfl_sync(0xFFFFFFFFu, base, 31) + inc - mine;
-      if (base + mine > LIST) hits = 0;  // the list will not be used
+      if (base + mine > SORT) hits = 0;  // the list will not be used
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (hits >> i & 1) sh.list[base++] = static_cast<unsigned long long>(~order_of(v[i])) << 32 | static_cast<uint32_t>(index_of(seg, i));
-    }, LIST);
+    }, SORT);
     __syncthreads();
   };
 
@@ -398,8 +398,8 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
     __syncthreads();
     const int bin = sh.bin;
     collect(bin == BINS - 1 ? -kLargest : floor_of(-0.125f * (bin + 1)));
-    const unsigned mine = sh.n;  // a list that does not fit counts as too many candidates
-    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : mine > LIST ? SORT + 1u : mine}, cs, turn).count;
+    const unsigned mine = sh.n;
+    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : min(mine, SORT + 1u)}, cs, turn).count;
     if (total <= SORT) {
       const unsigned at = sh.lower;
       if (cs > 1) {
@@ -478,69 +478,49 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
     const uint32_t o = order_of(x);
     return o > xl || (o == xl && idx < il);
   };
-  double mass = 1.0;  // of the tokens that top-p sums: all from the segments, a top-k's in round 0 of the race
-  float cut = min_p > 0.f ? __log2f(min_p) : -INFINITY;  // log2 of the smallest w that can be kept
-  if (top_p < 1.f && all) {
-    unsigned long long part = 0;
-    for (int i = threadIdx.x; i < rounds * NW; i += NT) {
-      const float2 f = seg_mass[i];
-      if (f.x > -INFINITY) part += __float2ull_rn(f.y * ex2(z2_of(f.x)) * kUnit);
-    }
-    count_maxima();
-    if (threadIdx.x == 0) sh.bin = BINS;
-    mass = static_cast<double>(reduce(sh, Word{part, ~0ull, 0, 0}, cs, turn).sum);
-    // c = 2^(-b/8): lanes whose maximum lies in bin b or below weigh at most 32 * 2^(-bin/8) each, the others 32 c.
-    // The last bin holds all that is further down, of weight below 2^-31 each, and gives no cut.
-    const unsigned cnt = bin_count();
-    unsigned long long lanes, tail;
-    const unsigned long long above = scan(cnt, &lanes) - cnt;
-    const float edge = ex2(-0.125f * threadIdx.x);
-    const unsigned long long own = __float2ull_ru(32.f * cnt * edge * kUnit);
-    const unsigned long long upto = scan(own, &tail);
-    const double weight = static_cast<double>(tail - upto + own) + 32.0 * kUnit * static_cast<double>(above) * edge;
-    if (threadIdx.x < BINS - 1 && weight * 1.001 <= (1.0 - static_cast<double>(top_p)) * mass) atomicMin(&sh.bin, static_cast<int>(threadIdx.x));
-    __syncthreads();
-    if (sh.bin < BINS) cut = fmaxf(cut, -0.125f * sh.bin);
-  }
+  // log2 of the smallest w that can be kept (see above; the total is at least the largest token's 1)
+  float cut = min_p > 0.f ? __log2f(min_p) : -INFINITY;
+  if (top_p < 1.f) cut = fmaxf(cut, __log2f((1.f - top_p) / static_cast<float>(p.v)));
   const float least = cut > -INFINITY ? floor_of(cut) : -kLargest;
-  bool listed = cut > -INFINITY && all;  // as far as this CTA can tell
-  if (listed) {
-    collect(least);
-    listed = sh.n <= LIST;
-  }
-  // The largest logit's own time bounds the winner's: it is in every race that is not empty.  A token can
-  // only win when E / w <= bound; E >= u, so nearly all are out by u > bound w: a product, an ex2 and a
-  // comparison (with a margin over what those are off); logarithm, exponential and division are for the rest.
+  // The largest logit's own time bounds the winner's: it is in every race that is not empty.  E >= u, so a token
+  // with u > bound w is out (with a margin over what ex2 and the product are off).
   const float bound = __uint_as_float(static_cast<uint32_t>(race(mx, token, word_of(token)) >> 32));
-  const float reach = __log2f(bound) + 32.01f - mx * inv + fabsf(mx * inv) * 0x1p-20f;
-  auto loses = [&](float x, uint32_t q) { return __uint2float_rn(q) > ex2(fmaf(x, inv, reach)); };  // an infinite mx: NaN, may win
+  const float reach = __log2f(bound) + 32.01f;  // 2^(reach + log2 w): the largest word that may win
   Word w{0, ~0ull, 0, 0};
-  auto run = [&](float x, int idx, uint32_t q) {
+  auto enter = [&](int idx) {
+    if (idx >= p.v) return;  // padding of the last segment
+    const float x = fetch(idx);
+    const uint32_t q = word_of(idx);
+    if (x == -INFINITY || !(all || in(x, idx)) || __uint2float_rn(q) > ex2(z2_of(x) + reach)) return;
     const unsigned long long k = race(x, idx, q);
     if (k < w.key) w.key = k, w.aux = order_of(x);
   };
   // the race among values of at least `from` that rank before (xl, il)
   auto race_all = [&](float from) {
-    visit(from, [&](int seg, float (&v)[32]) {
-      uint32_t may = 0;  // the few that may win
+    for (int r = 0; r < rounds; ++r) {
+      const float m = lane_max[(r * NW + warp) * 32 + lane];  // -inf past the last segment
+      const bool hit = m >= from;
+      if (!__any_sync(0xFFFFFFFFu, hit)) continue;
+      const uint32_t top = __float2uint_ru(ex2(z2_of(m) + reach));
+      const int seg = seg_of(r);
+      uint32_t may = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int idx = index_of(seg, 4 * j);
-        if (!all) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * j + e] = in(v[4 * j + e], idx + e) ? v[4 * j + e] : -INFINITY;
-          if (fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3])) == -INFINITY) continue;
-        }
-        const uint4 r = philox(static_cast<uint32_t>(idx) >> 2);
-        const uint32_t q[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) may |= v[4 * j + e] > -INFINITY && !loses(v[4 * j + e], q[e]) ? 1u << (4 * j + e) : 0u;
+        const uint4 q = philox(static_cast<uint32_t>(index_of(seg, 4 * j)) >> 2);
+        may |= (q.x <= top ? 1u << (4 * j) : 0u) | (q.y <= top ? 2u << (4 * j) : 0u) | (q.z <= top ? 4u << (4 * j) : 0u) |
+               (q.w <= top ? 8u << (4 * j) : 0u);
       }
-      for (; may; may &= may - 1) {  // read again: this path is rare, and one copy of it keeps the loop above in the instruction cache
-        const int idx = index_of(seg, __ffs(may) - 1);
-        run(fetch(idx), idx, word_of(idx));
+      // These are read.  A lane of a likely token passes most of its words: the warp takes its values side by
+      // side, one latency for all; the stray ones of other lanes are their own.
+      if (!hit) may = 0;
+      for (unsigned busy = __ballot_sync(0xFFFFFFFFu, __popc(may) > 2); busy; busy &= busy - 1) {
+        const int of = __ffs(busy) - 1;
+        const uint32_t his = __shfl_sync(0xFFFFFFFFu, may, of);
+        if (his >> lane & 1) enter(index_of(seg, lane) + 4 * (of - lane));
+        if (lane == of) may = 0;
       }
-    });
+      for (; may; may &= may - 1) enter(index_of(seg, __ffs(may) - 1));
+    }
   };
   // the mass of what ranks before (xl, il); lanes below it are not read again
   auto mass_all = [&] {
@@ -550,47 +530,30 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
         if (in(v[i], index_of(seg, i))) w.sum += mass_of(z2_of(v[i]));
     });
   };
-  // from the list both at once
-  auto race_list = [&] {
-    const unsigned m = sh.n;
-    for (unsigned i = threadIdx.x; i < m; i += NT) {
-      const unsigned long long key = sh.list[i];
-      const int idx = static_cast<int>(key & 0xFFFFFFFFu);
-      const float x = value_of(key);
-      if (!all) {
-        if (!in(x, idx)) continue;
-        w.sum += mass_of(z2_of(x));
+  if (top_p < 1.f) {  // the whole: of all tokens from the segments, of a top-k's by a pass
+    if (all) {
+      for (int i = threadIdx.x; i < rounds * NW; i += NT) {
+        const float2 f = seg_mass[i];
+        if (f.x > -INFINITY) w.sum += __float2ull_rn(f.y * ex2(z2_of(f.x)) * kUnit);
       }
-      const uint32_t q = word_of(idx);
-      if (!loses(x, q)) run(x, idx, q);
+    } else {
+      mass_all();
     }
-  };
-  const Word none{0, ~0ull, 0, 0};
-  if (listed) {
-    race_list();
-  } else {
-    if (top_p < 1.f && !all) mass_all();  // of a top-k
-    race_all(least);
   }
-  // the steps below are the same in all CTAs of the cluster: from lists only if every CTA's candidates fit one
-  w.count = threadIdx.x == 0 && !listed ? 1u : 0u;
+  race_all(least);
   w = reduce(sh, w, cs, turn);
-  listed = w.count == 0;
-  if (!all) mass = static_cast<double>(w.sum);
   token = static_cast<int>(w.key & 0xFFFFFFFFu);
+  const double enough = static_cast<double>(top_p) * static_cast<double>(w.sum);
   while (top_p < 1.f) {
     // the mass before the winner; below p of the whole it stands, else the race goes on among what ranks before it
     xl = w.aux, il = token, all = false;
-    w = none;
-    if (listed) race_list();
-    else mass_all();
+    w = Word{0, ~0ull, 0, 0};
+    mass_all();
     w = reduce(sh, w, cs, turn);
-    if (static_cast<double>(w.sum) < static_cast<double>(top_p) * mass) break;
-    if (!listed) {
-      w = none;
-      race_all(fmaxf(least, value_bits(xl)));
-      w = reduce(sh, w, cs, turn);
-    }
+    if (static_cast<double>(w.sum) < enough) break;
+    w = Word{0, ~0ull, 0, 0};
+    race_all(fmaxf(least, value_bits(xl)));
+    w = reduce(sh, w, cs, turn);
     if (w.key == ~0ull) break;  // nothing before it
     token = static_cast<int>(w.key & 0xFFFFFFFFu);
   }
@@ -650,10 +613,10 @@ extern "C" int sb_sample(const void* logits, int dtype, int64_t ld, int rows, in
   p.vec = sb::aligned(logits, 4 * size) && (rows == 1 || ld % 4 == 0);
   p.segs = (vocab + SEG - 1) / SEG;
   p.softcap = softcap;
-  // CTAs per row: four segments per warp, so that rows that need every random word spread over several SMs;
-  // fewer segments, down to one, while the CTAs do not fill the GPU
+  // CTAs per row: as many as make about seven per SM in all, while each warp has a segment.  128 rows of 262144
+  // with mixed settings: 8 per row
   int cs = 1;
-  while (cs < MAX_CS && p.segs >= cs * 2 * NW * (static_cast<int64_t>(rows) * cs * 2 <= CTAS * sb::num_sms() ? 1 : 4)) cs *= 2;
+  while (cs < MAX_CS && p.segs >= cs * 2 * NW && static_cast<int64_t>(rows) * cs * 2 <= 7 * sb::num_sms()) cs *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == SB_F32) return launch_sample<float>(p, rows, cs, s);
   if (dtype == SB_F16) return launch_sample<__half>(p, rows, cs, s);
