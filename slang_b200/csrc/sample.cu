@@ -41,7 +41,7 @@
 namespace {
 
 constexpr int NT = 256;         // threads per CTA
-constexpr int CTAS = 3;         // CTAs per SM
+constexpr int CTAS = 4;         // CTAs per SM
 constexpr int NW = NT / 32;
 constexpr int MAX_CS = 16;      // CTAs per row
 constexpr int SEG = 1024;       // values per segment: 32 per lane, in 8 vectors
