@@ -2,24 +2,37 @@
 // sequences of different lengths end to end in one tensor, grouped heads, a
 // sliding window, more keys than queries (a cached prefix).
 //
-// The rows of a query tile are (token, query head of the kv head's group), 128 /
-// group tokens of all heads that share K and V, so each K/V block serves the
-// whole group.  A CTA owns NQ tiles of 128 rows (two for head_dim 64 and 128,
-// one for 256) and walks the key blocks of 128 that its tokens see:
-//   warp 0        TMA: the Q tiles once, then K and V through a ring of slots.
-//   warp 1        one thread issues tcgen05.mma: S = Q K^T (both operands in
-//                 shared memory) and O += P V (P from tensor memory).
+// The rows of a query tile are (token, query head of the kv head's group): 128 /
+// group tokens of all heads that share K and V, so each K/V block of 128 keys
+// serves the whole group.  Two kernels:
+//
+// attn_packed_pair_kernel (head_dim 128 and 256): a CTA pair (cta_group::2) takes
+// two query tiles, one per CTA.  The pair's MMAs run over 256 rows; each CTA holds
+// 64 of a block's keys and half of its values' dims, so a block is loaded and read
+// from shared memory half as often.  One CTA alone is bound by shared memory,
+// not by its tensor cores: at head_dim 256 a block costs it 128 KB of operand reads for
+// Q K^T, 64 KB for P V and 128 KB of TMA writes, 2560 cycles at 128 bytes per cycle
+// against 2048 of MMA (measured 1.70 us = 3200 cycles); the pair needs 1536.
+//   warp 0        TMA: this CTA's Q tile, then its halves of K and V through a ring
+//                 of slots whose arrival is counted in the even CTA.
+//   warp 1        even CTA, one thread: tcgen05.mma S = Q K^T, then O += P V (P from
+//                 tensor memory).
 //   warps 2, 3    zero the V rows past the sequence's end in its last block: those
 //                 rows belong to another sequence, and 0 times a NaN there would
 //                 reach this one.
-//   warps 4 ...   softmax, a thread per query row of its tile: the row's 128
-//                 scores from tensor memory, running maximum m (raised, with O
-//                 rescaled, only when a score passes it by 2^8) and sum l,
-//                 p = 2^(s - m) in the input type back into the scores' columns.
-// While the softmax works on one block the tensor cores run the other tile's
-// products (two tiles), or the next block's scores (one tile, two score
-// buffers).  The issuing thread's MMAs execute in order, so a score buffer may
-// be overwritten by an MMA issued after the one that reads the P in it.
+//   warps 4 .. 7  softmax, a thread per query row: the row's 128 scores from tensor
+//                 memory, running maximum m (raised, with O rescaled, only when a
+//                 score passes it by 2^8) and sum l, p = 2^(s - m) in the input
+//                 type back into the scores' columns.
+// At 256, tensor memory holds O and two score buffers: the next block's scores are
+// issued before this block's P V.  At 128, two pairs fit an SM pair, and one's
+// MMAs run under the other's softmax, prologue and output.
+//
+// attn_packed_64_kernel (head_dim 64): one CTA takes two query tiles, each with its
+// own softmax warps; while one tile is in its softmax the other's products run.
+//
+// MMAs execute in the order of their issue, so a score buffer may be
+// overwritten by an MMA issued after the one that reads the P in it.
 //
 // Work per 128 x 128 block and head dim HD: 2 * 128 * 128 * HD multiply-adds = 8 HD
 // cycles at 4096 per cycle and SM, and 128 * 128 exponentials = 1024 cycles at 16:
@@ -43,19 +56,30 @@ constexpr int KB = 128;  // keys per block
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRise = 8.f;  // log2 units: p stays below 2^8
 
-template <int HD>
-struct Cfg {
-  static constexpr int NQ = HD == 256 ? 1 : 2;
+// head_dim 64, one CTA
+struct Cfg64 {
+  static constexpr int HD = 64, NQ = 2;
   static constexpr int THREADS = 128 + 128 * NQ;
   static constexpr int Q_BYTES = QR * HD * 2;
-  static constexpr int SLOT = HD == 64 ? 16384 : 32768;  // a K block, or half of one (256)
-  static constexpr int PER = KB * HD * 2 / SLOT;         // slots per K or V block
-  static constexpr int NSLOT = HD == 64 ? 8 : 5;
-  static constexpr int VK = KB / PER;  // keys of V per slot
+  static constexpr int SLOT = KB * HD * 2;  // a block of K or of V
+  static constexpr int NSLOT = 8;
   static constexpr int OFF_SLOT = NQ * Q_BYTES;
   static constexpr int OFF_BAR = OFF_SLOT + NSLOT * SLOT;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment slack
   static constexpr uint32_t TM_S = NQ * HD;          // S buffers (and P) after the O accumulators
+};
+
+// head_dim 128 and 256, a CTA pair
+template <int HD>
+struct PairCfg {
+  static constexpr int CTAS = HD == 256 ? 1 : 2;  // per SM
+  static constexpr int SB = HD == 256 ? 2 : 1;    // score buffers
+  static constexpr int Q_BYTES = QR * HD * 2;
+  static constexpr int SLOT = KB / 2 * HD * 2;    // this CTA's half of a block of K or of V
+  static constexpr int NSLOT = HD == 256 ? 5 : 4;
+  static constexpr int OFF_BAR = Q_BYTES + NSLOT * SLOT;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static constexpr uint32_t TM_S = HD, TM_COLS = HD == 256 ? 512 : 256;
 };
 
 struct Bars {
@@ -68,7 +92,7 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 256, "barrier block");
 
-struct Tile {  // one CTA's queries, as sb_attn_packed_plan lays them out
+struct Tile {  // two query tiles, as sb_attn_packed_plan lays them out
   int q0, n_tok, k0, k_len, pos0, pad[3];
 };
 
@@ -80,6 +104,16 @@ struct PackedParams {
   int t_q, t_k, nkv, group, tpt, window;
   float scale2;  // scale * log2(e)
 };
+
+// 32 lanes x 16 consecutive columns (thread t -> lane base + t).
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -103,18 +137,371 @@ __device__ __forceinline__ bool drain_wait(uint64_t* bar, uint32_t parity) {
   return true;
 }
 
+// Both operands f16, or both bf16.
 template <typename T>
-constexpr uint32_t idesc(int n, int b_mn) {
-  const uint32_t bf = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;
-  return sbd::umma_idesc_f16(QR, n, 0, b_mn) | bf << 7 | bf << 10;
+constexpr uint32_t idesc(int m, int n, int b_mn) {
+  const uint32_t bf = std::is_same<T, __half>::value ? 0u : 1u;
+  return sbd::umma_idesc_f16(m, n, 0, b_mn) | bf << 7 | bf << 10;
+}
+
+// The pair's forms: completion counted on a barrier of the pair's even CTA (`bar`: a shared::cluster address), and
+// both operands from shared memory (A: this CTA's 128 rows in each CTA; B: N / 2 rows in each).
+__device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, uint32_t bar, void* dst, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(sbd::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ss_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                 uint32_t accumulate) {
+  const uint32_t z = 0;  // no output lanes disabled
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z)
+      : "memory");
+}
+
+// One query row's part in a block: masks the scores (keys [lo, hi) of the sequence; `whole`: all of them), raises
+// the running maximum and rescales O where a score asks for it, writes P over the scores and adds to the sum.
+// Warp-collective; false when a wait failed.
+template <typename T, int HD>
+__device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t to, int kb, int lo, int hi, bool whole, float scale2,
+                                              float& m, float& l, uint64_t* pv_done, uint32_t pv_parity,
+                                              volatile int* abort, int* err) {
+  uint32_t sv[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) sbd::tmem_ld_32x32b_x32(ts + 32 * c, sv[c]);
+  sbd::tmem_wait_ld();
+  if (!whole) {
+    const int v0 = lo - kb, v1 = hi - kb;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sv[c][e] = 32 * c + e >= v0 && 32 * c + e < v1 ? sv[c][e] : 0xFF800000u;  // -inf
+  }
+  float mx[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    mx[c] = __uint_as_float(sv[c][0]);
+#pragma unroll
+    for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(sv[c][e]));
+  }
+  const float mx2 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+  const bool start = m == -INFINITY;  // O is still zero in this row
+  const bool rise = !start && mx2 > m + kRise;
+  if (__any_sync(0xFFFFFFFFu, rise)) {
+    // O += P V of the block before has to be complete before it is scaled
+    if (!__all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(pv_done, pv_parity, abort, err))) return false;
+    sbd::tc_fence_after();
+    const float alpha = rise ? ex2(m - mx2) : 1.f;
+#pragma unroll 1
+    for (int c = 0; c < HD / 16; ++c) {
+      uint32_t ov[16];
+      tmem_ld_x16(to + 16 * c, ov);
+      sbd::tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+      sbd::tmem_st_32x32b_x16(to + 16 * c, ov);
+    }
+    sbd::tmem_wait_st();
+    l *= alpha;
+  }
+  if (start || rise) m = mx2;
+  const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t pk[16];
+    float ls[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p0 = ex2(fmaf(__uint_as_float(sv[c][2 * e]), scale2, -mu));
+      const float p1 = ex2(fmaf(__uint_as_float(sv[c][2 * e + 1]), scale2, -mu));
+      ls[0] += p0;
+      ls[1] += p1;
+      pk[e] = sbp::pack2<T>(p0, p1);
+    }
+    l += ls[0] + ls[1];
+    sbd::tmem_st_32x32b_x16(ts + 16 * c, pk);
+  }
+  sbd::tmem_wait_st();
+  sbd::tc_fence_before();
+  return true;
+}
+
+// A finished row: O / l to memory (zeros where the row saw no key).  Warp-collective.
+template <typename T, int HD>
+__device__ __forceinline__ void store_row(uint32_t to, float l, T* dst, bool store) {
+  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+#pragma unroll
+  for (int c = 0; c < HD / 32; ++c) {
+    uint32_t ov[32];
+    sbd::tmem_ld_32x32b_x32(to + 32 * c, ov);
+    sbd::tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        w[q] = l == 0.f ? 0u : sbp::pack2<T>(__uint_as_float(ov[e + 2 * q]) * inv, __uint_as_float(ov[e + 2 * q + 1]) * inv);
+      if (store) *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// Zeroes rows [from, KB) of a V block of `boxes` boxes [KB rows x 128 bytes]: whole rows, the swizzle only permutes
+// inside them.  64 threads.
+__device__ __forceinline__ void zero_rows(uint8_t* vs, int boxes, int from, int thread) {
+  for (int b = 0; b < boxes; ++b)
+    for (int x = from * 8 + thread; x < KB * 8; x += 64) *reinterpret_cast<uint4*>(vs + b * (KB * 128) + x * 16) = make_uint4(0, 0, 0, 0);
+  sbd::fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// A query row as its softmax thread sees it.
+struct Row {
+  int tok, head;           // of its tile and of the group
+  int lo, hi;              // keys [lo, hi) of the sequence
+  int all_lo, all_hi;      // keys that every row of the tile sees
+  bool ok;
+};
+__device__ __forceinline__ Row row_of(const PackedParams& p, const Tile& tl, int i, int row, int k_len) {
+  Row r;
+  r.tok = row / p.group, r.head = row - r.tok * p.group;
+  const int n_tok = min(p.tpt, tl.n_tok - i * p.tpt), pos0 = tl.pos0 + i * p.tpt, pos = pos0 + r.tok;
+  r.ok = r.tok < n_tok;
+  r.hi = r.ok ? min(pos + 1, k_len) : 0;
+  r.lo = p.window > 0 ? pos + 1 - p.window : 0;
+  r.all_hi = min(pos0 + 1, k_len);
+  r.all_lo = p.window > 0 ? pos0 + n_tok - p.window : 0;
+  return r;
+}
+
+// Key blocks [j0, j0 + nb[i]) of the CTA's or the pair's tiles.
+__device__ __forceinline__ void block_range(const PackedParams& p, const Tile& tl, int k_len, int* j0, int (&nb)[2]) {
+  *j0 = p.window > 0 ? max(0, tl.pos0 + 1 - p.window) / KB : 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int n = min(p.tpt, tl.n_tok - i * p.tpt);
+    const int last = min(tl.pos0 + i * p.tpt + n - 1, k_len - 1);  // the tile's furthest key
+    nb[i] = n > 0 ? max(0, (last >= 0 ? last / KB + 1 : 0) - *j0) : 0;
+  }
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
-    attn_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                       const __grid_constant__ CUtensorMap tmV, const PackedParams p) {
-  using C = Cfg<HD>;
-  constexpr int NQ = C::NQ, PER = C::PER, NSLOT = C::NSLOT;
+__global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
+    attn_packed_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                            const __grid_constant__ CUtensorMap tmV, const PackedParams p) {
+  using C = PairCfg<HD>;
+  constexpr int SB = C::SB, NSLOT = C::NSLOT;
+  constexpr uint16_t kBoth = 3;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + C::OFF_BAR);
+  volatile int* abort = &bars->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(sbd::cluster_ctarank());
+  const bool lead = rank == 0;
+  sbd::griddep_launch_dependents();
+  const int kv = (blockIdx.x >> 1) % p.nkv;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      sbd::mbar_init(&bars->s_full[i], 1);
+      sbd::mbar_init(&bars->p_full[i], 8);
+      sbd::mbar_init(&bars->pv_done[i], 1);
+    }
+    for (int i = 0; i < NSLOT; ++i) {
+      sbd::mbar_init(&bars->full[i], 1);
+      sbd::mbar_init(&bars->empty[i], 1);
+    }
+    sbd::mbar_init(&bars->q_full[0], 1);
+    sbd::mbar_init(&bars->dirty, 1);
+    sbd::mbar_init(&bars->clean, 4);
+    sbd::mbar_init(&bars->drain, 1);
+    bars->abort = 0;
+    sbd::fence_mbar_init();
+    sbd::fence_proxy_async_smem();
+    sbd::prefetch_tmap(&tmQ);
+    sbd::prefetch_tmap(&tmK);
+    sbd::prefetch_tmap(&tmV);
+  }
+  if (warp == 1) {
+    sbd::tmem_alloc_pair(&bars->tmem_slot, C::TM_COLS);
+    sbd::tmem_relinquish_pair();
+  }
+  sbd::griddep_wait();
+  const Tile tl = p.tiles[(blockIdx.x >> 1) / p.nkv];
+  sbd::tc_fence_before();
+  sbd::cluster_sync_all();  // both CTAs' barriers exist
+  sbd::tc_fence_after();
+  const uint32_t tmem = bars->tmem_slot;
+  const int k_len = min(tl.k_len, p.t_k);
+  int nbs[2], j0;
+  block_range(p, tl, k_len, &j0, nbs);
+  const int nb = max(nbs[0], nbs[1]);  // the pair walks its blocks together
+  // the block that holds the sequence's end inside it, if the pair reads it
+  const int j_end = k_len % KB ? k_len / KB : -1;
+  const bool cleans = j_end >= j0 && j_end < j0 + nb;
+
+  // at head_dim 128 two CTAs share an SM: 128 registers a thread at launch, then 56 and 200 in the two warpgroups
+  if (warp < 4) {
+    if constexpr (HD == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer
+      if (lane == 0 && nb > 0) {
+        const int q_bytes = p.tpt * p.group * HD * 2;  // a box of tpt tokens x group heads; tokens past the tensor read as zero
+        if (lead) sbd::mbar_arrive_expect_tx(&bars->q_full[0], 2 * q_bytes);
+        const uint32_t q_bar = sbd::mapa_shared(sbd::smem_u32(&bars->q_full[0]), 0);
+        for (int b = 0; b < HD / 64; ++b)
+          tma_load_3d_pair(&tmQ, q_bar, smem + b * (QR * 128), 64 * b, kv * p.group, tl.q0 + rank * p.tpt);
+        int it = 0;
+        bool ok = true;
+        auto load = [&](bool is_v, int j) {  // this CTA's half of block j of K or V into the next slot
+          const int st = it % NSLOT;
+          ok = ok && sbd::mbar_wait_cluster(&bars->empty[st], ((it / NSLOT) & 1) ^ 1, abort, p.err);
+          if (!ok) return;
+          uint8_t* dst = smem + C::Q_BYTES + st * C::SLOT;
+          if (lead) sbd::mbar_arrive_expect_tx(&bars->full[st], 2 * C::SLOT);
+          const uint32_t bar = sbd::mapa_shared(sbd::smem_u32(&bars->full[st]), 0);
+          if (is_v) {  // 128 keys, dims rank * HD / 2 ...
+            for (int b = 0; b < HD / 128; ++b)
+              tma_load_3d_pair(&tmV, bar, dst + b * (KB * 128), rank * (HD / 2) + 64 * b, kv, tl.k0 + j * KB);
+          } else {  // keys rank * 64 ..., all dims
+            for (int b = 0; b < HD / 64; ++b)
+              tma_load_3d_pair(&tmK, bar, dst + b * (KB / 2 * 128), 64 * b, kv, tl.k0 + j * KB + rank * (KB / 2));
+          }
+          ++it;
+        };
+        for (int j = 0; j <= nb && ok; ++j) {
+          if (j < nb) load(false, j0 + j);
+          const int vj = j - (SB - 1);  // two score buffers: the next block's scores come before this block's P V
+          if (vj >= 0 && vj < nb) load(true, j0 + vj);
+        }
+        if (*abort && lead) {  // copies in flight land before shared memory is released (the even CTA counts both CTAs')
+          drain_wait(&bars->q_full[0], 0);
+          for (int i = max(0, it - NSLOT); i < it; ++i) drain_wait(&bars->full[i % NSLOT], (i / NSLOT) & 1);
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer (even CTA)
+      if (lane == 0 && lead && nb > 0) {
+        constexpr uint32_t idesc_s = idesc<T>(2 * QR, KB, 0), idesc_o = idesc<T>(2 * QR, HD, 1);
+        const uint64_t qd = sbd::umma_desc(sbd::smem_u32(smem), 16, 1024, sbd::kLayoutSwizzle128B);
+        const uint64_t kd = sbd::umma_desc(sbd::smem_u32(smem + C::Q_BYTES), 16, 1024, sbd::kLayoutSwizzle128B);
+        const uint64_t vd = sbd::umma_desc(sbd::smem_u32(smem + C::Q_BYTES), KB * 128, 1024, sbd::kLayoutSwizzle128B);
+        int it = 0;
+        bool ok = true;
+        auto slot_wait = [&](int i) { ok = ok && sbd::mbar_wait_cluster(&bars->full[i % NSLOT], (i / NSLOT) & 1, abort, p.err); };
+        auto scores = [&](int j) {  // S(j) = Q K_j^T
+          slot_wait(it);
+          if (!ok) return;
+          sbd::tc_fence_after();
+          const uint32_t d = tmem + C::TM_S + (SB == 2 ? j & 1 : 0) * KB;
+          const uint64_t k = kd + static_cast<uint64_t>((it % NSLOT) * (C::SLOT >> 4));
+  #pragma unroll
+          for (int s = 0; s < HD / 16; ++s)
+            umma_f16_ss_pair(d, qd + (s >> 2) * (QR * 128 >> 4) + (s & 3) * 2, k + (s >> 2) * (KB / 2 * 128 >> 4) + (s & 3) * 2,
+                             idesc_s, s > 0 ? 1u : 0u);
+          sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
+          sbd::umma_commit_pair(&bars->s_full[SB == 2 ? j & 1 : 0], kBoth);
+          ++it;
+        };
+        ok = sbd::mbar_wait_cluster(&bars->q_full[0], 0, abort, p.err);
+        if (ok) scores(0);
+        for (int j = 0; j < nb && ok; ++j) {
+          if (SB == 2 && j + 1 < nb) scores(j + 1);
+          if (ok) slot_wait(it);
+          if (ok && cleans && j0 + j == j_end) {
+            sbd::mbar_arrive(&bars->dirty);
+            sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->dirty), 1));
+            ok = sbd::mbar_wait_cluster(&bars->clean, 0, abort, p.err);
+          }
+          const int buf = SB == 2 ? j & 1 : 0;
+          ok = ok && sbd::mbar_wait_cluster(&bars->p_full[buf], (SB == 2 ? j >> 1 : j) & 1, abort, p.err);
+          if (!ok) break;
+          sbd::tc_fence_after();
+          // O += P V_j
+          const uint64_t v = vd + static_cast<uint64_t>((it % NSLOT) * (C::SLOT >> 4));
+  #pragma unroll
+          for (int s = 0; s < KB / 16; ++s)
+            sbd::umma_f16_ts_pair(tmem, tmem + C::TM_S + buf * KB + s * 8, v + s * (2048 >> 4), idesc_o, j > 0 || s > 0 ? 1u : 0u);
+          sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
+          sbd::umma_commit_pair(&bars->pv_done[buf], kBoth);
+          ++it;
+          if (SB == 1 && j + 1 < nb) scores(j + 1);
+        }
+        // every MMA issued has finished before tensor and shared memory are released
+        sbd::umma_commit_pair(&bars->drain, kBoth);
+        drain_wait(&bars->drain, 0);
+      }
+    } else {
+      // ------------------------------------------------------------ V rows past the sequence's end
+      if (cleans) {
+        const int j = j_end - j0, item = SB == 2 ? min(j + 2, nb) + j : 2 * j + 1;  // in the producer's order
+        if (__all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->dirty, 0, abort, p.err))) {
+          zero_rows(smem + C::Q_BYTES + item % NSLOT * C::SLOT, HD / 128, k_len % KB, threadIdx.x - 64);
+          if (lane == 0) {
+            if (lead) sbd::mbar_arrive(&bars->clean);
+            else sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->clean), 0));
+          }
+        }
+      }
+    }
+  } else {
+    if constexpr (HD == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ------------------------------------------------------------ softmax and output
+    // P V of block j completes in the phases of a barrier per score buffer: with two buffers the scores of
+    // block j + 1 do not wait for P V of block j, and one barrier's phases could be mistaken two blocks apart.  A
+    // buffer's scores are issued after the P V that read it, so its barrier is never more than a phase behind.
+    const int quad = warp & 3;
+    const Row r = row_of(p, tl, rank, quad * 32 + lane, k_len);
+    const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t p_lead = sbd::mapa_shared(sbd::smem_u32(&bars->p_full[0]), 0);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nb && ok; ++j) {
+      const int buf = SB == 2 ? j & 1 : 0, kb = (j0 + j) * KB;
+      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->s_full[buf], (SB == 2 ? j >> 1 : j) & 1, abort, p.err));
+      if (!ok) break;
+      sbd::tc_fence_after();
+      ok = softmax_block<T, HD>(tm + C::TM_S + buf * KB, tm, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m,
+                                l, &bars->pv_done[SB == 2 ? (j - 1) & 1 : 0], (SB == 2 ? (j - 1) >> 1 : j - 1) & 1, abort, p.err);
+      __syncwarp();
+      if (lane == 0 && ok) {
+        if (lead) sbd::mbar_arrive(&bars->p_full[buf]);
+        else sbd::mbar_arrive_remote_cta(p_lead + buf * sizeof(uint64_t));
+      }
+    }
+    if (ok && nb > 0) {
+      const int e = nb - 1;
+      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->pv_done[SB == 2 ? e & 1 : 0], (SB == 2 ? e >> 1 : e) & 1, abort, p.err));
+    }
+    if (ok) {
+      sbd::tc_fence_after();
+      const int64_t token = static_cast<int64_t>(tl.q0) + rank * p.tpt + r.tok;
+      T* dst = static_cast<T*>(p.out) + token * p.out_token + static_cast<int64_t>(kv * p.group + r.head) * p.out_head;
+      store_row<T, HD>(tm, l, dst, r.ok && token >= 0 && token < p.t_q);
+    }
+  }
+
+  // both CTAs are done with each other's barriers and with tensor memory (the MMAs have completed)
+  sbd::tc_fence_before();
+  sbd::cluster_sync_all();
+  if (warp == 1) {
+    sbd::tc_fence_after();
+    sbd::tmem_dealloc_pair(tmem, C::TM_COLS);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(Cfg64::THREADS, 1)
+    attn_packed_64_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                          const __grid_constant__ CUtensorMap tmV, const PackedParams p) {
+  using C = Cfg64;
+  constexpr int NQ = C::NQ, NSLOT = C::NSLOT, HD = C::HD;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars* bars = reinterpret_cast<Bars*>(smem + C::OFF_BAR);
@@ -154,302 +541,123 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
   __syncthreads();
   sbd::tc_fence_after();
   const uint32_t tmem = bars->tmem_slot;
-
-  // key blocks [j0, j0 + nb[i]) of tile i; rows see keys (pos - window, pos] of [0, k_len)
   const int k_len = min(tl.k_len, p.t_k);
-  int nb[2] = {0, 0}, j0 = 0, nb_all = 0;
-  {
-    const int first = tl.pos0;
-    j0 = p.window > 0 ? max(0, first + 1 - p.window) / KB : 0;
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int n = min(p.tpt, tl.n_tok - i * p.tpt);
-      const int last = min(first + i * p.tpt + n - 1, k_len - 1);  // the tile's furthest key
-      nb[i] = n > 0 ? max(0, (last >= 0 ? last / KB + 1 : 0) - j0) : 0;
-      nb_all = max(nb_all, nb[i]);
-    }
-  }
-  // the block that holds the sequence's end inside it, if this CTA reads it
+  int nb[2], j0;
+  block_range(p, tl, k_len, &j0, nb);
+  const int nb_all = max(nb[0], nb[1]);
   const int j_end = k_len % KB ? k_len / KB : -1;
   const bool cleans = j_end >= j0 && j_end < j0 + nb_all;
+  // items in the ring: K_0, V_0, K_1, V_1, ... (one slot each)
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && nb_all > 0) {
-      for (int i = 0; i < NQ; ++i) {
-        if (nb[i] == 0) continue;
-        // a box of tpt tokens x group heads; tokens past the tensor read as zero
-        sbd::mbar_arrive_expect_tx(&bars->q_full[i], p.tpt * p.group * HD * 2);
-        for (int b = 0; b < HD / 64; ++b)
-          tma_load_3d(&tmQ, &bars->q_full[i], smem + i * C::Q_BYTES + b * (QR * 128), 64 * b, kv * p.group,
-                      tl.q0 + i * p.tpt);
-      }
-      int it = 0;
-      bool ok = true;
-      auto load = [&](bool is_v, int j, int c) {  // part c of block j of K or V into the next slot
-        const int st = it % NSLOT;
-        ok = ok && sbd::mbar_wait(&bars->empty[st], ((it / NSLOT) & 1) ^ 1, abort, p.err);
-        if (!ok) return;
-        uint8_t* dst = smem + C::OFF_SLOT + st * C::SLOT;
-        sbd::mbar_arrive_expect_tx(&bars->full[st], C::SLOT);
-        if (is_v) {
-          for (int b = 0; b < HD / 64; ++b)
-            tma_load_3d(&tmV, &bars->full[st], dst + b * (C::VK * 128), 64 * b, kv, tl.k0 + j * KB + c * C::VK);
-        } else {
-          for (int b = 0; b < HD / 64 / PER; ++b)
-            tma_load_3d(&tmK, &bars->full[st], dst + b * (KB * 128), 64 * (c * (HD / 64 / PER) + b), kv, tl.k0 + j * KB);
+  // 168 registers a thread at launch, then 72 in the first warpgroup and 216 in the softmax's two
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer
+      if (lane == 0 && nb_all > 0) {
+        for (int i = 0; i < NQ; ++i) {
+          if (nb[i] == 0) continue;
+          sbd::mbar_arrive_expect_tx(&bars->q_full[i], p.tpt * p.group * HD * 2);
+          tma_load_3d(&tmQ, &bars->q_full[i], smem + i * C::Q_BYTES, 0, kv * p.group, tl.q0 + i * p.tpt);
         }
-        ++it;
-      };
-      for (int j = 0; j <= nb_all && ok; ++j) {
-        if (j < nb_all)
-          for (int c = 0; c < PER; ++c) load(false, j0 + j, c);
-        const int vj = NQ == 1 ? j - 1 : j;  // one tile: the next block's scores come before this block's P V
-        if (vj >= 0 && vj < nb_all)
-          for (int c = 0; c < PER; ++c) load(true, j0 + vj, c);
-      }
-      if (*abort) {  // copies in flight land before this CTA's shared memory is released
-        for (int i = 0; i < NQ; ++i)
-          if (nb[i] > 0) drain_wait(&bars->q_full[i], 0);
-        for (int i = max(0, it - NSLOT); i < it; ++i) drain_wait(&bars->full[i % NSLOT], (i / NSLOT) & 1);
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && nb_all > 0) {
-      constexpr uint32_t idesc_s = idesc<T>(KB, 0), idesc_o = idesc<T>(HD, 1);
-      int it = 0;
-      bool ok = true;
-      auto slot_wait = [&](int i) {
-        ok = ok && sbd::mbar_wait(&bars->full[i % NSLOT], (i / NSLOT) & 1, abort, p.err);
-        return smem + C::OFF_SLOT + (i % NSLOT) * C::SLOT;
-      };
-      // block j's V has landed (its items start at `at`); if it holds the sequence's end, also cleaned
-      auto v_ready = [&](int j, int at) {
-        if (!cleans || j0 + j != j_end) return;
-        for (int c = 0; c < PER && ok; ++c) slot_wait(at + c);
-        if (!ok) return;
-        sbd::mbar_arrive(&bars->dirty);
-        ok = sbd::mbar_wait(&bars->clean, 0, abort, p.err);
-      };
-      // part c of S_i(buf) = Q_i K^T from slot `ks`
-      auto issue_s = [&](int i, int buf, int c, const uint8_t* ks) {
-        const uint32_t qb = sbd::smem_u32(smem + i * C::Q_BYTES), kb = sbd::smem_u32(ks);
-        constexpr int STEPS = HD / 16 / PER;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          const int gs = c * STEPS + s;  // k-step of 16 dims
-          const uint64_t ad = sbd::umma_desc(qb + (gs >> 2) * (QR * 128) + (gs & 3) * 32, 16, 1024, sbd::kLayoutSwizzle128B);
-          const uint64_t bd = sbd::umma_desc(kb + (s >> 2) * (KB * 128) + (s & 3) * 32, 16, 1024, sbd::kLayoutSwizzle128B);
-          sbd::umma_f16(tmem + C::TM_S + buf * KB, ad, bd, idesc_s, gs > 0 ? 1u : 0u);
+        int it = 0;
+        for (; it < 2 * nb_all; ++it) {
+          const int st = it % NSLOT;
+          if (!sbd::mbar_wait(&bars->empty[st], ((it / NSLOT) & 1) ^ 1, abort, p.err)) break;
+          sbd::mbar_arrive_expect_tx(&bars->full[st], C::SLOT);
+          tma_load_3d(it & 1 ? &tmV : &tmK, &bars->full[st], smem + C::OFF_SLOT + st * C::SLOT, 0, kv, tl.k0 + (j0 + it / 2) * KB);
         }
-      };
-      // O_i += P(buf) V for part c of the block, from slot `vs`
-      auto issue_pv = [&](int i, int buf, int c, const uint8_t* vs, bool first) {
-        const uint32_t vb = sbd::smem_u32(vs);
-#pragma unroll
-        for (int s = 0; s < C::VK / 16; ++s) {
-          const uint64_t bd = sbd::umma_desc(vb + s * 2048, C::VK * 128, 1024, sbd::kLayoutSwizzle128B);
-          sbd::umma_f16_ts(tmem + i * HD, tmem + C::TM_S + buf * KB + c * (C::VK / 2) + s * 8, bd, idesc_o,
-                           first && c == 0 && s == 0 ? 0u : 1u);
+        if (*abort) {  // copies in flight land before this CTA's shared memory is released
+          for (int i = 0; i < NQ; ++i)
+            if (nb[i] > 0) drain_wait(&bars->q_full[i], 0);
+          for (int i = max(0, it - NSLOT); i < it; ++i) drain_wait(&bars->full[i % NSLOT], (i / NSLOT) & 1);
         }
-      };
-      for (int i = 0; i < NQ && ok; ++i)
-        if (nb[i] > 0) ok = sbd::mbar_wait(&bars->q_full[i], 0, abort, p.err);
-      if constexpr (NQ == 1) {
-        auto scores = [&](int j) {
-          for (int c = 0; c < PER && ok; ++c) {
-            const uint8_t* ks = slot_wait(it);
-            if (!ok) return;
-            sbd::tc_fence_after();
-            issue_s(0, j & 1, c, ks);
-            sbd::umma_commit(&bars->empty[it % NSLOT]);
-            ++it;
-          }
-          if (ok) sbd::umma_commit(&bars->s_full[j & 1]);
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      if (lane == 0 && nb_all > 0) {
+        constexpr uint32_t idesc_s = idesc<T>(QR, KB, 0), idesc_o = idesc<T>(QR, HD, 1);
+        bool ok = true;
+        auto slot_wait = [&](int i) {
+          ok = ok && sbd::mbar_wait(&bars->full[i % NSLOT], (i / NSLOT) & 1, abort, p.err);
+          return sbd::smem_u32(smem + C::OFF_SLOT + (i % NSLOT) * C::SLOT);
         };
-        if (ok) scores(0);
-        for (int j = 0; j < nb_all && ok; ++j) {
-          if (j + 1 < nb_all) scores(j + 1);
-          if (ok) v_ready(j, it);
-          ok = ok && sbd::mbar_wait(&bars->p_full[j & 1], (j >> 1) & 1, abort, p.err);
-          for (int c = 0; c < PER && ok; ++c) {
-            const uint8_t* vs = slot_wait(it);
-            if (!ok) break;
-            sbd::tc_fence_after();
-            issue_pv(0, j & 1, c, vs, j == 0);
-            sbd::umma_commit(&bars->empty[it % NSLOT]);
-            ++it;
-          }
-          if (ok) sbd::umma_commit(&bars->pv_done[0]);
-        }
-      } else {
-        // items: K_0, V_0, K_1, V_1, ... (one slot each)
-        const uint8_t* ks = slot_wait(0);
+        auto issue_s = [&](int i, uint32_t ks) {  // S_i = Q_i K^T
+          const uint32_t qb = sbd::smem_u32(smem + i * C::Q_BYTES);
+  #pragma unroll
+          for (int s = 0; s < HD / 16; ++s)
+            sbd::umma_f16(tmem + C::TM_S + i * KB, sbd::umma_desc(qb + s * 32, 16, 1024, sbd::kLayoutSwizzle128B),
+                          sbd::umma_desc(ks + s * 32, 16, 1024, sbd::kLayoutSwizzle128B), idesc_s, s > 0 ? 1u : 0u);
+          sbd::umma_commit(&bars->s_full[i]);
+        };
+        for (int i = 0; i < NQ && ok; ++i)
+          if (nb[i] > 0) ok = sbd::mbar_wait(&bars->q_full[i], 0, abort, p.err);
+        const uint32_t ks = slot_wait(0);
         if (ok) {
           sbd::tc_fence_after();
           for (int i = 0; i < NQ; ++i)
-            if (nb[i] > 0) {
-              issue_s(i, i, 0, ks);
-              sbd::umma_commit(&bars->s_full[i]);
-            }
+            if (nb[i] > 0) issue_s(i, ks);
           sbd::umma_commit(&bars->empty[0]);
         }
         for (int j = 0; j < nb_all && ok; ++j) {
-          const uint8_t* vs = slot_wait(2 * j + 1);
-          if (ok) v_ready(j, 2 * j + 1);
-          const uint8_t* kn = j + 1 < nb_all ? slot_wait(2 * j + 2) : nullptr;
+          const uint32_t vs = slot_wait(2 * j + 1);
+          if (ok && cleans && j0 + j == j_end) {
+            sbd::mbar_arrive(&bars->dirty);
+            ok = sbd::mbar_wait(&bars->clean, 0, abort, p.err);
+          }
+          const uint32_t kn = j + 1 < nb_all ? slot_wait(2 * j + 2) : 0;
           for (int i = 0; i < NQ && ok; ++i) {
             if (j >= nb[i]) continue;
             ok = sbd::mbar_wait(&bars->p_full[i], j & 1, abort, p.err);
             if (!ok) break;
             sbd::tc_fence_after();
-            issue_pv(i, i, 0, vs, j == 0);
+  #pragma unroll
+            for (int s = 0; s < KB / 16; ++s)  // O_i += P_i V
+              sbd::umma_f16_ts(tmem + i * HD, tmem + C::TM_S + i * KB + s * 8,
+                               sbd::umma_desc(vs + s * 2048, KB * 128, 1024, sbd::kLayoutSwizzle128B), idesc_o, j > 0 || s > 0 ? 1u : 0u);
             sbd::umma_commit(&bars->pv_done[i]);
-            if (j + 1 < nb[i]) {
-              issue_s(i, i, 0, kn);
-              sbd::umma_commit(&bars->s_full[i]);
-            }
+            if (j + 1 < nb[i]) issue_s(i, kn);
           }
           if (!ok) break;
           sbd::umma_commit(&bars->empty[(2 * j + 1) % NSLOT]);
           if (j + 1 < nb_all) sbd::umma_commit(&bars->empty[(2 * j + 2) % NSLOT]);
         }
+        // every MMA issued has finished before tensor and shared memory are released
+        sbd::umma_commit(&bars->drain);
+        drain_wait(&bars->drain, 0);
       }
-      // every MMA issued has finished before tensor and shared memory are released
-      sbd::umma_commit(&bars->drain);
-      drain_wait(&bars->drain, 0);
-    }
-  } else if (warp < 4) {
-    // ------------------------------------------------------------ V rows past the sequence's end
-    if (cleans) {
-      const int j = j_end - j0, from = k_len % KB;
-      // V_j's first item in the producer's order
-      const int item = NQ == 1 ? PER * (min(j + 2, nb_all) + j) : 2 * j + 1;
-      // the issuer, which follows the slots' phases, says when they have landed
-      const bool ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->dirty, 0, abort, p.err));
-      for (int c = 0; c < PER && ok; ++c) {
-        uint8_t* vs = smem + C::OFF_SLOT + (item + c) % NSLOT * C::SLOT;
-        // whole rows of 128 bytes per box: the swizzle only permutes inside them
-        const int lo = max(0, from - c * C::VK);
-        for (int b = 0; b < HD / 64; ++b)
-          for (int x = lo * 8 + (threadIdx.x - 64); x < C::VK * 8; x += 64)
-            *reinterpret_cast<uint4*>(vs + b * (C::VK * 128) + x * 16) = make_uint4(0, 0, 0, 0);
+    } else {
+      // ------------------------------------------------------------ V rows past the sequence's end
+      // (the issuer, which follows the slots' phases, says when they have landed)
+      if (cleans && __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->dirty, 0, abort, p.err))) {
+        zero_rows(smem + C::OFF_SLOT + (2 * (j_end - j0) + 1) % NSLOT * C::SLOT, 1, k_len % KB, threadIdx.x - 64);
+        if (lane == 0) sbd::mbar_arrive(&bars->clean);
       }
-      sbd::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0 && ok) sbd::mbar_arrive(&bars->clean);
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------------------ softmax and output
-    const int i = (warp - 4) >> 2;  // tile
-    const int quad = warp & 3, row = quad * 32 + lane;
-    const int tok = row / p.group, head = row - tok * p.group;
-    const int n_tok = min(p.tpt, tl.n_tok - i * p.tpt);
-    const bool row_ok = tok < n_tok;
-    const int pos = tl.pos0 + i * p.tpt + tok;
-    // keys [lo, hi) of the sequence
-    const int hi = row_ok ? min(pos + 1, k_len) : 0;
-    const int lo = p.window > 0 ? pos + 1 - p.window : 0;
-    // blocks that every row of the tile sees whole need no mask
-    const int all_hi = min(tl.pos0 + i * p.tpt + 1, k_len);
-    const int all_lo = p.window > 0 ? tl.pos0 + i * p.tpt + n_tok - p.window : 0;
+    const int i = (warp - 4) >> 2, quad = warp & 3;  // tile, lane quadrant
+    const Row r = row_of(p, tl, i, quad * 32 + lane, k_len);
     const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nb[i] && ok; ++j) {
-      const int buf = NQ == 1 ? j & 1 : i;
-      const uint32_t ph = NQ == 1 ? (j >> 1) & 1 : j & 1;
-      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->s_full[buf], ph, abort, p.err));
+      const int kb = (j0 + j) * KB;
+      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->s_full[i], j & 1, abort, p.err));
       if (!ok) break;
       sbd::tc_fence_after();
-      const uint32_t ts = tm + C::TM_S + buf * KB;
-      uint32_t sv[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) sbd::tmem_ld_32x32b_x32(ts + 32 * c, sv[c]);
-      sbd::tmem_wait_ld();
-      const int kb = (j0 + j) * KB;
-      if (kb + KB > all_hi || kb < all_lo) {
-        const int v0 = lo - kb, v1 = hi - kb;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            sv[c][e] = 32 * c + e >= v0 && 32 * c + e < v1 ? sv[c][e] : 0xFF800000u;  // -inf
-      }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(sv[c][0]);
-#pragma unroll
-        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(sv[c][e]));
-      }
-      const float mx2 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
-      const bool start = m == -INFINITY;  // O is still zero in this row
-      const bool rise = !start && mx2 > m + kRise;
-      if (__any_sync(0xFFFFFFFFu, rise)) {
-        // O += P_{j-1} V_{j-1} has to be complete before it is scaled
-        ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->pv_done[i], (j - 1) & 1, abort, p.err));
-        if (!ok) break;
-        sbd::tc_fence_after();
-        const float alpha = rise ? ex2(m - mx2) : 1.f;
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t ov[32];
-          sbd::tmem_ld_32x32b_x32(tm + i * HD + 32 * c, ov);
-          sbd::tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-          sbd::tmem_st_32x32b_x16(tm + i * HD + 32 * c, *reinterpret_cast<const uint32_t(*)[16]>(&ov[0]));
-          sbd::tmem_st_32x32b_x16(tm + i * HD + 32 * c + 16, *reinterpret_cast<const uint32_t(*)[16]>(&ov[16]));
-        }
-        sbd::tmem_wait_st();
-        l *= alpha;
-      }
-      if (start || rise) m = mx2;
-      const float mu = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
-        float ls[2] = {0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = ex2(fmaf(__uint_as_float(sv[c][2 * e]), p.scale2, -mu));
-          const float p1 = ex2(fmaf(__uint_as_float(sv[c][2 * e + 1]), p.scale2, -mu));
-          ls[0] += p0;
-          ls[1] += p1;
-          pk[e] = sbp::pack2<T>(p0, p1);
-        }
-        l += ls[0] + ls[1];
-        sbd::tmem_st_32x32b_x16(ts + 16 * c, pk);
-      }
-      sbd::tmem_wait_st();
-      sbd::tc_fence_before();
+      ok = softmax_block<T, HD>(tm + C::TM_S + i * KB, tm + i * HD, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo,
+                                p.scale2, m, l, &bars->pv_done[i], (j - 1) & 1, abort, p.err);
       __syncwarp();
-      if (lane == 0) sbd::mbar_arrive(&bars->p_full[buf]);
+      if (lane == 0 && ok) sbd::mbar_arrive(&bars->p_full[i]);
     }
-    // ------------------------------------------------------------ O / l
     if (ok && nb[i] > 0) ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->pv_done[i], (nb[i] - 1) & 1, abort, p.err));
     if (ok) {
       sbd::tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-      const int64_t token = static_cast<int64_t>(tl.q0) + i * p.tpt + tok;
-      T* dst = static_cast<T*>(p.out) + token * p.out_token + static_cast<int64_t>(kv * p.group + head) * p.out_head;
-      const bool store = row_ok && token >= 0 && token < p.t_q;
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t ov[32];
-        if (nb[i] > 0) {
-          sbd::tmem_ld_32x32b_x32(tm + i * HD + 32 * c, ov);
-          sbd::tmem_wait_ld();
-        }
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          uint32_t w[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            w[q] = l == 0.f ? 0u : sbp::pack2<T>(__uint_as_float(ov[e + 2 * q]) * inv, __uint_as_float(ov[e + 2 * q + 1]) * inv);
-          if (store) *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+      const int64_t token = static_cast<int64_t>(tl.q0) + i * p.tpt + r.tok;
+      T* dst = static_cast<T*>(p.out) + token * p.out_token + static_cast<int64_t>(kv * p.group + r.head) * p.out_head;
+      store_row<T, HD>(tm + i * HD, l, dst, r.ok && token >= 0 && token < p.t_q);
     }
   }
 
@@ -481,40 +689,78 @@ struct Strides {
   int64_t q_token, q_head, k_token, k_head;
 };
 
-template <typename T, int HD>
-int launch_packed(const void* q, const void* k, const void* v, const Strides& st, const PackedParams& p, int n_tiles,
-                  cudaStream_t stream) {
-  using C = Cfg<HD>;
-  constexpr bool bf = !std::is_same<T, __half>::value;
-  CUtensorMap tq, tk, tv;
-  int rc = make_map3(&tq, bf, q, HD, p.group * p.nkv, p.t_q, st.q_head, st.q_token, p.group, p.tpt);
-  const int t_k = std::max(p.t_k, 1);
-  if (!rc) rc = make_map3(&tk, bf, k, HD, p.nkv, t_k, st.k_head, st.k_token, 1, KB);
-  if (!rc) rc = make_map3(&tv, bf, v, HD, p.nkv, t_k, st.k_head, st.k_token, 1, C::VK);
-  if (rc) return rc;
-  static bool set[64] = {};
+template <typename K>
+int raise_smem(K kernel, int bytes, bool (&set)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(attn_packed_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return sb::cuda_fail(e, "attn_packed_kernel smem attribute");
-    if (dev >= 0 && dev < 64) set[dev] = true;
-  }
-  cudaError_t e = sb::launch_pdl(attn_packed_kernel<T, HD>, dim3(n_tiles * p.nkv), dim3(C::THREADS), C::SMEM, stream, tq, tk, tv, p);
-  if (e != cudaSuccess) return sb::cuda_fail(e, "attn_packed_kernel");
-  return sb::launch_status("attn_packed_kernel");
+  if (dev >= 0 && dev < 64 && set[dev]) return SB_OK;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return sb::cuda_fail(e, "attn_packed smem attribute");
+  if (dev >= 0 && dev < 64) set[dev] = true;
+  return SB_OK;
+}
+
+// K in boxes of k_rows keys, V of KB.
+template <typename T>
+int make_maps(const void* q, const void* k, const void* v, const Strides& st, const PackedParams& p, int hd, int k_rows,
+              CUtensorMap (&m)[3]) {
+  constexpr bool bf = !std::is_same<T, __half>::value;
+  const int t_k = std::max(p.t_k, 1);
+  int rc = make_map3(&m[0], bf, q, hd, p.group * p.nkv, p.t_q, st.q_head, st.q_token, p.group, p.tpt);
+  if (!rc) rc = make_map3(&m[1], bf, k, hd, p.nkv, t_k, st.k_head, st.k_token, 1, k_rows);
+  if (!rc) rc = make_map3(&m[2], bf, v, hd, p.nkv, t_k, st.k_head, st.k_token, 1, KB);
+  return rc;
+}
+
+template <typename T>
+int launch_64(const void* q, const void* k, const void* v, const Strides& st, const PackedParams& p, int n_tiles, cudaStream_t stream) {
+  static bool set[64] = {};
+  CUtensorMap m[3];
+  int rc = make_maps<T>(q, k, v, st, p, 64, KB, m);
+  if (!rc) rc = raise_smem(attn_packed_64_kernel<T>, Cfg64::SMEM, set);
+  if (rc) return rc;
+  cudaError_t e = sb::launch_pdl(attn_packed_64_kernel<T>, dim3(n_tiles * p.nkv), dim3(Cfg64::THREADS), Cfg64::SMEM, stream, m[0], m[1], m[2], p);
+  if (e != cudaSuccess) return sb::cuda_fail(e, "attn_packed_64_kernel");
+  return sb::launch_status("attn_packed_64_kernel");
+}
+
+template <typename T, int HD>
+int launch_pair(const void* q, const void* k, const void* v, const Strides& st, const PackedParams& p, int n_tiles, cudaStream_t stream) {
+  using C = PairCfg<HD>;
+  static bool set[64] = {};
+  CUtensorMap m[3];
+  int rc = make_maps<T>(q, k, v, st, p, HD, KB / 2, m);
+  if (!rc) rc = raise_smem(attn_packed_pair_kernel<T, HD>, C::SMEM, set);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * n_tiles * p.nkv);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_packed_pair_kernel<T, HD>, m[0], m[1], m[2], p);
+  if (e != cudaSuccess) return sb::cuda_fail(e, "attn_packed_pair_kernel");
+  return sb::launch_status("attn_packed_pair_kernel");
 }
 
 template <typename T>
 int launch_packed_hd(int hd, const void* q, const void* k, const void* v, const Strides& st, const PackedParams& p,
                      int n_tiles, cudaStream_t s) {
-  if (hd == 64) return launch_packed<T, 64>(q, k, v, st, p, n_tiles, s);
-  if (hd == 128) return launch_packed<T, 128>(q, k, v, st, p, n_tiles, s);
-  return launch_packed<T, 256>(q, k, v, st, p, n_tiles, s);
+  if (hd == 64) return launch_64<T>(q, k, v, st, p, n_tiles, s);
+  if (hd == 128) return launch_pair<T, 128>(q, k, v, st, p, n_tiles, s);
+  return launch_pair<T, 256>(q, k, v, st, p, n_tiles, s);
 }
 
-// Query tokens per CTA.
-int tokens_per_cta(int group, int hd) { return (hd == 256 ? 1 : 2) * (QR / group); }
+// Query tokens per tile of the plan: two query tiles, of one CTA or of a pair.
+int tokens_per_tile(int group) { return 2 * (QR / group); }
 
 int check_heads(const char* who, int n_heads, int n_kv_heads, int hd) {
   SB_CHECK_ARG(hd == 64 || hd == 128 || hd == 256, "%s: head_dim %d not in {64, 128, 256}", who, hd);
@@ -530,7 +776,7 @@ extern "C" int sb_attn_packed_plan(const int32_t* q_lens, const int32_t* kv_lens
   int rc = check_heads("sb_attn_packed_plan", n_heads, n_kv_heads, head_dim);
   if (rc) return rc;
   SB_CHECK_ARG(n >= 0 && window >= 0 && max_tiles >= 0 && n_tiles && (n == 0 || q_lens), "sb_attn_packed_plan: bad arguments");
-  const int per = tokens_per_cta(n_heads / n_kv_heads, head_dim);
+  const int per = tokens_per_tile(n_heads / n_kv_heads);
   int64_t count = 0, tq = 0, tk = 0;
   for (int i = 0; i < n; ++i) {
     const int kl = kv_lens ? kv_lens[i] : q_lens[i];
@@ -539,7 +785,7 @@ extern "C" int sb_attn_packed_plan(const int32_t* q_lens, const int32_t* kv_lens
     tq += q_lens[i];
     tk += kl;
   }
-  SB_CHECK_ARG(tq < (1ll << 31) && tk < (1ll << 31) && count * n_kv_heads < (1ll << 31), "sb_attn_packed_plan: too many tokens");
+  SB_CHECK_ARG(tq < (1ll << 31) && tk < (1ll << 31) && count * n_kv_heads < (1ll << 30), "sb_attn_packed_plan: too many tokens");
   *n_tiles = static_cast<int>(count);
   if (!tiles) return SB_OK;  // the count alone
   SB_CHECK_ARG(count <= max_tiles, "sb_attn_packed_plan: %lld tiles, room for %d", static_cast<long long>(count), max_tiles);
@@ -568,7 +814,7 @@ extern "C" int sb_attn_prefill_packed(const void* q, int64_t q_token, int64_t q_
   if (rc) return rc;
   SB_CHECK_ARG(dtype == SB_F16 || dtype == SB_BF16, "sb_attn_prefill_packed: q, k, v and out are f16 or bf16");
   SB_CHECK_ARG(t_q >= 0 && t_k >= 0 && window >= 0 && n_tiles >= 0 &&
-                   static_cast<int64_t>(n_tiles) * n_kv_heads < (1ll << 31), "sb_attn_prefill_packed: bad sizes");
+                   static_cast<int64_t>(n_tiles) * n_kv_heads < (1ll << 30), "sb_attn_prefill_packed: bad sizes");
   SB_CHECK_ARG(scale > 0.f && scale <= 3.0e38f, "sb_attn_prefill_packed: scale must be positive and finite");
   if (t_q == 0 || n_tiles == 0) return SB_OK;
   SB_CHECK_ARG(q && out && tiles && (t_k == 0 || (k && v)), "sb_attn_prefill_packed: null pointer");

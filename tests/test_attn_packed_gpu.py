@@ -48,7 +48,7 @@ def _inputs(tq, tk, nh, nkv, hd, dtype, seed, dev):
 def test_plan_covers_every_query_once():
     """Each query of each sequence lies in one tile, with its sequence's keys and its own position."""
     lens, kv = [1, 0, 300, 17, 64], [1, 5, 300, 400, 20]
-    for nh, nkv, hd, per in ((8, 1, 256, 16), (6, 2, 128, 84), (5, 1, 64, 50), (12, 1, 256, 10), (128, 1, 64, 2)):
+    for nh, nkv, hd, per in ((8, 1, 256, 32), (6, 2, 128, 84), (5, 1, 64, 50), (12, 1, 256, 20), (128, 1, 64, 2)):
         plan = kern.PackedPlan(lens, nh, nkv, hd, kv_lens=kv, window=9, device="cpu")
         seen = {}
         for q0, n, k0, kl, pos0 in plan.tiles[:, :5].tolist():
@@ -196,3 +196,15 @@ def test_attn_prefill_packed_refusals(cuda):
     assert e.value.code == _lib.SB_ERR_ALIGN
     none = kern.attn_prefill_packed(q[:0], k[:0], v[:0], kern.PackedPlan([0], 4, 2, 64, device=cuda))
     assert none.shape == (0, 4, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nh,nkv,hd,lens", [(8, 1, 256, [500]), (16, 4, 128, [500, 300]), (6, 2, 64, [600, 100])])
+def test_attn_prefill_packed_repeats(cuda, nh, nkv, hd, lens):
+    """200 launches back to back give the same bits, each right: the kernel's roles hand over in order."""
+    q, k, v = _inputs(sum(lens), sum(lens), nh, nkv, hd, torch.float16, 12, cuda)
+    plan = kern.PackedPlan(lens, nh, nkv, hd, device=cuda)
+    want, mass = _reference(q, k, v, lens, lens, 0.2, 0)
+    outs = [kern.attn_prefill_packed(q, k, v, plan, scale=0.2) for _ in range(200)]
+    _check(outs[0], want, mass, torch.float16)
+    assert all(torch.equal(o, outs[0]) for o in outs)
