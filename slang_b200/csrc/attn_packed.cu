@@ -3,12 +3,12 @@
 // sliding window, more keys than queries (a cached prefix).
 //
 // The rows of a query tile are (token, query head of the kv head's group): 128 /
-// group tokens of all heads that share K and V, so each K/V block of 128 keys
-// serves the whole group.  Two kernels:
+// group tokens of all heads that share K and V, so each K/V block serves the
+// whole group.  Two kernels:
 //
 // attn_packed_pair_kernel (head_dim 128 and 256): a CTA pair (cta_group::2) takes
 // two query tiles, one per CTA.  The pair's MMAs run over 256 rows; each CTA holds
-// 64 of a block's keys and half of its values' dims, so a block is loaded and read
+// half of a block's keys and half of its values' dims, so a block is loaded and read
 // from shared memory half as often.  One CTA alone is bound by shared memory,
 // not by its tensor cores: at head_dim 256 a block costs it 128 KB of operand reads for
 // Q K^T, 64 KB for P V and 128 KB of TMA writes, 2560 cycles at 128 bytes per cycle
@@ -24,9 +24,10 @@
 //                 memory, running maximum m (raised, with O rescaled, only when a
 //                 score passes it by 2^8) and sum l, p = 2^(s - m) in the input
 //                 type back into the scores' columns.
-// At 256, tensor memory holds O and two score buffers: the next block's scores are
-// issued before this block's P V.  At 128, two pairs fit an SM pair, and one's
-// MMAs run under the other's softmax, prologue and output.
+// The next block's scores, in a second buffer, are issued before this block's P V.
+// At 256 (blocks of 128 keys) O and the two buffers fill tensor memory; at 128
+// (blocks of 64) two pairs fit an SM pair, and one's MMAs run under the other's
+// softmax, prologue and output.
 //
 // attn_packed_64_kernel (head_dim 64): one CTA takes two query tiles, each with its
 // own softmax warps; while one tile is in its softmax the other's products run.
@@ -52,13 +53,12 @@
 namespace {
 
 constexpr int QR = 128;  // query rows per tile
-constexpr int KB = 128;  // keys per block
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRise = 8.f;  // log2 units: p stays below 2^8
 
 // head_dim 64, one CTA
 struct Cfg64 {
-  static constexpr int HD = 64, NQ = 2;
+  static constexpr int HD = 64, NQ = 2, KB = 128;  // KB: keys per block
   static constexpr int THREADS = 128 + 128 * NQ;
   static constexpr int Q_BYTES = QR * HD * 2;
   static constexpr int SLOT = KB * HD * 2;  // a block of K or of V
@@ -72,11 +72,11 @@ struct Cfg64 {
 // head_dim 128 and 256, a CTA pair
 template <int HD>
 struct PairCfg {
-  static constexpr int CTAS = HD == 256 ? 1 : 2;  // per SM
-  static constexpr int SB = HD == 256 ? 2 : 1;    // score buffers
+  static constexpr int CTAS = HD == 256 ? 1 : 2;   // per SM
+  static constexpr int KB = HD == 256 ? 128 : 64;  // keys per block
   static constexpr int Q_BYTES = QR * HD * 2;
   static constexpr int SLOT = KB / 2 * HD * 2;    // this CTA's half of a block of K or of V
-  static constexpr int NSLOT = HD == 256 ? 5 : 4;
+  static constexpr int NSLOT = HD == 256 ? 5 : 8;
   static constexpr int OFF_BAR = Q_BYTES + NSLOT * SLOT;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
   static constexpr uint32_t TM_S = HD, TM_COLS = HD == 256 ? 512 : 256;
@@ -167,27 +167,28 @@ __device__ __forceinline__ void umma_f16_ss_pair(uint32_t tmem_d, uint64_t adesc
 // One query row's part in a block: masks the scores (keys [lo, hi) of the sequence; `whole`: all of them), raises
 // the running maximum and rescales O where a score asks for it, writes P over the scores and adds to the sum.
 // Warp-collective; false when a wait failed.
-template <typename T, int HD>
+template <typename T, int HD, int KB>
 __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t to, int kb, int lo, int hi, bool whole, float scale2,
                                               float& m, float& l, uint64_t* pv_done, uint32_t pv_parity,
                                               volatile int* abort, int* err) {
-  uint32_t sv[4][32];
+  constexpr int CH = KB / 32;
+  uint32_t sv[CH][32];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) sbd::tmem_ld_32x32b_x32(ts + 32 * c, sv[c]);
+  for (int c = 0; c < CH; ++c) sbd::tmem_ld_32x32b_x32(ts + 32 * c, sv[c]);
   sbd::tmem_wait_ld();
   if (!whole) {
     const int v0 = lo - kb, v1 = hi - kb;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int e = 0; e < 32; ++e) sv[c][e] = 32 * c + e >= v0 && 32 * c + e < v1 ? sv[c][e] : 0xFF800000u;  // -inf
   }
   float mx[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    mx[c] = __uint_as_float(sv[c][0]);
+    mx[c] = __uint_as_float(sv[0][c]);
 #pragma unroll
-    for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(sv[c][e]));
+    for (int e = 4 + c; e < KB; e += 4) mx[c] = fmaxf(mx[c], __uint_as_float(sv[e >> 5][e & 31]));
   }
   const float mx2 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
   const bool start = m == -INFINITY;  // O is still zero in this row
@@ -212,7 +213,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t to, int kb, 
   if (start || rise) m = mx2;
   const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < CH; ++c) {
     uint32_t pk[16];
     float ls[2] = {0.f, 0.f};
 #pragma unroll
@@ -253,6 +254,7 @@ __device__ __forceinline__ void store_row(uint32_t to, float l, T* dst, bool sto
 
 // Zeroes rows [from, KB) of a V block of `boxes` boxes [KB rows x 128 bytes]: whole rows, the swizzle only permutes
 // inside them.  64 threads.
+template <int KB>
 __device__ __forceinline__ void zero_rows(uint8_t* vs, int boxes, int from, int thread) {
   for (int b = 0; b < boxes; ++b)
     for (int x = from * 8 + thread; x < KB * 8; x += 64) *reinterpret_cast<uint4*>(vs + b * (KB * 128) + x * 16) = make_uint4(0, 0, 0, 0);
@@ -280,6 +282,7 @@ __device__ __forceinline__ Row row_of(const PackedParams& p, const Tile& tl, int
 }
 
 // Key blocks [j0, j0 + nb[i]) of the CTA's or the pair's tiles.
+template <int KB>
 __device__ __forceinline__ void block_range(const PackedParams& p, const Tile& tl, int k_len, int* j0, int (&nb)[2]) {
   *j0 = p.window > 0 ? max(0, tl.pos0 + 1 - p.window) / KB : 0;
 #pragma unroll
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
     attn_packed_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmV, const PackedParams p) {
   using C = PairCfg<HD>;
-  constexpr int SB = C::SB, NSLOT = C::NSLOT;
+  constexpr int KB = C::KB, NSLOT = C::NSLOT;
   constexpr uint16_t kBoth = 3;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -340,15 +343,13 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
   const uint32_t tmem = bars->tmem_slot;
   const int k_len = min(tl.k_len, p.t_k);
   int nbs[2], j0;
-  block_range(p, tl, k_len, &j0, nbs);
+  block_range<KB>(p, tl, k_len, &j0, nbs);
   const int nb = max(nbs[0], nbs[1]);  // the pair walks its blocks together
   // the block that holds the sequence's end inside it, if the pair reads it
   const int j_end = k_len % KB ? k_len / KB : -1;
   const bool cleans = j_end >= j0 && j_end < j0 + nb;
 
-  // at head_dim 128 two CTAs share an SM: 128 registers a thread at launch, then 56 and 200 in the two warpgroups
   if (warp < 4) {
-    if constexpr (HD == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
       // ------------------------------------------------------------ TMA producer
       if (lane == 0 && nb > 0) {
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
         };
         for (int j = 0; j <= nb && ok; ++j) {
           if (j < nb) load(false, j0 + j);
-          const int vj = j - (SB - 1);  // two score buffers: the next block's scores come before this block's P V
+          const int vj = j - 1;  // the next block's scores come before this block's P V
           if (vj >= 0 && vj < nb) load(true, j0 + vj);
         }
         if (*abort && lead) {  // copies in flight land before shared memory is released (the even CTA counts both CTAs')
@@ -399,28 +400,28 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
           slot_wait(it);
           if (!ok) return;
           sbd::tc_fence_after();
-          const uint32_t d = tmem + C::TM_S + (SB == 2 ? j & 1 : 0) * KB;
+          const uint32_t d = tmem + C::TM_S + (j & 1) * KB;
           const uint64_t k = kd + static_cast<uint64_t>((it % NSLOT) * (C::SLOT >> 4));
   #pragma unroll
           for (int s = 0; s < HD / 16; ++s)
             umma_f16_ss_pair(d, qd + (s >> 2) * (QR * 128 >> 4) + (s & 3) * 2, k + (s >> 2) * (KB / 2 * 128 >> 4) + (s & 3) * 2,
                              idesc_s, s > 0 ? 1u : 0u);
           sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
-          sbd::umma_commit_pair(&bars->s_full[SB == 2 ? j & 1 : 0], kBoth);
+          sbd::umma_commit_pair(&bars->s_full[j & 1], kBoth);
           ++it;
         };
         ok = sbd::mbar_wait_cluster(&bars->q_full[0], 0, abort, p.err);
         if (ok) scores(0);
         for (int j = 0; j < nb && ok; ++j) {
-          if (SB == 2 && j + 1 < nb) scores(j + 1);
+          if (j + 1 < nb) scores(j + 1);
           if (ok) slot_wait(it);
           if (ok && cleans && j0 + j == j_end) {
             sbd::mbar_arrive(&bars->dirty);
             sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->dirty), 1));
             ok = sbd::mbar_wait_cluster(&bars->clean, 0, abort, p.err);
           }
-          const int buf = SB == 2 ? j & 1 : 0;
-          ok = ok && sbd::mbar_wait_cluster(&bars->p_full[buf], (SB == 2 ? j >> 1 : j) & 1, abort, p.err);
+          const int buf = j & 1;
+          ok = ok && sbd::mbar_wait_cluster(&bars->p_full[buf], (j >> 1) & 1, abort, p.err);
           if (!ok) break;
           sbd::tc_fence_after();
           // O += P V_j
@@ -431,8 +432,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
           sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
           sbd::umma_commit_pair(&bars->pv_done[buf], kBoth);
           ++it;
-          if (SB == 1 && j + 1 < nb) scores(j + 1);
-        }
+          }
         // every MMA issued has finished before tensor and shared memory are released
         sbd::umma_commit_pair(&bars->drain, kBoth);
         drain_wait(&bars->drain, 0);
@@ -440,9 +440,9 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
     } else {
       // ------------------------------------------------------------ V rows past the sequence's end
       if (cleans) {
-        const int j = j_end - j0, item = SB == 2 ? min(j + 2, nb) + j : 2 * j + 1;  // in the producer's order
+        const int j = j_end - j0, item = min(j + 2, nb) + j;  // in the producer's order
         if (__all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->dirty, 0, abort, p.err))) {
-          zero_rows(smem + C::Q_BYTES + item % NSLOT * C::SLOT, HD / 128, k_len % KB, threadIdx.x - 64);
+          zero_rows<KB>(smem + C::Q_BYTES + item % NSLOT * C::SLOT, HD / 128, k_len % KB, threadIdx.x - 64);
           if (lane == 0) {
             if (lead) sbd::mbar_arrive(&bars->clean);
             else sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->clean), 0));
@@ -451,9 +451,8 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
       }
     }
   } else {
-    if constexpr (HD == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------------------ softmax and output
-    // P V of block j completes in the phases of a barrier per score buffer: with two buffers the scores of
+    // P V of block j completes in the phases of a barrier per score buffer: the scores of
     // block j + 1 do not wait for P V of block j, and one barrier's phases could be mistaken two blocks apart.  A
     // buffer's scores are issued after the P V that read it, so its barrier is never more than a phase behind.
     const int quad = warp & 3;
@@ -463,12 +462,12 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nb && ok; ++j) {
-      const int buf = SB == 2 ? j & 1 : 0, kb = (j0 + j) * KB;
-      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->s_full[buf], (SB == 2 ? j >> 1 : j) & 1, abort, p.err));
+      const int buf = j & 1, kb = (j0 + j) * KB;
+      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->s_full[buf], (j >> 1) & 1, abort, p.err));
       if (!ok) break;
       sbd::tc_fence_after();
-      ok = softmax_block<T, HD>(tm + C::TM_S + buf * KB, tm, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m,
-                                l, &bars->pv_done[SB == 2 ? (j - 1) & 1 : 0], (SB == 2 ? (j - 1) >> 1 : j - 1) & 1, abort, p.err);
+      ok = softmax_block<T, HD, KB>(tm + C::TM_S + buf * KB, tm, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m,
+                                l, &bars->pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort, p.err);
       __syncwarp();
       if (lane == 0 && ok) {
         if (lead) sbd::mbar_arrive(&bars->p_full[buf]);
@@ -477,7 +476,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
     }
     if (ok && nb > 0) {
       const int e = nb - 1;
-      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->pv_done[SB == 2 ? e & 1 : 0], (SB == 2 ? e >> 1 : e) & 1, abort, p.err));
+      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->pv_done[e & 1], (e >> 1) & 1, abort, p.err));
     }
     if (ok) {
       sbd::tc_fence_after();
@@ -501,7 +500,7 @@ __global__ void __launch_bounds__(Cfg64::THREADS, 1)
     attn_packed_64_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                           const __grid_constant__ CUtensorMap tmV, const PackedParams p) {
   using C = Cfg64;
-  constexpr int NQ = C::NQ, NSLOT = C::NSLOT, HD = C::HD;
+  constexpr int NQ = C::NQ, NSLOT = C::NSLOT, HD = C::HD, KB = C::KB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars* bars = reinterpret_cast<Bars*>(smem + C::OFF_BAR);
@@ -543,7 +542,7 @@ __global__ void __launch_bounds__(Cfg64::THREADS, 1)
   const uint32_t tmem = bars->tmem_slot;
   const int k_len = min(tl.k_len, p.t_k);
   int nb[2], j0;
-  block_range(p, tl, k_len, &j0, nb);
+  block_range<KB>(p, tl, k_len, &j0, nb);
   const int nb_all = max(nb[0], nb[1]);
   const int j_end = k_len % KB ? k_len / KB : -1;
   const bool cleans = j_end >= j0 && j_end < j0 + nb_all;
@@ -630,7 +629,7 @@ __global__ void __launch_bounds__(Cfg64::THREADS, 1)
       // ------------------------------------------------------------ V rows past the sequence's end
       // (the issuer, which follows the slots' phases, says when they have landed)
       if (cleans && __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->dirty, 0, abort, p.err))) {
-        zero_rows(smem + C::OFF_SLOT + (2 * (j_end - j0) + 1) % NSLOT * C::SLOT, 1, k_len % KB, threadIdx.x - 64);
+        zero_rows<KB>(smem + C::OFF_SLOT + (2 * (j_end - j0) + 1) % NSLOT * C::SLOT, 1, k_len % KB, threadIdx.x - 64);
         if (lane == 0) sbd::mbar_arrive(&bars->clean);
       }
     }
@@ -647,7 +646,7 @@ __global__ void __launch_bounds__(Cfg64::THREADS, 1)
       ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->s_full[i], j & 1, abort, p.err));
       if (!ok) break;
       sbd::tc_fence_after();
-      ok = softmax_block<T, HD>(tm + C::TM_S + i * KB, tm + i * HD, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo,
+      ok = softmax_block<T, HD, KB>(tm + C::TM_S + i * KB, tm + i * HD, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo,
                                 p.scale2, m, l, &bars->pv_done[i], (j - 1) & 1, abort, p.err);
       __syncwarp();
       if (lane == 0 && ok) sbd::mbar_arrive(&bars->p_full[i]);
@@ -700,15 +699,15 @@ int raise_smem(K kernel, int bytes, bool (&set)[64]) {
   return SB_OK;
 }
 
-// K in boxes of k_rows keys, V of KB.
+// K in boxes of k_rows keys, V of v_rows.
 template <typename T>
 int make_maps(const void* q, const void* k, const void* v, const Strides& st, const PackedParams& p, int hd, int k_rows,
-              CUtensorMap (&m)[3]) {
+              int v_rows, CUtensorMap (&m)[3]) {
   constexpr bool bf = !std::is_same<T, __half>::value;
   const int t_k = std::max(p.t_k, 1);
   int rc = make_map3(&m[0], bf, q, hd, p.group * p.nkv, p.t_q, st.q_head, st.q_token, p.group, p.tpt);
   if (!rc) rc = make_map3(&m[1], bf, k, hd, p.nkv, t_k, st.k_head, st.k_token, 1, k_rows);
-  if (!rc) rc = make_map3(&m[2], bf, v, hd, p.nkv, t_k, st.k_head, st.k_token, 1, KB);
+  if (!rc) rc = make_map3(&m[2], bf, v, hd, p.nkv, t_k, st.k_head, st.k_token, 1, v_rows);
   return rc;
 }
 
@@ -716,7 +715,7 @@ template <typename T>
 int launch_64(const void* q, const void* k, const void* v, const Strides& st, const PackedParams& p, int n_tiles, cudaStream_t stream) {
   static bool set[64] = {};
   CUtensorMap m[3];
-  int rc = make_maps<T>(q, k, v, st, p, 64, KB, m);
+  int rc = make_maps<T>(q, k, v, st, p, 64, Cfg64::KB, Cfg64::KB, m);
   if (!rc) rc = raise_smem(attn_packed_64_kernel<T>, Cfg64::SMEM, set);
   if (rc) return rc;
   cudaError_t e = sb::launch_pdl(attn_packed_64_kernel<T>, dim3(n_tiles * p.nkv), dim3(Cfg64::THREADS), Cfg64::SMEM, stream, m[0], m[1], m[2], p);
@@ -729,7 +728,7 @@ int launch_pair(const void* q, const void* k, const void* v, const Strides& st, 
   using C = PairCfg<HD>;
   static bool set[64] = {};
   CUtensorMap m[3];
-  int rc = make_maps<T>(q, k, v, st, p, HD, KB / 2, m);
+  int rc = make_maps<T>(q, k, v, st, p, HD, C::KB / 2, C::KB, m);
   if (!rc) rc = raise_smem(attn_packed_pair_kernel<T, HD>, C::SMEM, set);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
