@@ -23,17 +23,18 @@
 //   warps 4 .. 7  softmax, a thread per query row: the row's 128 scores from tensor
 //                 memory, running maximum m (raised, with O rescaled, only when a
 //                 score passes it by 2^8) and sum l, p = 2^(s - m) in the input
-//                 type back into the scores' columns.
-// The next block's scores, in a second buffer, are issued before this block's P V.
-// At 256 (blocks of 128 keys) O and the two buffers fill tensor memory; at 128
-// (blocks of 64) two pairs fit an SM pair, and one's MMAs run under the other's
-// softmax, prologue and output.
+//                 type to tensor memory.
+// P has buffers of its own, so the next block's scores are issued as soon as every
+// row has read this block's, and run under its softmax; P V follows when P is
+// there.  At 256 (blocks of 128 keys) O, the scores and two P buffers fill tensor
+// memory; at 128 (blocks of 64) two pairs fit an SM pair, and one's MMAs run under
+// the other's softmax, prologue and output.
 //
 // attn_packed_64_kernel (head_dim 64): one CTA takes two query tiles, each with its
-// own softmax warps; while one tile is in its softmax the other's products run.
-//
-// MMAs execute in the order of their issue, so a score buffer may be
-// overwritten by an MMA issued after the one that reads the P in it.
+// own softmax warps; while one tile is in its softmax the other's products run.  P
+// takes the place of the scores it was made from: MMAs execute in the order of
+// their issue, so the next scores may overwrite it by an MMA issued after the one
+// that reads it.
 //
 // Work per 128 x 128 block and head dim HD: 2 * 128 * 128 * HD multiply-adds = 8 HD
 // cycles at 4096 per cycle and SM, and 128 * 128 exponentials = 1024 cycles at 16:
@@ -79,13 +80,13 @@ struct PairCfg {
   static constexpr int NSLOT = HD == 256 ? 5 : 8;
   static constexpr int OFF_BAR = Q_BYTES + NSLOT * SLOT;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
-  static constexpr uint32_t TM_S = HD, TM_COLS = HD == 256 ? 512 : 256;
+  static constexpr uint32_t TM_S = HD, TM_P = HD + KB, TM_COLS = HD + 2 * KB;  // scores, two P buffers of KB / 2
 };
 
 struct Bars {
   uint64_t q_full[2];
   uint64_t full[8], empty[8];
-  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint64_t s_full[2], s_free, p_full[2], pv_done[2];
   uint64_t dirty, clean, drain;
   uint32_t tmem_slot;
   int abort;
@@ -164,18 +165,19 @@ __device__ __forceinline__ void umma_f16_ss_pair(uint32_t tmem_d, uint64_t adesc
       : "memory");
 }
 
-// One query row's part in a block: masks the scores (keys [lo, hi) of the sequence; `whole`: all of them), raises
-// the running maximum and rescales O where a score asks for it, writes P over the scores and adds to the sum.
-// Warp-collective; false when a wait failed.
-template <typename T, int HD, int KB>
-__device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t to, int kb, int lo, int hi, bool whole, float scale2,
-                                              float& m, float& l, uint64_t* pv_done, uint32_t pv_parity,
-                                              volatile int* abort, int* err) {
+// One query row's part in a block: reads the scores (then `loaded()`), masks them (keys [lo, hi) of the sequence;
+// `whole`: all of them), raises the running maximum and rescales O where a score asks for it, once `pv_before()`
+// says that the P V of the block before is complete, writes P to `tp` once `p_free()` says that its place is free,
+// and adds to the sum.  Warp-collective; false when a wait failed.
+template <typename T, int HD, int KB, typename Loaded, typename Before, typename Free>
+__device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t to, int kb, int lo, int hi, bool whole,
+                                              float scale2, float& m, float& l, Loaded loaded, Before pv_before, Free p_free) {
   constexpr int CH = KB / 32;
   uint32_t sv[CH][32];
 #pragma unroll
   for (int c = 0; c < CH; ++c) sbd::tmem_ld_32x32b_x32(ts + 32 * c, sv[c]);
   sbd::tmem_wait_ld();
+  loaded();
   if (!whole) {
     const int v0 = lo - kb, v1 = hi - kb;
 #pragma unroll
@@ -195,7 +197,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t to, int kb, 
   const bool rise = !start && mx2 > m + kRise;
   if (__any_sync(0xFFFFFFFFu, rise)) {
     // O += P V of the block before has to be complete before it is scaled
-    if (!__all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(pv_done, pv_parity, abort, err))) return false;
+    if (!__all_sync(0xFFFFFFFFu, pv_before())) return false;
     sbd::tc_fence_after();
     const float alpha = rise ? ex2(m - mx2) : 1.f;
 #pragma unroll 1
@@ -212,6 +214,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t to, int kb, 
   }
   if (start || rise) m = mx2;
   const float mu = m == -INFINITY ? 0.f : m;
+  if (!__all_sync(0xFFFFFFFFu, p_free())) return false;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     uint32_t pk[16];
@@ -225,7 +228,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t to, int kb, 
       pk[e] = sbp::pack2<T>(p0, p1);
     }
     l += ls[0] + ls[1];
-    sbd::tmem_st_32x32b_x16(ts + 16 * c, pk);
+    sbd::tmem_st_32x32b_x16(tp + 16 * c, pk);
   }
   sbd::tmem_wait_st();
   sbd::tc_fence_before();
@@ -312,7 +315,6 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      sbd::mbar_init(&bars->s_full[i], 1);
       sbd::mbar_init(&bars->p_full[i], 8);
       sbd::mbar_init(&bars->pv_done[i], 1);
     }
@@ -321,6 +323,8 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
       sbd::mbar_init(&bars->empty[i], 1);
     }
     sbd::mbar_init(&bars->q_full[0], 1);
+    sbd::mbar_init(&bars->s_full[0], 1);
+    sbd::mbar_init(&bars->s_free, 8);
     sbd::mbar_init(&bars->dirty, 1);
     sbd::mbar_init(&bars->clean, 4);
     sbd::mbar_init(&bars->drain, 1);
@@ -400,20 +404,23 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
           slot_wait(it);
           if (!ok) return;
           sbd::tc_fence_after();
-          const uint32_t d = tmem + C::TM_S + (j & 1) * KB;
+          const uint32_t d = tmem + C::TM_S;
           const uint64_t k = kd + static_cast<uint64_t>((it % NSLOT) * (C::SLOT >> 4));
   #pragma unroll
           for (int s = 0; s < HD / 16; ++s)
             umma_f16_ss_pair(d, qd + (s >> 2) * (QR * 128 >> 4) + (s & 3) * 2, k + (s >> 2) * (KB / 2 * 128 >> 4) + (s & 3) * 2,
                              idesc_s, s > 0 ? 1u : 0u);
           sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
-          sbd::umma_commit_pair(&bars->s_full[j & 1], kBoth);
+          sbd::umma_commit_pair(&bars->s_full[0], kBoth);
           ++it;
         };
         ok = sbd::mbar_wait_cluster(&bars->q_full[0], 0, abort, p.err);
         if (ok) scores(0);
         for (int j = 0; j < nb && ok; ++j) {
-          if (j + 1 < nb) scores(j + 1);
+          if (j + 1 < nb) {  // the scores' columns are free once every row has read them
+            ok = sbd::mbar_wait_cluster(&bars->s_free, j & 1, abort, p.err);
+            if (ok) scores(j + 1);
+          }
           if (ok) slot_wait(it);
           if (ok && cleans && j0 + j == j_end) {
             sbd::mbar_arrive(&bars->dirty);
@@ -428,7 +435,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
           const uint64_t v = vd + static_cast<uint64_t>((it % NSLOT) * (C::SLOT >> 4));
   #pragma unroll
           for (int s = 0; s < KB / 16; ++s)
-            sbd::umma_f16_ts_pair(tmem, tmem + C::TM_S + buf * KB + s * 8, v + s * (2048 >> 4), idesc_o, j > 0 || s > 0 ? 1u : 0u);
+            sbd::umma_f16_ts_pair(tmem, tmem + C::TM_P + buf * (KB / 2) + s * 8, v + s * (2048 >> 4), idesc_o, j > 0 || s > 0 ? 1u : 0u);
           sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
           sbd::umma_commit_pair(&bars->pv_done[buf], kBoth);
           ++it;
@@ -452,32 +459,39 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
     }
   } else {
     // ------------------------------------------------------------ softmax and output
-    // P V of block j completes in the phases of a barrier per score buffer: the scores of
-    // block j + 1 do not wait for P V of block j, and one barrier's phases could be mistaken two blocks apart.  A
-    // buffer's scores are issued after the P V that read it, so its barrier is never more than a phase behind.
+    // P V of block j completes in the phases of a barrier per P buffer: the scores of block j + 1 do not wait for P V
+    // of block j, and one barrier's phases could be mistaken two blocks apart.  A buffer is written only after its
+    // last P V, so no wait is more than a phase behind.
     const int quad = warp & 3;
     const Row r = row_of(p, tl, rank, quad * 32 + lane, k_len);
     const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t p_lead = sbd::mapa_shared(sbd::smem_u32(&bars->p_full[0]), 0);
+    const uint32_t lead_bar = sbd::mapa_shared(sbd::smem_u32(bars), 0);
+    // a warp's arrival on a barrier of the even CTA
+    auto arrive = [&](uint64_t* bar) {
+      __syncwarp();
+      if (lane == 0) {
+        if (lead) sbd::mbar_arrive(bar);
+        else sbd::mbar_arrive_remote_cta(lead_bar + static_cast<uint32_t>(reinterpret_cast<uint8_t*>(bar) - reinterpret_cast<uint8_t*>(bars)));
+      }
+    };
+    auto pv_complete = [&](int j) { return sbd::mbar_wait_cluster(&bars->pv_done[j & 1], (j >> 1) & 1, abort, p.err); };
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nb && ok; ++j) {
       const int buf = j & 1, kb = (j0 + j) * KB;
-      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->s_full[buf], (j >> 1) & 1, abort, p.err));
+      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->s_full[0], j & 1, abort, p.err));
       if (!ok) break;
       sbd::tc_fence_after();
-      ok = softmax_block<T, HD, KB>(tm + C::TM_S + buf * KB, tm, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m,
-                                l, &bars->pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort, p.err);
-      __syncwarp();
-      if (lane == 0 && ok) {
-        if (lead) sbd::mbar_arrive(&bars->p_full[buf]);
-        else sbd::mbar_arrive_remote_cta(p_lead + buf * sizeof(uint64_t));
-      }
+      ok = softmax_block<T, HD, KB>(
+          tm + C::TM_S, tm + C::TM_P + buf * (KB / 2), tm, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m, l,
+          [&] {
+            sbd::tc_fence_before();
+            arrive(&bars->s_free);
+          },
+          [&] { return pv_complete(j - 1); }, [&] { return j < 2 || pv_complete(j - 2); });
+      if (ok) arrive(&bars->p_full[buf]);
     }
-    if (ok && nb > 0) {
-      const int e = nb - 1;
-      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->pv_done[e & 1], (e >> 1) & 1, abort, p.err));
-    }
+    if (ok && nb > 0) ok = __all_sync(0xFFFFFFFFu, pv_complete(nb - 1));
     if (ok) {
       sbd::tc_fence_after();
       const int64_t token = static_cast<int64_t>(tl.q0) + rank * p.tpt + r.tok;
@@ -646,8 +660,10 @@ __global__ void __launch_bounds__(Cfg64::THREADS, 1)
       ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->s_full[i], j & 1, abort, p.err));
       if (!ok) break;
       sbd::tc_fence_after();
-      ok = softmax_block<T, HD, KB>(tm + C::TM_S + i * KB, tm + i * HD, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo,
-                                p.scale2, m, l, &bars->pv_done[i], (j - 1) & 1, abort, p.err);
+      const uint32_t ts = tm + C::TM_S + i * KB;  // P takes the place of the scores it was made from
+      ok = softmax_block<T, HD, KB>(
+          ts, ts, tm + i * HD, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m, l, [] {},
+          [&] { return sbd::mbar_wait(&bars->pv_done[i], (j - 1) & 1, abort, p.err); }, [] { return true; });
       __syncwarp();
       if (lane == 0 && ok) sbd::mbar_arrive(&bars->p_full[i]);
     }
