@@ -167,11 +167,10 @@ __device__ __forceinline__ void umma_f16_ss_pair(uint32_t tmem_d, uint64_t adesc
 
 // One query row's part in a block: reads the scores (then `loaded()`), masks them (keys [lo, hi) of the sequence;
 // `whole`: all of them), raises the running maximum and rescales O where a score asks for it, once `pv_before()`
-// says that the P V of the block before is complete, writes P to `tp` once `p_free()` says that its place is free,
-// and adds to the sum.  Warp-collective; false when a wait failed.
-template <typename T, int HD, int KB, typename Loaded, typename Before, typename Free>
+// says that the P V of the block before is complete, writes P to `tp` and adds to the sum.  Warp-collective; false when a wait failed.
+template <typename T, int HD, int KB, typename Loaded, typename Before>
 __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t to, int kb, int lo, int hi, bool whole,
-                                              float scale2, float& m, float& l, Loaded loaded, Before pv_before, Free p_free) {
+                                              float scale2, float& m, float& l, Loaded loaded, Before pv_before) {
   constexpr int CH = KB / 32;
   uint32_t sv[CH][32];
 #pragma unroll
@@ -214,7 +213,6 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
   }
   if (start || rise) m = mx2;
   const float mu = m == -INFINITY ? 0.f : m;
-  if (!__all_sync(0xFFFFFFFFu, p_free())) return false;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     uint32_t pk[16];
@@ -235,9 +233,13 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
   return true;
 }
 
-// A finished row: O / l to memory (zeros where the row saw no key).  Warp-collective.
+// A warp's 32 finished rows: O / l to memory (zeros where a row saw no key), `dst` and `store` each lane's own row's.
+// The rows go through shared memory (`stage`: 32 rows of HD, the idle Q tile's; 16-byte chunks swizzled by the row, so
+// that neither side conflicts), because a lane's own row straight from registers would be 32 rows per store.
 template <typename T, int HD>
-__device__ __forceinline__ void store_row(uint32_t to, float l, T* dst, bool store) {
+__device__ __forceinline__ void store_rows(uint32_t to, float l, uint8_t* stage, T* dst, bool store) {
+  constexpr int CPR = HD / 8;  // chunks per row
+  const int lane = threadIdx.x & 31;
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
 #pragma unroll
   for (int c = 0; c < HD / 32; ++c) {
@@ -250,8 +252,18 @@ __device__ __forceinline__ void store_row(uint32_t to, float l, T* dst, bool sto
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         w[q] = l == 0.f ? 0u : sbp::pack2<T>(__uint_as_float(ov[e + 2 * q]) * inv, __uint_as_float(ov[e + 2 * q + 1]) * inv);
-      if (store) *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(stage + lane * (HD * 2) + (((4 * c + e / 8) ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
+  }
+  __syncwarp();
+  const unsigned stored = __ballot_sync(0xFFFFFFFFu, store);
+  const unsigned long long mine = reinterpret_cast<unsigned long long>(dst);
+#pragma unroll 4
+  for (int i = 0; i < CPR; ++i) {
+    const int row = i * (32 / CPR) + lane / CPR, chunk = lane % CPR;
+    const unsigned long long to_row = __shfl_sync(0xFFFFFFFFu, mine, row);
+    const uint4 v = *reinterpret_cast<const uint4*>(stage + row * (HD * 2) + ((chunk ^ (row & 7)) * 16));
+    if (stored >> row & 1) *reinterpret_cast<uint4*>(to_row + chunk * 16) = v;
   }
 }
 
@@ -366,7 +378,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
         bool ok = true;
         auto load = [&](bool is_v, int j) {  // this CTA's half of block j of K or V into the next slot
           const int st = it % NSLOT;
-          ok = ok && sbd::mbar_wait_cluster(&bars->empty[st], ((it / NSLOT) & 1) ^ 1, abort, p.err);
+          ok = ok && sbd::mbar_wait(&bars->empty[st], ((it / NSLOT) & 1) ^ 1, abort, p.err);
           if (!ok) return;
           uint8_t* dst = smem + C::Q_BYTES + st * C::SLOT;
           if (lead) sbd::mbar_arrive_expect_tx(&bars->full[st], 2 * C::SLOT);
@@ -399,7 +411,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
         const uint64_t vd = sbd::umma_desc(sbd::smem_u32(smem + C::Q_BYTES), KB * 128, 1024, sbd::kLayoutSwizzle128B);
         int it = 0;
         bool ok = true;
-        auto slot_wait = [&](int i) { ok = ok && sbd::mbar_wait_cluster(&bars->full[i % NSLOT], (i / NSLOT) & 1, abort, p.err); };
+        auto slot_wait = [&](int i) { ok = ok && sbd::mbar_wait(&bars->full[i % NSLOT], (i / NSLOT) & 1, abort, p.err); };
         auto scores = [&](int j) {  // S(j) = Q K_j^T
           slot_wait(it);
           if (!ok) return;
@@ -414,21 +426,21 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
           sbd::umma_commit_pair(&bars->s_full[0], kBoth);
           ++it;
         };
-        ok = sbd::mbar_wait_cluster(&bars->q_full[0], 0, abort, p.err);
+        ok = sbd::mbar_wait(&bars->q_full[0], 0, abort, p.err);
         if (ok) scores(0);
         for (int j = 0; j < nb && ok; ++j) {
           if (j + 1 < nb) {  // the scores' columns are free once every row has read them
-            ok = sbd::mbar_wait_cluster(&bars->s_free, j & 1, abort, p.err);
+            ok = sbd::mbar_wait(&bars->s_free, j & 1, abort, p.err);
             if (ok) scores(j + 1);
           }
           if (ok) slot_wait(it);
           if (ok && cleans && j0 + j == j_end) {
             sbd::mbar_arrive(&bars->dirty);
             sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->dirty), 1));
-            ok = sbd::mbar_wait_cluster(&bars->clean, 0, abort, p.err);
+            ok = sbd::mbar_wait_cluster(&bars->clean, 0, abort, p.err);  // shared memory that the other CTA wrote
           }
           const int buf = j & 1;
-          ok = ok && sbd::mbar_wait_cluster(&bars->p_full[buf], (j >> 1) & 1, abort, p.err);
+          ok = ok && sbd::mbar_wait(&bars->p_full[buf], (j >> 1) & 1, abort, p.err);
           if (!ok) break;
           sbd::tc_fence_after();
           // O += P V_j
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
       // ------------------------------------------------------------ V rows past the sequence's end
       if (cleans) {
         const int j = j_end - j0, item = min(j + 2, nb) + j;  // in the producer's order
-        if (__all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->dirty, 0, abort, p.err))) {
+        if (__all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->dirty, 0, abort, p.err))) {
           zero_rows<KB>(smem + C::Q_BYTES + item % NSLOT * C::SLOT, HD / 128, k_len % KB, threadIdx.x - 64);
           if (lane == 0) {
             if (lead) sbd::mbar_arrive(&bars->clean);
@@ -460,8 +472,9 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
   } else {
     // ------------------------------------------------------------ softmax and output
     // P V of block j completes in the phases of a barrier per P buffer: the scores of block j + 1 do not wait for P V
-    // of block j, and one barrier's phases could be mistaken two blocks apart.  A buffer is written only after its
-    // last P V, so no wait is more than a phase behind.
+    // of block j, and one barrier's phases could be mistaken two blocks apart.  They do follow P V of block j - 1
+    // in the order of issue, and a commit counts every MMA before it: scores of block j in place say that P V of block
+    // j - 2 is done, so its P buffer is free, and that no wait on pv_done is more than a phase behind.
     const int quad = warp & 3;
     const Row r = row_of(p, tl, rank, quad * 32 + lane, k_len);
     const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -474,12 +487,12 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
         else sbd::mbar_arrive_remote_cta(lead_bar + static_cast<uint32_t>(reinterpret_cast<uint8_t*>(bar) - reinterpret_cast<uint8_t*>(bars)));
       }
     };
-    auto pv_complete = [&](int j) { return sbd::mbar_wait_cluster(&bars->pv_done[j & 1], (j >> 1) & 1, abort, p.err); };
+    auto pv_complete = [&](int j) { return sbd::mbar_wait(&bars->pv_done[j & 1], (j >> 1) & 1, abort, p.err); };
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nb && ok; ++j) {
       const int buf = j & 1, kb = (j0 + j) * KB;
-      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait_cluster(&bars->s_full[0], j & 1, abort, p.err));
+      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->s_full[0], j & 1, abort, p.err));
       if (!ok) break;
       sbd::tc_fence_after();
       ok = softmax_block<T, HD, KB>(
@@ -488,7 +501,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
             sbd::tc_fence_before();
             arrive(&bars->s_free);
           },
-          [&] { return pv_complete(j - 1); }, [&] { return j < 2 || pv_complete(j - 2); });
+          [&] { return pv_complete(j - 1); });
       if (ok) arrive(&bars->p_full[buf]);
     }
     if (ok && nb > 0) ok = __all_sync(0xFFFFFFFFu, pv_complete(nb - 1));
@@ -496,7 +509,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
       sbd::tc_fence_after();
       const int64_t token = static_cast<int64_t>(tl.q0) + rank * p.tpt + r.tok;
       T* dst = static_cast<T*>(p.out) + token * p.out_token + static_cast<int64_t>(kv * p.group + r.head) * p.out_head;
-      store_row<T, HD>(tm, l, dst, r.ok && token >= 0 && token < p.t_q);
+      store_rows<T, HD>(tm, l, smem + quad * (32 * HD * 2), dst, r.ok && token >= 0 && token < p.t_q);
     }
   }
 
@@ -663,7 +676,7 @@ __global__ void __launch_bounds__(Cfg64::THREADS, 1)
       const uint32_t ts = tm + C::TM_S + i * KB;  // P takes the place of the scores it was made from
       ok = softmax_block<T, HD, KB>(
           ts, ts, tm + i * HD, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m, l, [] {},
-          [&] { return sbd::mbar_wait(&bars->pv_done[i], (j - 1) & 1, abort, p.err); }, [] { return true; });
+          [&] { return sbd::mbar_wait(&bars->pv_done[i], (j - 1) & 1, abort, p.err); });
       __syncwarp();
       if (lane == 0 && ok) sbd::mbar_arrive(&bars->p_full[i]);
     }
@@ -672,7 +685,7 @@ __global__ void __launch_bounds__(Cfg64::THREADS, 1)
       sbd::tc_fence_after();
       const int64_t token = static_cast<int64_t>(tl.q0) + i * p.tpt + r.tok;
       T* dst = static_cast<T*>(p.out) + token * p.out_token + static_cast<int64_t>(kv * p.group + r.head) * p.out_head;
-      store_row<T, HD>(tm + i * HD, l, dst, r.ok && token >= 0 && token < p.t_q);
+      store_rows<T, HD>(tm + i * HD, l, smem + i * C::Q_BYTES + quad * (32 * HD * 2), dst, r.ok && token >= 0 && token < p.t_q);
     }
   }
 
