@@ -612,14 +612,15 @@ typedef struct sb_paged_kv {
  * j < rot/2, values from rot on pass through (rot a multiple of 16, 0 for no
  * rotation; cos_t, sin_t f32 [max_pos][rot/2]).  q goes to q_out
  * [t][n_heads][head_dim] in the cache's type (NULL: not wanted), k and v to
- * position pos[i] of the sequence of page-table row seq[i] (seq NULL: row i).
- * A token with pos[i] outside [0, max_pos) is padding: its q is zero and
- * nothing is appended.  Two tokens of one call must not share a place.
+ * position pos[i] of the sequence of page-table row seq[i] (seq NULL: row i) and, when
+ * k_out / v_out [t][n_kv_heads][head_dim] are given, there too (the packed keys and
+ * values of sb_attn_prefill_packed).  A token with pos[i] outside [0, max_pos) is
+ * padding: its rows are zero and nothing is appended.  Two tokens of one call must not share a place.
  */
 int sb_kv_append_paged(const sb_paged_kv* kv, const int32_t* page_table, int n_seqs, int max_pages, const void* qkv,
                        int qkv_dtype, int64_t ld, int t, int n_heads, const int32_t* seq, const int32_t* pos,
                        const float* q_norm, const float* k_norm, int v_norm, float eps, const float* cos_t,
-                       const float* sin_t, int rot, int max_pos, void* q_out, void* stream);
+                       const float* sin_t, int rot, int max_pos, void* q_out, void* k_out, void* v_out, void* stream);
 
 /*
  * Attention of one new token per sequence: out[i][h] = softmax(scale *

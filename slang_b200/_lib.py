@@ -79,7 +79,7 @@ SIGNATURES = {
                               _vp, _i, _vp, _vp, _sz, _vp], _i),
     "sb_decode_step_fused_scratch_size": ([_i, _i, _i, _i, _i], _sz),
     "sb_kv_append_paged": ([_vp, _vp, _i, _i, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _vp, _i, _f, _vp, _vp, _i, _i, _vp,
-                            _vp], _i),
+                            _vp, _vp, _vp], _i),
     "sb_attn_decode_paged": ([_vp, _vp, _i, _vp, _i, _vp, _i64, _i, _i, _f, _vp, _vp, _sz, _vp], _i),
     "sb_attn_decode_paged_workspace_size": ([_vp, _i, _i], _sz),
     "sb_attn_packed_plan": ([_vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp], _i),

@@ -18,7 +18,7 @@ namespace {
 struct AppendParams {
   const void* qkv;
   int64_t ld;
-  void* q_out;
+  void *q_out, *k_out, *v_out;
   const float *q_norm, *k_norm, *cos_t, *sin_t;
   const int32_t *seq, *pos;
   sbp::Pages pages;
@@ -55,14 +55,21 @@ __global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendParams p)
   }
   const int pos = p.pos[tok];
   const int seq = p.seq ? p.seq[tok] : tok;
-  D* q_row = static_cast<D*>(p.q_out) + static_cast<int64_t>(tok) * p.nh * HD;
-  if (pos < 0 || pos >= p.max_pos) {  // padding (the whole warp): its q is zero, nothing is appended
+  // where a head's packed row goes: q, and k and v when they are wanted; null: nowhere
+  auto out_row = [&](int head) -> D* {
+    if (head < p.nh) return p.q_out ? static_cast<D*>(p.q_out) + (static_cast<int64_t>(tok) * p.nh + head) * HD : nullptr;
+    const bool v = head >= p.nh + p.nkv;
+    D* base = static_cast<D*>(v ? p.v_out : p.k_out);
+    return base && head < heads ? base + (static_cast<int64_t>(tok) * p.nkv + head - p.nh - (v ? p.nkv : 0)) * HD : nullptr;
+  };
+  if (pos < 0 || pos >= p.max_pos) {  // padding (the whole warp): zero rows, nothing is appended
     const float zero[8] = {};
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (!p.q_out || head0 + r * HPW >= p.nh) continue;
-      sbp::store8(q_row + (head0 + r * HPW) * HD + at0, zero);
-      sbp::store8(q_row + (head0 + r * HPW) * HD + at1, zero);
+      D* dst = out_row(head0 + r * HPW);
+      if (!dst) continue;
+      sbp::store8(dst + at0, zero);
+      sbp::store8(dst + at1, zero);
     }
     return;
   }
@@ -113,11 +120,14 @@ __global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendParams p)
         x[r][1][e] = b * c[e] + a * sn[e];
       }
     }
-    // nothing is stored for a head past the last, a q that is not wanted, a key or value without a page
-    if (head >= heads || (is_q ? !p.q_out : page < 0)) continue;
-    D* dst = is_q ? q_row + head * HD
-                  : static_cast<D*>(const_cast<void*>(is_v ? p.pages.v : p.pages.k)) + kv_row +
-                        (head - p.nh - (is_v ? p.nkv : 0)) * p.pages.head_stride;
+    D* dst = out_row(head);
+    if (dst) {
+      sbp::store8(dst + at0, x[r][0]);
+      sbp::store8(dst + at1, x[r][1]);
+    }
+    if (is_q || head >= heads || page < 0) continue;  // a key or value without a page is not appended
+    dst = static_cast<D*>(const_cast<void*>(is_v ? p.pages.v : p.pages.k)) + kv_row +
+          (head - p.nh - (is_v ? p.nkv : 0)) * p.pages.head_stride;
     sbp::store8(dst + at0, x[r][0]);
     sbp::store8(dst + at1, x[r][1]);
   }
@@ -168,7 +178,7 @@ extern "C" int sb_kv_append_paged(const sb_paged_kv* kv, const int32_t* page_tab
                                   const void* qkv, int qkv_dtype, int64_t ld, int t, int n_heads, const int32_t* seq,
                                   const int32_t* pos, const float* q_norm, const float* k_norm, int v_norm, float eps,
                                   const float* cos_t, const float* sin_t, int rot, int max_pos, void* q_out,
-                                  void* stream) {
+                                  void* k_out, void* v_out, void* stream) {
   AppendParams p{};
   int rc = sbp::check_pages("sb_kv_append_paged", kv, page_table, max_pages, &p.pages);
   if (rc) return rc;
@@ -180,10 +190,11 @@ extern "C" int sb_kv_append_paged(const sb_paged_kv* kv, const int32_t* page_tab
   SB_CHECK_ARG(qkv && pos && (rot == 0 || (cos_t && sin_t)), "sb_kv_append_paged: null pointer");
   SB_CHECK_ARG(seq || t <= n_seqs, "sb_kv_append_paged: without `seq`, token i is sequence i: %d tokens, %d sequences", t, n_seqs);
   const int vec = qkv_dtype == SB_F32 ? 4 : 8;
-  if (!sb::aligned(qkv, 16) || ld % vec || !sb::aligned(q_out, 16) || !sb::aligned(cos_t, 16) || !sb::aligned(sin_t, 16) ||
+  if (!sb::aligned(qkv, 16) || ld % vec || !sb::aligned(q_out, 16) || !sb::aligned(k_out, 16) ||
+      !sb::aligned(v_out, 16) || !sb::aligned(cos_t, 16) || !sb::aligned(sin_t, 16) ||
       !sb::aligned(q_norm, 16) || !sb::aligned(k_norm, 16))
     return sb::fail(SB_ERR_ALIGN, "sb_kv_append_paged: rows, tables and norm weights must start on 16-byte boundaries");
-  p.qkv = qkv, p.ld = ld, p.q_out = q_out, p.q_norm = q_norm, p.k_norm = k_norm, p.cos_t = cos_t, p.sin_t = sin_t;
+  p.qkv = qkv, p.ld = ld, p.q_out = q_out, p.k_out = k_out, p.v_out = v_out, p.q_norm = q_norm, p.k_norm = k_norm, p.cos_t = cos_t, p.sin_t = sin_t;
   p.seq = seq, p.pos = pos, p.t = t, p.n_seqs = n_seqs, p.nh = n_heads, p.nkv = kv->n_kv_heads, p.rot = rot;
   p.max_pos = max_pos, p.v_norm = v_norm, p.eps = eps;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

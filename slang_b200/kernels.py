@@ -660,7 +660,8 @@ class PagedKV:
 def kv_append_paged(qkv: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, pos: torch.Tensor,
                     cos: torch.Tensor, sin: torch.Tensor, n_heads: int, seq: torch.Tensor | None = None,
                     q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, v_norm: bool = False,
-                    eps: float = 1e-6, q_out: torch.Tensor | None = None) -> torch.Tensor:
+                    eps: float = 1e-6, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
+                    v_out: torch.Tensor | None = None) -> torch.Tensor:
     """Normalise (optionally), rotate and append new tokens to a paged cache
     (``sb_kv_append_paged``); returns the rotated queries [t, n_heads, head_dim] in the
     cache's type.
@@ -669,7 +670,9 @@ def kv_append_paged(qkv: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     ``page_table`` [n_seqs, max_pages] and ``pos`` [t] int32; ``seq`` [t] int32 is each
     token's row of the page table (None: token i is sequence i, a decode step).
     ``cos`` / ``sin`` [max_pos, rot/2] f32 rotate values j and j + rot/2 of every q and k
-    head.  A token whose position is negative or past the tables is padding."""
+    head.  A token whose position is negative or past the tables is padding.  ``k_out`` /
+    ``v_out`` [t, n_kv_heads, head_dim] receive the same keys and values packed, for
+    :func:`attn_prefill_packed`."""
     gpu, hd = _gpu(qkv, "qkv"), cache.head_dim
     src = _DT_ALL.get(qkv.dtype)
     if src is None:
@@ -693,11 +696,15 @@ def kv_append_paged(qkv: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     elif q_out.dtype is not cache.dtype or q_out.shape != (t, n_heads, hd) or not q_out.is_contiguous() or \
             q_out.get_device() != gpu:
         raise ValueError(f"q_out must be a contiguous [{t}, {n_heads}, {hd}] tensor of the cache's type")
+    for o, name in ((k_out, "k_out"), (v_out, "v_out")):
+        if o is not None and (o.dtype is not cache.dtype or o.shape != (t, cache.n_kv_heads, hd) or
+                              not o.is_contiguous() or o.get_device() != gpu):
+            raise ValueError(f"{name} must be a contiguous [{t}, {cache.n_kv_heads}, {hd}] tensor of the cache's type")
     _lib.call("sb_kv_append_paged", cache.ptr, page_table.data_ptr(), n_seqs, max_pages, qkv.data_ptr(), src,
               qkv.stride(0) if t > 1 else width, t, n_heads, _vec(seq, "seq", _I32, t, gpu),
               _vec(pos, "pos", _I32, t, gpu), _vec(q_norm, "q_norm", _F32T, hd, gpu),
               _vec(k_norm, "k_norm", _F32T, hd, gpu), v_norm, eps, cos.data_ptr(), sin.data_ptr(), 2 * half, max_pos,
-              q_out.data_ptr(), _raw_stream(gpu))
+              q_out.data_ptr(), _ptr(k_out), _ptr(v_out), _raw_stream(gpu))
     return q_out
 
 

@@ -116,6 +116,30 @@ def test_kv_append_padding_and_missing_pages(cuda):
     assert torch.all(q == 0)
 
 
+def test_kv_append_packed_outputs(cuda):
+    """k_out and v_out hold what the pages hold, and zero rows for padding."""
+    gen = torch.Generator(device=cuda).manual_seed(6)
+    cache = _cache(6, 3, 8, 128, torch.bfloat16, "token", gen, cuda)
+    table = torch.tensor([[4, 1], [0, 5]], dtype=torch.int32, device=cuda)
+    qkv = torch.randn(5, 12 * 128, generator=gen, device=cuda).half()
+    qkv[3] = math.nan
+    seq = torch.tensor([0, 1, 1, 0, 0], dtype=torch.int32, device=cuda)
+    pos = torch.tensor([9, 0, 15, -1, 2], dtype=torch.int32, device=cuda)
+    cos = torch.rand(16, 64, generator=gen, device=cuda)
+    k, v = (torch.full((5, 3, 128), 7.0, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    q = kern.kv_append_paged(qkv, cache, table, pos, cos, cos, 6, seq=seq, k_out=k, v_out=v)
+    for i, (s, p) in enumerate(zip(seq.tolist(), pos.tolist())):
+        if p < 0:
+            assert torch.all(q[i] == 0) and torch.all(k[i] == 0) and torch.all(v[i] == 0)
+            continue
+        pg = int(table[s, p // 8])
+        assert torch.equal(k[i], cache.k[pg, :, p % 8]) and torch.equal(v[i], cache.v[pg, :, p % 8])
+    with pytest.raises(ValueError):
+        kern.kv_append_paged(qkv, cache, table, pos, cos, cos, 6, seq=seq, k_out=k[:4])
+    with pytest.raises(ValueError):
+        kern.kv_append_paged(qkv, cache, table, pos, cos, cos, 6, seq=seq, v_out=v.half())
+
+
 def test_kv_append_nothing(cuda):
     cache = kern.PagedKV.allocate(2, 16, 1, 64, device=cuda)
     none = torch.zeros(0, dtype=torch.int32, device=cuda)
