@@ -128,8 +128,7 @@ def load() -> C.CDLL:
 
 def call(name: str, *args) -> int:
     """Call an entry point; raise SlangError on a non-zero status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc != SB_OK:
-        raise SlangError(name, rc, lib.sb_last_error().decode(errors="replace"))
+        raise SlangError(name, rc, _lib.sb_last_error().decode(errors="replace"))
     return rc

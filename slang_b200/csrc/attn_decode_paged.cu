@@ -415,6 +415,19 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
       auto join = [&](int n, auto of, bool final) {
         float* wgt = sm_o;  // [n][HT] weights, then [HT] sums; the teams' O is no longer needed
         float* ls = wgt + (JOIN + 2) * HT;
+        // Every thread has the loads of several parts of its vectors in flight at once, the first of them before the
+        // weights are known.
+        constexpr int VPT = HT * HD / 4 / (W * 32), UX = VPT >= 16 ? 2 : 32 / VPT > 8 ? 8 : 32 / VPT;
+        float4 acc[VPT], v[UX][VPT];
+        auto fetch = [&](int x) {
+#pragma unroll
+          for (int y = 0; y < UX; ++y) {
+            const float4* src = reinterpret_cast<const float4*>(slot(of(min(x + y, n - 1)))) + threadIdx.x;
+#pragma unroll
+            for (int u = 0; u < VPT; ++u) v[y][u] = __ldcg(src + u * W * 32);
+          }
+        };
+        fetch(0);
         for (int i = threadIdx.x; i < n * HT; i += W * 32) {
           const float* src = slot(of(i / HT)) + HT * HD + i % HT;
           wgt[i] = __ldcg(src);
@@ -435,19 +448,10 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
           wgt[(n + 1) * HT + h] = M;
         }
         __syncthreads();
-        // every thread has the loads of several parts of its vectors in flight at once
-        constexpr int VPT = HT * HD / 4 / (W * 32), UX = VPT >= 16 ? 2 : 32 / VPT > 8 ? 8 : 32 / VPT;
-        float4 acc[VPT];
 #pragma unroll
         for (int u = 0; u < VPT; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int x = 0; x < n; x += UX) {
-          float4 v[UX][VPT];
-#pragma unroll
-          for (int y = 0; y < UX; ++y) {
-            const float4* src = reinterpret_cast<const float4*>(slot(of(min(x + y, n - 1)))) + threadIdx.x;
-#pragma unroll
-            for (int u = 0; u < VPT; ++u) v[y][u] = __ldcg(src + u * W * 32);
-          }
+          if (x) fetch(x);
 #pragma unroll
           for (int y = 0; y < UX; ++y)
 #pragma unroll

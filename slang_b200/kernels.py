@@ -598,16 +598,17 @@ def _num_sms(dev) -> int:
 _I32, _I64, _F32T = torch.int32, torch.int64, torch.float32
 _DT_PAGED = {torch.float16: SB_F16, torch.bfloat16: SB_BF16}
 _DT_ALL = {torch.float16: SB_F16, torch.bfloat16: SB_BF16, torch.float32: SB_F32}
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_empty = torch.empty
 
 
 def _gpu(t: torch.Tensor, name: str) -> int:
     """The GPU of an operator's leading tensor, which has to be the current one."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    gpu = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if gpu < 0:
         raise ValueError(f"{name} must be a CUDA tensor")
-    gpu = t.get_device()
-    if gpu != torch.cuda.current_device():
-        raise ValueError(f"{name} is on cuda:{gpu}, the current device is cuda:{torch.cuda.current_device()}")
+    if gpu != _current_device():
+        raise ValueError(f"{name} is on cuda:{gpu}, the current device is cuda:{_current_device()}")
     return gpu
 
 
@@ -622,7 +623,7 @@ def _vec(t: torch.Tensor | None, name: str, dtype, n: int, gpu: int) -> int | No
     """Address of a contiguous vector of n values (None passes through)."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous() or t.get_device() != gpu:
+    if t.dtype is not dtype or t.numel() != n or t.dim() != 1 or not t.is_contiguous() or t.get_device() != gpu:
         _refuse(t, name, dtype, (n,), gpu)
     return t.data_ptr()
 
@@ -673,34 +674,35 @@ def kv_append_paged(qkv: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     head.  A token whose position is negative or past the tables is padding.  ``k_out`` /
     ``v_out`` [t, n_kv_heads, head_dim] receive the same keys and values packed, for
     :func:`attn_prefill_packed`."""
-    gpu, hd = _gpu(qkv, "qkv"), cache.head_dim
+    gpu, hd, nkv = _gpu(qkv, "qkv"), cache.head_dim, cache.n_kv_heads
     src = _DT_ALL.get(qkv.dtype)
     if src is None:
         raise TypeError(f"qkv has dtype {qkv.dtype}, expected f16, bf16 or f32")
-    width = (n_heads + 2 * cache.n_kv_heads) * hd
+    width = (n_heads + 2 * nkv) * hd
     if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or gpu != cache.gpu:
         raise ValueError(f"qkv must be [t, {width}] rows with unit column stride on {cache.device}")
     t = qkv.shape[0]
     if page_table.dtype is not _I32 or page_table.dim() != 2 or not page_table.is_contiguous() or \
             page_table.get_device() != gpu:
         _refuse(page_table, "page_table", _I32, ("n_seqs", "max_pages"), gpu)
-    n_seqs, max_pages = page_table.shape
     if cos.dim() != 2 or cos.shape != sin.shape:
         raise ValueError("cos and sin must be [max_pos, rot / 2]")
-    max_pos, half = cos.shape
-    for c, name in ((cos, "cos"), (sin, "sin")):
-        if c.dtype is not _F32T or not c.is_contiguous() or c.get_device() != gpu:
-            _refuse(c, name, _F32T, cos.shape, gpu)
+    if cos.dtype is not _F32T or not cos.is_contiguous() or cos.get_device() != gpu:
+        _refuse(cos, "cos", _F32T, cos.shape, gpu)
+    if sin.dtype is not _F32T or not sin.is_contiguous() or sin.get_device() != gpu:
+        _refuse(sin, "sin", _F32T, sin.shape, gpu)
     if q_out is None:
-        q_out = torch.empty((t, n_heads, hd), dtype=cache.dtype, device=cache.device)
+        q_out = cache.k.new_empty((t, n_heads, hd))
     elif q_out.dtype is not cache.dtype or q_out.shape != (t, n_heads, hd) or not q_out.is_contiguous() or \
             q_out.get_device() != gpu:
         raise ValueError(f"q_out must be a contiguous [{t}, {n_heads}, {hd}] tensor of the cache's type")
-    for o, name in ((k_out, "k_out"), (v_out, "v_out")):
-        if o is not None and (o.dtype is not cache.dtype or o.shape != (t, cache.n_kv_heads, hd) or
-                              not o.is_contiguous() or o.get_device() != gpu):
-            raise ValueError(f"{name} must be a contiguous [{t}, {cache.n_kv_heads}, {hd}] tensor of the cache's type")
-    _lib.call("sb_kv_append_paged", cache.ptr, page_table.data_ptr(), n_seqs, max_pages, qkv.data_ptr(), src,
+    if k_out is not None or v_out is not None:
+        for o, name in ((k_out, "k_out"), (v_out, "v_out")):
+            if o is not None and (o.dtype is not cache.dtype or o.shape != (t, nkv, hd) or not o.is_contiguous() or
+                                  o.get_device() != gpu):
+                raise ValueError(f"{name} must be a contiguous [{t}, {nkv}, {hd}] tensor of the cache's type")
+    max_pos, half = cos.shape
+    _lib.call("sb_kv_append_paged", cache.ptr, page_table.data_ptr(), *page_table.shape, qkv.data_ptr(), src,
               qkv.stride(0) if t > 1 else width, t, n_heads, _vec(seq, "seq", _I32, t, gpu),
               _vec(pos, "pos", _I32, t, gpu), _vec(q_norm, "q_norm", _F32T, hd, gpu),
               _vec(k_norm, "k_norm", _F32T, hd, gpu), v_norm, eps, cos.data_ptr(), sin.data_ptr(), 2 * half, max_pos,
@@ -791,7 +793,7 @@ def attn_prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan:
     if k.get_device() != gpu or v.get_device() != gpu or plan.gpu != gpu:
         raise ValueError(f"k, v and the plan must be on cuda:{gpu}")
     if out is None:
-        out = torch.empty((plan.total_q, nh, hd), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((plan.total_q, nh, hd))
     elif out.dtype is not q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.get_device() != gpu:
         raise ValueError("out must match q, with unit stride in head_dim")
     _lib.call("sb_attn_prefill_packed", q.data_ptr(), _step(q, 0), _step(q, 1), k.data_ptr(), v.data_ptr(), _step(k, 0),
@@ -822,7 +824,7 @@ def sample(logits: torch.Tensor, seeds: torch.Tensor, pos: torch.Tensor, tempera
         raise ValueError("logits must be [rows, vocab] with unit column stride")
     rows, vocab = logits.shape
     if tokens is None:
-        tokens = torch.empty(rows, dtype=_I32, device=logits.device)
+        tokens = _empty(rows, dtype=_I32, device=logits.device)
     _lib.call("sb_sample", logits.data_ptr(), dtype, logits.stride(0) if rows > 1 else vocab, rows, vocab,
               _vec(seeds, "seeds", _I64, rows, gpu), _vec(pos, "pos", _I32, rows, gpu),
               _vec(temperature, "temperature", _F32T, rows, gpu), _vec(top_k, "top_k", _I32, rows, gpu),
