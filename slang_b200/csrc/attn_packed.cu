@@ -84,7 +84,7 @@ struct PairCfg {
 };
 
 struct Bars {
-  uint64_t q_full[2];
+  uint64_t q_full[2], q_free;
   uint64_t full[8], empty[8];
   uint64_t s_full[2], s_free, p_full[2], pv_done[2];
   uint64_t dirty, clean, drain;
@@ -102,7 +102,7 @@ struct PackedParams {
   int64_t out_token, out_head;  // strides, elements
   const Tile* tiles;
   int* err;
-  int t_q, t_k, nkv, group, tpt, window;
+  int t_q, t_k, n_tiles, nkv, group, tpt, window;
   float scale2;  // scale * log2(e)
 };
 
@@ -299,36 +299,41 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
 }
 
 // A warp's 32 finished rows: O / l to memory (zeros where a row saw no key), `dst` and `store` each lane's own row's.
-// The rows go through shared memory (`stage`: 32 rows of HD, the idle Q tile's; 16-byte chunks swizzled by the row, so
-// that neither side conflicts), because a lane's own row straight from registers would be 32 rows per store.
+// Four lanes exchange the 64 bytes that each has of its row at a time, so that a store instruction writes 64 bytes of
+// 8 rows in place of 16 bytes of 32 (a lane's own row straight from registers).
 template <typename T, int HD>
-__device__ __forceinline__ void store_rows(uint32_t to, float l, uint8_t* stage, T* dst, bool store) {
-  constexpr int CPR = HD / 8;  // chunks per row
+__device__ __forceinline__ void store_rows(uint32_t to, float l, T* dst, bool store) {
   const int lane = threadIdx.x & 31;
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+  const unsigned stored = __ballot_sync(0xFFFFFFFFu, store) >> (lane & 28);
+  unsigned long long row[4];
 #pragma unroll
+  for (int r = 0; r < 4; ++r)
+    row[r] = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(dst), (lane & 28) + r) + (lane & 3) * 16;
+#pragma unroll 2
   for (int c = 0; c < HD / 32; ++c) {
-    uint32_t ov[32];
+    uint32_t ov[32], w[4][4];
     sbd::tmem_ld_32x32b_x32(to + 32 * c, ov);
     sbd::tmem_wait_ld();
 #pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-      uint32_t w[4];
+    for (int e = 0; e < 32; e += 2)
+      w[e / 8][e / 2 % 4] = l == 0.f ? 0u : sbp::pack2<T>(__uint_as_float(ov[e]) * inv, __uint_as_float(ov[e + 1]) * inv);
+    // w[i]: chunk i of this lane's row -> chunk (lane & 3) of the group's row i
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        w[q] = l == 0.f ? 0u : sbp::pack2<T>(__uint_as_float(ov[e + 2 * q]) * inv, __uint_as_float(ov[e + 2 * q + 1]) * inv);
-      *reinterpret_cast<uint4*>(stage + lane * (HD * 2) + (((4 * c + e / 8) ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  __syncwarp();
-  const unsigned stored = __ballot_sync(0xFFFFFFFFu, store);
-  const unsigned long long mine = reinterpret_cast<unsigned long long>(dst);
-#pragma unroll 4
-  for (int i = 0; i < CPR; ++i) {
-    const int row = i * (32 / CPR) + lane / CPR, chunk = lane % CPR;
-    const unsigned long long to_row = __shfl_sync(0xFFFFFFFFu, mine, row);
-    const uint4 v = *reinterpret_cast<const uint4*>(stage + row * (HD * 2) + ((chunk ^ (row & 7)) * 16));
-    if (stored >> row & 1) *reinterpret_cast<uint4*>(to_row + chunk * 16) = v;
+    for (int b = 1; b < 4; b *= 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i & b) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, lane & b ? w[i][q] : w[i + b][q], b);
+          if (lane & b) w[i][q] = got;
+          else w[i + b][q] = got;
+        }
+      }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (stored >> r & 1) *reinterpret_cast<uint4*>(row[r] + c * 64) = make_uint4(w[r][0], w[r][1], w[r][2], w[r][3]);
   }
 }
 
@@ -373,6 +378,29 @@ __device__ __forceinline__ void block_range(const PackedParams& p, const Tile& t
   }
 }
 
+// What a pair does at a time: a plan's tile and a kv head.
+struct Item {
+  Tile tl;
+  int kv;
+};
+
+// Key blocks [j0, j0 + nb) that the pair walks together; `unclean`: the one of them that holds the sequence's end
+// inside it, -1 if none does.
+struct Blocks {
+  int k_len, j0, nb, unclean;
+};
+template <int KB>
+__device__ __forceinline__ Blocks blocks_of(const PackedParams& p, const Tile& tl) {
+  Blocks b;
+  int nb[2];
+  b.k_len = min(tl.k_len, p.t_k);
+  block_range<KB>(p, tl, b.k_len, &b.j0, nb);
+  b.nb = max(nb[0], nb[1]);
+  b.unclean = b.k_len % KB ? b.k_len / KB - b.j0 : -1;
+  if (b.unclean >= b.nb) b.unclean = -1;
+  return b;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
     attn_packed_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -388,7 +416,6 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
   const int rank = static_cast<int>(sbd::cluster_ctarank());
   const bool lead = rank == 0;
   sbd::griddep_launch_dependents();
-  const int kv = (blockIdx.x >> 1) % p.nkv;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -400,6 +427,7 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
       sbd::mbar_init(&bars->empty[i], 1);
     }
     sbd::mbar_init(&bars->q_full[0], 1);
+    sbd::mbar_init(&bars->q_free, 1);
     sbd::mbar_init(&bars->s_full[0], 1);
     sbd::mbar_init(&bars->s_free, 8);
     sbd::mbar_init(&bars->dirty, 1);
@@ -417,67 +445,82 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
     sbd::tmem_relinquish_pair();
   }
   sbd::griddep_wait();
-  const Tile tl = p.tiles[(blockIdx.x >> 1) / p.nkv];
   sbd::tc_fence_before();
   sbd::cluster_sync_all();  // both CTAs' barriers exist
   sbd::tc_fence_after();
   const uint32_t tmem = bars->tmem_slot;
-  const int k_len = min(tl.k_len, p.t_k);
-  int nbs[2], j0;
-  block_range<KB>(p, tl, k_len, &j0, nbs);
-  const int nb = max(nbs[0], nbs[1]);  // the pair walks its blocks together
-  // the block that holds the sequence's end inside it, if the pair reads it
-  const int j_end = k_len % KB ? k_len / KB : -1;
-  const bool cleans = j_end >= j0 && j_end < j0 + nb;
+  // A pair stays and takes one tile and kv head after another, there and back over the rest of the plan: the plan's
+  // tiles come in falling order of their keys, so each pair's sum is about the same.  Each role walks the pair's items
+  // by itself, so the loads and scores of one run ahead into the softmax and output of the one before; the rings and
+  // the barriers' phases carry on.
+  const int pairs = gridDim.x >> 1, pair = blockIdx.x >> 1, items = p.n_tiles * p.nkv;
+  auto item_at = [&](int n, Item& it) {
+    const int64_t i = static_cast<int64_t>(n) * pairs + (n & 1 ? pairs - 1 - pair : pair);
+    if (i >= items) return false;
+    it.kv = static_cast<int>(i) % p.nkv;
+    it.tl = p.tiles[i / p.nkv];
+    return true;
+  };
 
   if (warp < 4) {
     if (warp == 0) {
       // ------------------------------------------------------------ TMA producer
-      if (lane == 0 && nb > 0) {
+      if (lane == 0) {
         const int q_bytes = p.tpt * p.group * HD * 2;  // a box of tpt tokens x group heads; tokens past the tensor read as zero
-        if (lead) sbd::mbar_arrive_expect_tx(&bars->q_full[0], 2 * q_bytes);
         const uint32_t q_bar = sbd::mapa_shared(sbd::smem_u32(&bars->q_full[0]), 0);
-        for (int b = 0; b < HD / 64; ++b)
-          tma_load_3d_pair(&tmQ, q_bar, smem + b * (QR * 128), 64 * b, kv * p.group, tl.q0 + rank * p.tpt);
-        int it = 0;
+        int it = 0, nq = 0;
         bool ok = true;
-        auto load = [&](bool is_v, int j) {  // this CTA's half of block j of K or V into the next slot
-          const int st = it % NSLOT;
-          ok = ok && sbd::mbar_wait(&bars->empty[st], ((it / NSLOT) & 1) ^ 1, abort, p.err);
-          if (!ok) return;
-          uint8_t* dst = smem + C::Q_BYTES + st * C::SLOT;
-          if (lead) sbd::mbar_arrive_expect_tx(&bars->full[st], 2 * C::SLOT);
-          const uint32_t bar = sbd::mapa_shared(sbd::smem_u32(&bars->full[st]), 0);
-          if (is_v) {  // 128 keys, dims rank * HD / 2 ...
-            for (int b = 0; b < HD / 128; ++b)
-              tma_load_3d_pair(&tmV, bar, dst + b * (KB * 128), rank * (HD / 2) + 64 * b, kv, tl.k0 + j * KB);
-          } else {  // keys rank * 64 ..., all dims
-            for (int b = 0; b < HD / 64; ++b)
-              tma_load_3d_pair(&tmK, bar, dst + b * (KB / 2 * 128), 64 * b, kv, tl.k0 + j * KB + rank * (KB / 2));
+        Item w;
+        for (int n = 0; ok && item_at(n, w); ++n) {
+          const Blocks blk = blocks_of<KB>(p, w.tl);
+          if (blk.nb == 0) continue;
+          auto load = [&](bool is_v, int j) {  // this CTA's half of block j of K or V into the next slot
+            const int st = it % NSLOT;
+            ok = ok && sbd::mbar_wait(&bars->empty[st], ((it / NSLOT) & 1) ^ 1, abort, p.err);
+            if (!ok) return;
+            uint8_t* dst = smem + C::Q_BYTES + st * C::SLOT;
+            if (lead) sbd::mbar_arrive_expect_tx(&bars->full[st], 2 * C::SLOT);
+            const uint32_t bar = sbd::mapa_shared(sbd::smem_u32(&bars->full[st]), 0);
+            if (is_v) {  // KB keys, dims rank * HD / 2 ...
+              for (int b = 0; b < HD / 128; ++b)
+                tma_load_3d_pair(&tmV, bar, dst + b * (KB * 128), rank * (HD / 2) + 64 * b, w.kv, w.tl.k0 + j * KB);
+            } else {  // keys rank * KB / 2 ..., all dims
+              for (int b = 0; b < HD / 64; ++b)
+                tma_load_3d_pair(&tmK, bar, dst + b * (KB / 2 * 128), 64 * b, w.kv, w.tl.k0 + j * KB + rank * (KB / 2));
+            }
+            ++it;
+          };
+          for (int j = 0; j <= blk.nb && ok; ++j) {
+            if (j < blk.nb) load(false, blk.j0 + j);
+            if (j == 0) {  // Q, once the scores of the tile before are done with it
+              ok = ok && sbd::mbar_wait(&bars->q_free, (nq & 1) ^ 1, abort, p.err);
+              if (!ok) break;
+              if (lead) sbd::mbar_arrive_expect_tx(&bars->q_full[0], 2 * q_bytes);
+              for (int b = 0; b < HD / 64; ++b)
+                tma_load_3d_pair(&tmQ, q_bar, smem + b * (QR * 128), 64 * b, w.kv * p.group, w.tl.q0 + rank * p.tpt);
+              ++nq;
+            } else {
+              load(true, blk.j0 + j - 1);  // the next block's scores come before this block's P V
+            }
           }
-          ++it;
-        };
-        for (int j = 0; j <= nb && ok; ++j) {
-          if (j < nb) load(false, j0 + j);
-          const int vj = j - 1;  // the next block's scores come before this block's P V
-          if (vj >= 0 && vj < nb) load(true, j0 + vj);
         }
         if (*abort && lead) {  // copies in flight land before shared memory is released (the even CTA counts both CTAs')
-          drain_wait(&bars->q_full[0], 0);
+          if (nq > 0) drain_wait(&bars->q_full[0], (nq - 1) & 1);
           for (int i = max(0, it - NSLOT); i < it; ++i) drain_wait(&bars->full[i % NSLOT], (i / NSLOT) & 1);
         }
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer (even CTA)
-      if (lane == 0 && lead && nb > 0) {
+      if (lane == 0 && lead) {
         constexpr uint32_t idesc_s = idesc<T>(2 * QR, KB, 0), idesc_o = idesc<T>(2 * QR, HD, 1);
         const uint64_t qd = sbd::umma_desc(sbd::smem_u32(smem), 16, 1024, sbd::kLayoutSwizzle128B);
         const uint64_t kd = sbd::umma_desc(sbd::smem_u32(smem + C::Q_BYTES), 16, 1024, sbd::kLayoutSwizzle128B);
         const uint64_t vd = sbd::umma_desc(sbd::smem_u32(smem + C::Q_BYTES), KB * 128, 1024, sbd::kLayoutSwizzle128B);
-        int it = 0;
+        int it = 0, nq = 0, g = 0;  // ring items, tiles with keys and blocks so far
         bool ok = true;
         auto slot_wait = [&](int i) { ok = ok && sbd::mbar_wait(&bars->full[i % NSLOT], (i / NSLOT) & 1, abort, p.err); };
-        auto scores = [&](int j) {  // S(j) = Q K_j^T
+        auto scores = [&](bool last) {  // S = Q K_j^T, once every row has read the scores of the block before
+          ok = ok && sbd::mbar_wait(&bars->s_free, (g & 1) ^ 1, abort, p.err);
           slot_wait(it);
           if (!ok) return;
           sbd::tc_fence_after();
@@ -488,50 +531,64 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
             umma_f16_ss_pair(d, qd + (s >> 2) * (QR * 128 >> 4) + (s & 3) * 2, k + (s >> 2) * (KB / 2 * 128 >> 4) + (s & 3) * 2,
                              idesc_s, s > 0 ? 1u : 0u);
           sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
+          if (last) sbd::umma_commit_pair(&bars->q_free, kBoth);
           sbd::umma_commit_pair(&bars->s_full[0], kBoth);
-          ++it;
+          ++it, ++g;
         };
-        ok = sbd::mbar_wait(&bars->q_full[0], 0, abort, p.err);
-        if (ok) scores(0);
-        for (int j = 0; j < nb && ok; ++j) {
-          if (j + 1 < nb) {  // the scores' columns are free once every row has read them
-            ok = sbd::mbar_wait(&bars->s_free, j & 1, abort, p.err);
-            if (ok) scores(j + 1);
-          }
-          if (ok) slot_wait(it);
-          if (ok && cleans && j0 + j == j_end) {
-            sbd::mbar_arrive(&bars->dirty);
-            sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->dirty), 1));
-            ok = sbd::mbar_wait_cluster(&bars->clean, 0, abort, p.err);  // shared memory that the other CTA wrote
-          }
-          const int buf = j & 1;
-          ok = ok && sbd::mbar_wait(&bars->p_full[buf], (j >> 1) & 1, abort, p.err);
-          if (!ok) break;
-          sbd::tc_fence_after();
-          // O += P V_j
-          const uint64_t v = vd + static_cast<uint64_t>((it % NSLOT) * (C::SLOT >> 4));
+        Item w;
+        for (int n = 0; ok && item_at(n, w); ++n) {
+          const Blocks blk = blocks_of<KB>(p, w.tl);
+          if (blk.nb == 0) continue;
+          ok = sbd::mbar_wait(&bars->q_full[0], nq & 1, abort, p.err);
+          scores(blk.nb == 1);
+          for (int j = 0; j < blk.nb && ok; ++j) {
+            if (j + 1 < blk.nb) scores(j + 2 == blk.nb);
+            slot_wait(it);
+            if (ok && j == (blk.unclean >= 0 ? blk.unclean : blk.nb - 1)) {
+              ok = sbd::mbar_wait_cluster(&bars->clean, (nq & 1) ^ 1, abort, p.err);  // the cleaners' answer for the tile before
+              sbd::mbar_arrive(&bars->dirty);
+              sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->dirty), 1));
+              if (blk.unclean >= 0)  // shared memory that the other CTA wrote
+                ok = ok && sbd::mbar_wait_cluster(&bars->clean, nq & 1, abort, p.err);
+            }
+            const int at = j + 1 < blk.nb ? g - 2 : g - 1, buf = at & 1;  // this block's number
+            ok = ok && sbd::mbar_wait(&bars->p_full[buf], (at >> 1) & 1, abort, p.err);
+            if (!ok) break;
+            sbd::tc_fence_after();
+            // O += P V_j.  The first of a tile overwrites the last tile's O: whoever wrote P had read it.
+            const uint64_t v = vd + static_cast<uint64_t>((it % NSLOT) * (C::SLOT >> 4));
   #pragma unroll
-          for (int s = 0; s < KB / 16; ++s)
-            sbd::umma_f16_ts_pair(tmem, tmem + C::TM_P + buf * (KB / 2) + s * 8, v + s * (2048 >> 4), idesc_o, j > 0 || s > 0 ? 1u : 0u);
-          sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
-          sbd::umma_commit_pair(&bars->pv_done[buf], kBoth);
-          ++it;
+            for (int s = 0; s < KB / 16; ++s)
+              sbd::umma_f16_ts_pair(tmem, tmem + C::TM_P + buf * (KB / 2) + s * 8, v + s * (2048 >> 4), idesc_o, j > 0 || s > 0 ? 1u : 0u);
+            sbd::umma_commit_pair(&bars->empty[it % NSLOT], kBoth);
+            sbd::umma_commit_pair(&bars->pv_done[buf], kBoth);
+            ++it;
           }
+          ++nq;
+        }
         // every MMA issued has finished before tensor and shared memory are released
         sbd::umma_commit_pair(&bars->drain, kBoth);
         drain_wait(&bars->drain, 0);
       }
     } else {
       // ------------------------------------------------------------ V rows past the sequence's end
-      if (cleans) {
-        const int j = j_end - j0, item = min(j + 2, nb) + j;  // in the producer's order
-        if (__all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->dirty, 0, abort, p.err))) {
-          zero_rows<KB>(smem + C::Q_BYTES + item % NSLOT * C::SLOT, HD / 128, k_len % KB, threadIdx.x - 64);
-          if (lane == 0) {
-            if (lead) sbd::mbar_arrive(&bars->clean);
-            else sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->clean), 0));
-          }
+      // asked once per tile, also where there is nothing to do: no wait here lasts longer than a tile
+      int it = 0, nq = 0;
+      Item w;
+      for (int n = 0; item_at(n, w); ++n) {
+        const Blocks blk = blocks_of<KB>(p, w.tl);
+        if (blk.nb == 0) continue;
+        if (!__all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->dirty, nq & 1, abort, p.err))) break;
+        if (blk.unclean >= 0) {
+          const int item = it + min(blk.unclean + 2, blk.nb) + blk.unclean;  // in the producer's order
+          zero_rows<KB>(smem + C::Q_BYTES + item % NSLOT * C::SLOT, HD / 128, blk.k_len % KB, threadIdx.x - 64);
         }
+        if (lane == 0) {
+          if (lead) sbd::mbar_arrive(&bars->clean);
+          else sbd::mbar_arrive_remote(sbd::mapa_shared(sbd::smem_u32(&bars->clean), 0));
+        }
+        it += 2 * blk.nb;
+        ++nq;
       }
     }
   } else {
@@ -541,7 +598,6 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
     // in the order of issue, and a commit counts every MMA before it: scores of block j in place say that P V of block
     // j - 2 is done, so its P buffer is free, and that no wait on pv_done is more than a phase behind.
     const int quad = warp & 3;
-    const Row r = row_of(p, tl, rank, quad * 32 + lane, k_len);
     const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t lead_bar = sbd::mapa_shared(sbd::smem_u32(bars), 0);
     // a warp's arrival on a barrier of the even CTA
@@ -553,28 +609,36 @@ __global__ void __launch_bounds__(256, PairCfg<HD>::CTAS)
       }
     };
     auto pv_complete = [&](int j) { return sbd::mbar_wait(&bars->pv_done[j & 1], (j >> 1) & 1, abort, p.err); };
-    float m = -INFINITY, l = 0.f;
+    int g = 0;  // blocks so far
     bool ok = true;
-    for (int j = 0; j < nb && ok; ++j) {
-      const int buf = j & 1, kb = (j0 + j) * KB;
-      ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->s_full[0], j & 1, abort, p.err));
+    Item w;
+    bool more = item_at(0, w);
+    for (int n = 1; ok && more; ++n) {
+      const Blocks blk = blocks_of<KB>(p, w.tl);
+      const Row r = row_of(p, w.tl, rank, quad * 32 + lane, blk.k_len);
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < blk.nb; ++j, ++g) {
+        const int kb = (blk.j0 + j) * KB;
+        ok = __all_sync(0xFFFFFFFFu, sbd::mbar_wait(&bars->s_full[0], g & 1, abort, p.err));
+        if (!ok) break;
+        sbd::tc_fence_after();
+        ok = softmax_block<T, HD, KB>(
+            tm + C::TM_S, tm + C::TM_P + (g & 1) * (KB / 2), tm, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m, l,
+            [&] {
+              sbd::tc_fence_before();
+              arrive(&bars->s_free);
+            },
+            [&] { return pv_complete(g - 1); });
+        if (!ok) break;
+        arrive(&bars->p_full[g & 1]);
+      }
+      const int64_t token = static_cast<int64_t>(w.tl.q0) + rank * p.tpt + r.tok;
+      T* dst = static_cast<T*>(p.out) + token * p.out_token + static_cast<int64_t>(w.kv * p.group + r.head) * p.out_head;
+      more = item_at(n, w);  // on its way while P V completes
+      if (ok && blk.nb > 0) ok = __all_sync(0xFFFFFFFFu, pv_complete(g - 1));
       if (!ok) break;
       sbd::tc_fence_after();
-      ok = softmax_block<T, HD, KB>(
-          tm + C::TM_S, tm + C::TM_P + buf * (KB / 2), tm, kb, r.lo, r.hi, kb + KB <= r.all_hi && kb >= r.all_lo, p.scale2, m, l,
-          [&] {
-            sbd::tc_fence_before();
-            arrive(&bars->s_free);
-          },
-          [&] { return pv_complete(j - 1); });
-      if (ok) arrive(&bars->p_full[buf]);
-    }
-    if (ok && nb > 0) ok = __all_sync(0xFFFFFFFFu, pv_complete(nb - 1));
-    if (ok) {
-      sbd::tc_fence_after();
-      const int64_t token = static_cast<int64_t>(tl.q0) + rank * p.tpt + r.tok;
-      T* dst = static_cast<T*>(p.out) + token * p.out_token + static_cast<int64_t>(kv * p.group + r.head) * p.out_head;
-      store_rows<T, HD>(tm, l, smem + quad * (32 * HD * 2), dst, r.ok && token >= 0 && token < p.t_q);
+      store_rows<T, HD>(tm, l, dst, r.ok && token >= 0 && token < p.t_q);
     }
   }
 
@@ -750,7 +814,7 @@ __global__ void __launch_bounds__(Cfg64::THREADS, 1)
       sbd::tc_fence_after();
       const int64_t token = static_cast<int64_t>(tl.q0) + i * p.tpt + r.tok;
       T* dst = static_cast<T*>(p.out) + token * p.out_token + static_cast<int64_t>(kv * p.group + r.head) * p.out_head;
-      store_rows<T, HD>(tm + i * HD, l, smem + i * C::Q_BYTES + quad * (32 * HD * 2), dst, r.ok && token >= 0 && token < p.t_q);
+      store_rows<T, HD>(tm + i * HD, l, dst, r.ok && token >= 0 && token < p.t_q);
     }
   }
 
@@ -826,7 +890,7 @@ int launch_pair(const void* q, const void* k, const void* v, const Strides& st, 
   if (!rc) rc = raise_smem(attn_packed_pair_kernel<T, HD>, C::SMEM, set);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * n_tiles * p.nkv);
+  cfg.gridDim = dim3(2 * std::min(n_tiles * p.nkv, sb::num_sms() / 2 * C::CTAS));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
@@ -919,7 +983,7 @@ extern "C" int sb_attn_prefill_packed(const void* q, int64_t q_token, int64_t q_
   PackedParams p{};
   p.out = out, p.out_token = out_token, p.out_head = out_head, p.tiles = reinterpret_cast<const Tile*>(tiles);
   p.err = sb::device_error_word();
-  p.t_q = t_q, p.t_k = t_k, p.nkv = n_kv_heads, p.group = n_heads / n_kv_heads, p.tpt = QR / p.group;
+  p.t_q = t_q, p.t_k = t_k, p.n_tiles = n_tiles, p.nkv = n_kv_heads, p.group = n_heads / n_kv_heads, p.tpt = QR / p.group;
   p.window = window, p.scale2 = scale * kLog2e;
   if (t_k == 0) k = v = q;  // nothing is read; the maps need an address
   const Strides st{q_token, q_head, k_token, k_head};
