@@ -214,6 +214,9 @@ __device__ __forceinline__ float2 exp2_fma(uint64_t y) {
                      __int_as_float(__float_as_int(v.y) + (__float_as_int(k.y) << 23)));
 }
 
+// n low bits set, none below 0 and all from 32 on
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u; }
+
 // One query row's part in a block: reads the scores (then `loaded()`), masks them (keys [lo, hi) of the sequence;
 // `whole`: all of them), raises the running maximum and rescales O where a score asks for it, once `pv_before()`
 // says that the P V of the block before is complete, writes P to `tp` and adds to the sum.  Warp-collective; false when a wait failed.
@@ -227,11 +230,12 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
   sbd::tmem_wait_ld();
   loaded();
   if (!whole) {
-    const int v0 = lo - kb, v1 = hi - kb;
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+      const uint32_t seen = low_bits(hi - kb - 32 * c) & ~low_bits(lo - kb - 32 * c);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) sv[c][e] = 32 * c + e >= v0 && 32 * c + e < v1 ? sv[c][e] : 0xFF800000u;  // -inf
+      for (int e = 0; e < 32; ++e) sv[c][e] = seen & (1u << e) ? sv[c][e] : 0xFF800000u;  // -inf
+    }
   }
   float mx[4];
 #pragma unroll
