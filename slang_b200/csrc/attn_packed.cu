@@ -374,8 +374,7 @@ __device__ __forceinline__ Row row_of(const PackedParams& p, const Tile& tl, int
 // and back over the plan (`units` of them do): the tiles come in falling order of their keys, so the sums are about the
 // same.  Each role walks the items by itself, so the loads and scores of one run ahead into the softmax and output of
 // the one before; the rings and the barriers' phases carry on.  Against a CTA or pair per item: 8 packed prompts of
-// 32 x 128 heads, 8003 tokens, take 113 us in place of 133; of 16 x 64 heads, 59 in
-// place of 66 (the launch included).
+// 32 x 128 heads, 8003 tokens, take 113 us in place of 133; of 16 x 64 heads, 59 in place of 66 (the launch included).
 struct Item {
   Tile tl;
   int kv;
