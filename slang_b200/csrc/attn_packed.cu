@@ -269,9 +269,9 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
   const uint64_t scale_2 = pack_f2(scale2, scale2), shift_2 = pack_f2(-mu, -mu);
   uint64_t sum[2] = {0, 0};  // pairs of zeros
   // POLY of 16 pairs of exponentials leave the special-function unit, 16 a cycle and SM, for the FMA pipe; not where
-  // a masked score has to give exactly 0.  At head_dim 64, bound by that unit, 8000 packed tokens of 16 heads take
-  // 86 us with 5 of 16, 93 with none and 90 with 8; at 128 and 256 none is best (125 us against 128 with 4, 8 packed
-  // prompts of 32 x 128): there the issue slots are the scarcer ones.
+  // a masked score has to give exactly 0.  At head_dim 64, bound by that unit, one prompt of 8000 tokens and 16 heads
+  // takes 242 us with 5 of 16, 247 with none and 258 with 9; at 128 and 256 none is best (6 prompts of 2000 tokens,
+  // 32 heads of 128: 277 to 279 us with 0, 1 or 2, 283 with 6): there the issue slots are the scarcer ones.
   auto exps = [&](auto poly) {
     constexpr int POLY = decltype(poly)::value;
 #pragma unroll
