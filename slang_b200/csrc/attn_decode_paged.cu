@@ -34,8 +34,11 @@
 namespace {
 
 constexpr int W = 4;  // warps per CTA
-constexpr int JOIN = 24;  // partials one CTA joins: more than the square root of the grid
-constexpr int MIN_KEYS = 64;  // of a CTA
+// Partials one CTA joins: more than the square root of the grid, so two levels suffice.  One sequence of 130001 keys
+// (8 heads of 256 over one): 34.1 us with 24, 34.9 with 32, 34.7 with 12.
+constexpr int JOIN = 24;
+// Keys that a CTA has at least.  One sequence of 1091 keys (17 CTAs of 64): 10.2 us, 10.5 with 128, the same with 32.
+constexpr int MIN_KEYS = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRise = 8.f;  // log2 units: p stays below 2^8
 
@@ -99,7 +102,7 @@ struct Shape {
   static constexpr int PART = HT * (HD + 2);       // a partial: O [HT][HD], m [HT], l [HT]
   static constexpr int HP = HD + 4;                // a head's row in shared memory: neighbouring heads in other banks
   static constexpr int SM_O = TEAMS * HT * HP;     // each team's O
-  static_assert(SM_O >= (2 * JOIN + 2) * HT, "the join's weights and sums lie there too");
+  static_assert(SM_O >= (JOIN + 2) * HT && JOIN <= 32 && HT % W == 0, "the join's weights lie there too; a lane per part");
   static constexpr int SM_F = SM_O + 2 * TEAMS * HT + (HS > 1 ? W * 32 * 4 * NS * NT : 0);
 };
 
@@ -413,8 +416,7 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
       };
       // joins the partials of n CTAs (at most JOIN), the i-th in slot(of(i)): into the output, or into the first one's slot
       auto join = [&](int n, auto of, bool final) {
-        float* wgt = sm_o;  // [n][HT] weights, then [HT] sums; the teams' O is no longer needed
-        float* ls = wgt + (JOIN + 2) * HT;
+        float* wgt = sm_o;  // [n][HT] weights, [HT] sums, [HT] maxima; the teams' O is no longer needed
         // Every thread has the loads of several parts of its vectors in flight at once, the first of them before the
         // weights are known.
         constexpr int VPT = HT * HD / 4 / (W * 32), UX = VPT >= 16 ? 2 : 32 / VPT > 8 ? 8 : 32 / VPT;
@@ -428,24 +430,25 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
           }
         };
         fetch(0);
-        for (int i = threadIdx.x; i < n * HT; i += W * 32) {
-          const float* src = slot(of(i / HT)) + HT * HD + i % HT;
-          wgt[i] = __ldcg(src);
-          ls[i] = __ldcg(src + HT);
-        }
-        __syncthreads();
-        if (threadIdx.x < HT) {  // rows of heads that are not there hold anything: no weight
-          const int h = threadIdx.x;
-          float M = -INFINITY, L = 0.f;
-          for (int i = 0; i < n; ++i) M = fmaxf(M, wgt[i * HT + h]);
-          const float mu = M == -INFINITY ? 0.f : M;
-          for (int i = 0; i < n; ++i) {
-            const float f = h < nheads ? ex2(wgt[i * HT + h] - mu) : 0.f;
-            wgt[i * HT + h] = f;
-            L += f * ls[i * HT + h];
-          }
-          wgt[n * HT + h] = L;
-          wgt[(n + 1) * HT + h] = M;
+        // a warp's heads, a lane per part; rows of heads that are not there hold anything: no weight
+        constexpr int HW = HT / W;
+        const int at = min(lane, n - 1);
+        const float* src = slot(of(at)) + HT * HD + warp * HW;
+        float pm[HW], pl[HW];
+#pragma unroll
+        for (int x = 0; x < HW; ++x) pm[x] = __ldcg(src + x), pl[x] = __ldcg(src + HT + x);
+#pragma unroll
+        for (int x = 0; x < HW; ++x) {
+          const int h = warp * HW + x;
+          float M = pm[x];
+#pragma unroll
+          for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+          const float f = h < nheads && lane < n ? ex2(pm[x] - (M == -INFINITY ? 0.f : M)) : 0.f;
+          float L = h < nheads && lane < n ? f * pl[x] : 0.f;
+#pragma unroll
+          for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, o);
+          if (lane < n) wgt[lane * HT + h] = f;
+          if (lane == 0) wgt[n * HT + h] = L, wgt[(n + 1) * HT + h] = M;
         }
         __syncthreads();
 #pragma unroll
