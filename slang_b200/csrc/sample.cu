@@ -84,10 +84,8 @@ struct Word {
 };
 
 struct Shared {
-  Word slot[2];        // this CTA's contribution, in turn
-  Word warp[NW];
-  Word all;
-  unsigned int lower;  // the count in CTAs of lower rank
+  Word slot[2][MAX_CS * NW];  // the words of all warps of the cluster, in turn
+  unsigned long long scan[NW];
   unsigned int n;      // entries of this CTA's list
   int bin;
   unsigned int hist[BINS];
@@ -134,39 +132,37 @@ __device__ __forceinline__ Word warp_join(Word w) {
   return r;
 }
 
-// Joins the words of all threads of the cluster (keys differ, or are ~0).  Two
-// slots in turn: a CTA writes one again only after a barrier that every other
-// CTA reaches once it has read it.
-__device__ Word reduce(Shared& sh, Word w, int cs, int& turn) {
+// Joins the words of all threads of the cluster (keys differ, or are ~0).  Each warp puts its word into every CTA's
+// shared memory and, after one barrier, joins what has arrived in its own.  Two buffers in turn: a word is replaced
+// only after a barrier that its readers reach once they have read it.  `lower`: the count in CTAs of lower rank.
+__device__ Word reduce(Shared& sh, Word w, int cs, int& turn, unsigned* lower = nullptr) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = cs > 1 ? static_cast<int>(sbd::cluster_ctarank()) : 0;
+  Word* slot = sh.slot[turn];
+  turn ^= 1;
   w = warp_join(w);
-  if (lane == 0) sh.warp[warp] = w;
-  __syncthreads();
-  if (warp == 0) {
-    w = warp_join(lane < NW ? sh.warp[lane] : Word{0, ~0ull, 0, 0});
-    if (lane == 0) {
-      (cs > 1 ? sh.slot[turn] : sh.all) = w;
-      sh.lower = 0;
-    }
-  }
   if (cs > 1) {
-    sbd::cluster_sync_all();
-    if (warp == 0) {
-      w = Word{0, ~0ull, 0, 0};
-      if (lane < cs) {
-        const uint32_t a = sbd::mapa_shared(sbd::smem_u32(&sh.slot[turn]), lane);
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(w.sum) : "r"(a) : "memory");
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(w.key) : "r"(a + 8) : "memory");
-        asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(w.aux), "=r"(w.count) : "r"(a + 16) : "memory");
-      }
-      const unsigned lower = __reduce_add_sync(0xFFFFFFFFu, lane < static_cast<int>(sbd::cluster_ctarank()) ? w.count : 0u);
-      w = warp_join(w);
-      if (lane == 0) sh.all = w, sh.lower = lower;
+    if (lane < cs) {
+      const uint32_t a = sbd::mapa_shared(sbd::smem_u32(slot + rank * NW + warp), lane);
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(w.sum) : "memory");
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a + 8), "l"(w.key) : "memory");
+      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(a + 16), "r"(w.aux), "r"(w.count) : "memory");
     }
-    turn ^= 1;
+    sbd::cluster_sync_all();
+  } else {
+    if (lane == 0) slot[warp] = w;
+    __syncthreads();
   }
-  __syncthreads();
-  return sh.all;
+  w = Word{0, ~0ull, 0, 0};
+  unsigned below = 0;
+  for (int i = lane; i < cs * NW; i += 32) {
+    const Word o = slot[i];
+    w.sum += o.sum, w.count += o.count;
+    if (o.key < w.key) w.key = o.key, w.aux = o.aux;
+    below += i < rank * NW ? o.count : 0;
+  }
+  if (lower) *lower = __reduce_add_sync(0xFFFFFFFFu, below);
+  return warp_join(w);
 }
 
 template <typename T>
@@ -179,6 +175,7 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
   float2* seg_mass = reinterpret_cast<float2*>(lane_max + rounds * NW * 32);
   auto seg_of = [&](int round) { return (round * cs + rank) * NW + warp; };
   sbd::griddep_launch_dependents();
+  if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   if (threadIdx.x < BINS) sh.hist[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.n = 0;
   sbd::griddep_wait();
@@ -265,13 +262,13 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
   }
   Word w0{0, ~0ull, 0, 0};
   if (widx != ~0u && wmax > -INFINITY) w0.key = static_cast<unsigned long long>(~order_of(wmax)) << 32 | widx, w0.aux = __float_as_uint(wmax);
+  if (cs > 1) asm volatile("barrier.cluster.wait;" ::: "memory");  // the CTAs whose memory takes the words have started
   w0 = reduce(sh, w0, cs, turn);
   int token = static_cast<int>(w0.key & 0xFFFFFFFFu);  // -1 when no value is above -inf
   const float mx = __uint_as_float(w0.aux);
   if (w0.key == ~0ull || greedy) {
     if (rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
-    if (cs > 1) sbd::cluster_sync_all();  // no CTA leaves while another may read its slot
-    return;
+    return;  // what other CTAs write here has arrived
   }
   // log2 of w; fminf gives the maximum itself 0 even where it is infinite (inf - inf)
   auto z2_of = [&](float x) { return fminf((x - mx) * inv, 0.f); };
@@ -362,11 +359,11 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
       const unsigned long long c = __shfl_up_sync(0xFFFFFFFFu, v, o);
       if (lane >= o) v += c;
     }
-    if (lane == 31) sh.warp[warp].sum = v;
+    if (lane == 31) sh.scan[warp] = v;
     __syncthreads();
     *whole = 0;
     for (int w = 0; w < NW; ++w) {
-      const unsigned long long c = sh.warp[w].sum;
+      const unsigned long long c = sh.scan[w];
       v += w < warp ? c : 0;
       *whole += c;
     }
@@ -399,9 +396,9 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
     const int bin = sh.bin;
     collect(bin == BINS - 1 ? -kLargest : floor_of(-0.125f * (bin + 1)));
     const unsigned mine = sh.n;
-    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : min(mine, SORT + 1u)}, cs, turn).count;
+    unsigned at;
+    const unsigned total = reduce(sh, Word{0, ~0ull, 0, threadIdx.x ? 0u : min(mine, SORT + 1u)}, cs, turn, &at).count;
     if (total <= SORT) {
-      const unsigned at = sh.lower;
       if (cs > 1) {
         const uint32_t dst = sbd::mapa_shared(sbd::smem_u32(sh.keys), 0);
         for (unsigned i = threadIdx.x; i < mine; i += NT)
@@ -558,7 +555,6 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
     token = static_cast<int>(w.key & 0xFFFFFFFFu);
   }
   if (rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
-  if (cs > 1) sbd::cluster_sync_all();  // no CTA leaves while another may read its slot
 }
 
 template <typename T>
