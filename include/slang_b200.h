@@ -647,7 +647,9 @@ size_t sb_attn_decode_paged_workspace_size(const sb_paged_kv* kv, int n_heads, i
  * {64, 128, 256}, any number of query heads per kv head up to 128.  q [t_q][n_heads],
  * k and v [t_k][n_kv_heads] and out [t_q][n_heads] rows of head_dim lie *_token and
  * *_head elements apart (multiples of 8, k and v alike).  What lies in rows of
- * other sequences, NaN included, changes nothing.
+ * other sequences, NaN included, changes nothing; a NaN or infinity in a value row
+ * of the sequence itself may also reach queries before it (0 times it, in a block of
+ * up to 128 keys), one in a key row does not.
  * tiles: device copy of what sb_attn_packed_plan wrote for the same lengths, head
  * counts and head_dim (host arrays; tiles NULL: the count alone; kv_lens NULL: as
  * q_lens; 8 int32 per tile; `window` only orders them, longest first).  A plan

@@ -27,6 +27,12 @@
 // p = 2^(s - m) is rounded to the cache's type for the second product (its
 // relative error is that of the output's own rounding); m, l, S and O are f32.
 // m only rises when a score passes it by 2^8, so O is rarely rescaled.
+//
+// Measured: 96 sequences of 4096 keys on average (ragged, 32 heads of 128 over 8, bf16)
+// 270 us (1.61 GB, 6.0 TB/s, 0.93 of a copy's rate); one sequence of 130001 keys (8 heads
+// of 256 over one) 34 us, 21 of them its bytes: about 5 until the first keys arrive
+// (positions, page table, keys: each needs the one before), 2 to 3 for two
+// joins, 2 for the launch.  One sequence of 1091 keys 10.2 us: the same latencies.
 #include <algorithm>
 
 #include "paged.cuh"

@@ -10,7 +10,9 @@
 // rotation pairs, v and v + r / 8 (past the rotated part any two), so a pair
 // shares its angles, nothing is exchanged between lanes but the norm's sum, and
 // every load and store is a full vector whatever rot is.  A head takes
-// head_dim / 16 lanes, a warp holds 512 / head_dim heads.
+// head_dim / 16 lanes, a warp holds 512 / head_dim heads.  Measured: 16133 packed
+// tokens of 48 x 128 bf16 values 74 to 78 us (397 MB, 5.1 to 5.4 TB/s, 0.80 to 0.84 of
+// a copy's rate); in a graph one token 2.2 us, 256 tokens 3.1 us.
 #include "paged.cuh"
 
 namespace {

@@ -34,6 +34,14 @@
 //                 k tokens) is sorted by one CTA, which finishes the row alone.
 // Masses are added as integers, those of a segment in one order, so neither the
 // order of arrival nor the number of CTAs shows in the result.
+//
+// One row of 262144 f32 logits with top-p takes 11.5 us: 2.2 for the pass, 2.8
+// for the random words on the row's 16 SMs, the rest three joins of its CTAs.  128
+// such rows with mixed settings take 66 us (2.0 TB/s): greedy rows alone 24 (5.5
+// TB/s), min-p 34, top-k 58, no filter 59, top-p 100.  The random words bound the
+// last two: twenty 32 x 32 -> 64 products per four tokens, 16 a cycle and SM, are
+// 37 us for 33.5 million tokens.  (High words through f64 multiply-adds rounded
+// down are exact too and took 64 in place of 59.)
 #include <algorithm>
 
 #include "paged.cuh"
@@ -609,8 +617,8 @@ extern "C" int sb_sample(const void* logits, int dtype, int64_t ld, int rows, in
   p.vec = sb::aligned(logits, 4 * size) && (rows == 1 || ld % 4 == 0);
   p.segs = (vocab + SEG - 1) / SEG;
   p.softcap = softcap;
-  // CTAs per row: as many as make about seven per SM in all, while each warp has a segment.  128 rows of 262144
-  // with mixed settings: 8 per row
+  // CTAs per row: as many as make about seven per SM in all, while each warp has a segment.  128 rows of 262144 with
+  // mixed settings: 66 us with 8 per row (two waves, whose phases overlap), 117 with 4, 80 with 16
   int cs = 1;
   while (cs < MAX_CS && p.segs >= cs * 2 * NW && static_cast<int64_t>(rows) * cs * 2 <= 7 * sb::num_sms()) cs *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
