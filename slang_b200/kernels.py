@@ -679,13 +679,13 @@ def kv_append_paged(qkv: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     if src is None:
         raise TypeError(f"qkv has dtype {qkv.dtype}, expected f16, bf16 or f32")
     width = (n_heads + 2 * nkv) * hd
-    if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or gpu != cache.gpu:
+    shape, step, tab, angles = qkv.shape, qkv.stride(), page_table.shape, cos.shape
+    if len(shape) != 2 or shape[1] != width or step[1] != 1 or gpu != cache.gpu:
         raise ValueError(f"qkv must be [t, {width}] rows with unit column stride on {cache.device}")
-    t = qkv.shape[0]
-    if page_table.dtype is not _I32 or page_table.dim() != 2 or not page_table.is_contiguous() or \
-            page_table.get_device() != gpu:
+    t = shape[0]
+    if page_table.dtype is not _I32 or len(tab) != 2 or not page_table.is_contiguous() or page_table.get_device() != gpu:
         _refuse(page_table, "page_table", _I32, ("n_seqs", "max_pages"), gpu)
-    if cos.dim() != 2 or cos.shape != sin.shape:
+    if len(angles) != 2 or angles != sin.shape:
         raise ValueError("cos and sin must be [max_pos, rot / 2]")
     if cos.dtype is not _F32T or not cos.is_contiguous() or cos.get_device() != gpu:
         _refuse(cos, "cos", _F32T, cos.shape, gpu)
@@ -701,12 +701,12 @@ def kv_append_paged(qkv: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
             if o is not None and (o.dtype is not cache.dtype or o.shape != (t, nkv, hd) or not o.is_contiguous() or
                                   o.get_device() != gpu):
                 raise ValueError(f"{name} must be a contiguous [{t}, {nkv}, {hd}] tensor of the cache's type")
-    max_pos, half = cos.shape
-    _lib.call("sb_kv_append_paged", cache.ptr, page_table.data_ptr(), *page_table.shape, qkv.data_ptr(), src,
-              qkv.stride(0) if t > 1 else width, t, n_heads, _vec(seq, "seq", _I32, t, gpu),
-              _vec(pos, "pos", _I32, t, gpu), _vec(q_norm, "q_norm", _F32T, hd, gpu),
-              _vec(k_norm, "k_norm", _F32T, hd, gpu), v_norm, eps, cos.data_ptr(), sin.data_ptr(), 2 * half, max_pos,
-              q_out.data_ptr(), _ptr(k_out), _ptr(v_out), _raw_stream(gpu))
+    _lib.call("sb_kv_append_paged", cache.ptr, page_table.data_ptr(), tab[0], tab[1], qkv.data_ptr(), src,
+              step[0] if t > 1 else width, t, n_heads, None if seq is None else _vec(seq, "seq", _I32, t, gpu),
+              _vec(pos, "pos", _I32, t, gpu), None if q_norm is None else _vec(q_norm, "q_norm", _F32T, hd, gpu),
+              None if k_norm is None else _vec(k_norm, "k_norm", _F32T, hd, gpu), v_norm, eps, cos.data_ptr(),
+              sin.data_ptr(), 2 * angles[1], angles[0], q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
+              None if v_out is None else v_out.data_ptr(), _raw_stream(gpu))
     return q_out
 
 
@@ -729,25 +729,26 @@ def attn_decode_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     gpu = _gpu(q, "q")
     if q.dtype is not cache.dtype:
         raise TypeError(f"q has dtype {q.dtype}, expected the cache's {cache.dtype}")
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or gpu != cache.gpu:
+    shape, tab = q.shape, page_table.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or gpu != cache.gpu:
         raise ValueError(f"q must be [b, n_heads, {cache.head_dim}] on {cache.device}")
-    b, nh, hd = q.shape
+    b, nh, hd = shape
     dense = q.is_contiguous()
     if not dense and (q.stride(2) != 1 or (nh > 1 and q.stride(1) != hd)):
         raise ValueError("each sequence's heads of q must be contiguous")
-    if page_table.dtype is not _I32 or page_table.dim() != 2 or page_table.shape[0] != b or \
-            not page_table.is_contiguous() or page_table.get_device() != gpu:
+    if page_table.dtype is not _I32 or len(tab) != 2 or tab[0] != b or not page_table.is_contiguous() or \
+            page_table.get_device() != gpu:
         _refuse(page_table, "page_table", _I32, (b, "max_pages"), gpu)
     if out is None:
         out = torch.empty_like(q) if dense else torch.empty((b, nh, hd), dtype=q.dtype, device=q.device)
-    elif out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != gpu:
+    elif out.dtype is not q.dtype or out.shape != shape or not out.is_contiguous() or out.get_device() != gpu:
         raise ValueError("out must be contiguous and match q")
     if workspace is None:
         workspace = attn_decode_paged_workspace(cache, nh, b)
     elif not workspace.is_contiguous() or workspace.get_device() != gpu:
         raise ValueError(f"workspace must be a contiguous tensor on cuda:{gpu}")
-    _lib.call("sb_attn_decode_paged", cache.ptr, page_table.data_ptr(), page_table.shape[1],
-              _vec(pos, "pos", _I32, b, gpu), b, q.data_ptr(), q.stride(0) if b > 1 else nh * hd, nh, window, scale,
+    _lib.call("sb_attn_decode_paged", cache.ptr, page_table.data_ptr(), tab[1], _vec(pos, "pos", _I32, b, gpu), b,
+              q.data_ptr(), q.stride(0) if b > 1 else nh * hd, nh, window, scale,
               out.data_ptr(), workspace.data_ptr(), workspace.nbytes, _raw_stream(gpu))
     return out
 
