@@ -44,7 +44,7 @@
 // tensor-bound at 256, even at 128, bound by the exponentials at 64.  Measured:
 //   256  one prompt of 15001 tokens, 8 heads over one: 2570 cycles per block of 128
 //        keys (2048 of MMA), 617 to 635 us = 1.45 to 1.49 PFLOP/s (0.88 to 0.90 of
-//        the cuBLAS rate) in a single call, 732 us in a row of them, when the power
+//        the cuBLAS rate) in a single call, 732 to 754 us in a row of them, when the power
 //        limit takes the clock to 1.6 GHz and below.
 //   128  8 prompts, 8003 tokens, 32 heads over 8: 1710 cycles per block of 64 keys with
 //        two CTAs on an SM (512 each of MMA, 512 each of exponentials): 860 in the
