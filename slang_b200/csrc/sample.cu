@@ -37,11 +37,11 @@
 //
 // One row of 262144 f32 logits with top-p takes 11.5 us: 2.2 for the pass, 2.8
 // for the random words on the row's 16 SMs, the rest three joins of its CTAs.  128
-// such rows with mixed settings take 66 us (2.0 TB/s): greedy rows alone 24 (5.5
-// TB/s), min-p 34, top-k 58, no filter 59, top-p 100.  The random words bound the
+// such rows with mixed settings take 64 us (2.1 TB/s): greedy rows alone 26 (5.1
+// TB/s), min-p 36, top-k 61, no filter 63, top-p 110.  The random words bound the
 // last two: twenty 32 x 32 -> 64 products per four tokens, 16 a cycle and SM, are
 // 37 us for 33.5 million tokens.  (High words through f64 multiply-adds rounded
-// down are exact too and took 64 in place of 59.)
+// down are exact too and took 64 in place of 59 without a filter.)
 #include <algorithm>
 
 #include "paged.cuh"
@@ -65,6 +65,7 @@ struct SampleParams {
   int64_t ld;
   int v, segs;   // segs: segments of a row
   int vec;       // rows start on a 4-value boundary
+  int sorted;    // the costly rows first
   float softcap; // 0: off
   const int64_t* seeds;
   const int32_t* pos;
@@ -98,7 +99,7 @@ struct Shared {
   int bin;
   unsigned int hist[BINS];
   unsigned long long list[SORT];  // candidates here: (inverted ranking bits, index), smaller ranks before
-  unsigned long long keys[SORT];  // a top-k row's, in the CTA of rank 0
+  alignas(16) unsigned long long keys[SORT];  // a top-k row's, in the CTA of rank 0
 };
 
 // Philox4x32-10 under one key: the keys of its ten rounds are kept, a call is
@@ -173,11 +174,48 @@ __device__ Word reduce(Shared& sh, Word w, int cs, int& turn, unsigned* lower = 
   return warp_join(w);
 }
 
+// The row of this cluster when the rows are more than one wave of CTAs: within NT neighbours those that take longest
+// come first (top-p without top-k, no filter, top-k, min-p, greedy; stable), so that the last ones to start are short.
+// 128 rows of 262144 with mixed settings: 64 us in place of 78; rows all of one kind pay 2 us, of 24 (greedy) to 105.
+__device__ __forceinline__ int sorted_row(const SampleParams& p, Shared& sh) {
+  constexpr int KINDS = 6;  // the last: past the last row
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = static_cast<int>(blockIdx.y) / NT * NT, r = first + threadIdx.x;
+  int kind = KINDS - 1;
+  if (r < static_cast<int>(gridDim.y)) {
+    const float temp = p.temperature ? p.temperature[r] : 1.f, top_p = p.top_p ? p.top_p[r] : 1.f;
+    const float min_p = p.min_p ? p.min_p[r] : 0.f;
+    const int top_k = p.top_k ? p.top_k[r] : 0;
+    if (!(temp > 0.f) || top_p <= 0.f || top_k == 1) kind = 4;
+    else if (top_k > 0) kind = 2;
+    else if (min_p > 0.f) kind = 3;
+    else kind = top_p < 1.f ? 0 : 1;
+  }
+  unsigned* count = reinterpret_cast<unsigned*>(sh.keys);  // [KINDS][NW]
+  unsigned before = 0;
+#pragma unroll
+  for (int k = 0; k < KINDS; ++k) {
+    const unsigned m = __ballot_sync(0xFFFFFFFFu, kind == k);
+    if (lane == 0) count[k * NW + warp] = __popc(m);
+    if (kind == k) before = __popc(m & ((1u << lane) - 1u));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < KINDS * NW; i += 4) {
+    const uint4 c = *reinterpret_cast<const uint4*>(count + i);
+    const int n = kind * NW + warp - i;  // the counts before this warp's of its kind
+    before += (n > 0 ? c.x : 0) + (n > 1 ? c.y : 0) + (n > 2 ? c.z : 0) + (n > 3 ? c.w : 0);
+  }
+  if (before == blockIdx.y - first) sh.bin = r;
+  __syncthreads();
+  return sh.bin;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) float lane_max[];  // [local segment][lane], then [local segment] {largest, mass}
   __shared__ Shared sh;
-  const int cs = gridDim.x, rank = blockIdx.x, row = blockIdx.y;  // a cluster spans the x axis
+  const int cs = gridDim.x, rank = blockIdx.x;  // a cluster spans the x axis
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rounds = (p.segs + cs * NW - 1) / (cs * NW);  // segments per warp; local segment l = round * NW + warp
   float2* seg_mass = reinterpret_cast<float2*>(lane_max + rounds * NW * 32);
@@ -187,6 +225,7 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
   if (threadIdx.x < BINS) sh.hist[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.n = 0;
   sbd::griddep_wait();
+  const int row = p.sorted ? sorted_row(p, sh) : blockIdx.y;
   const float temp = p.temperature ? p.temperature[row] : 1.f;
   const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
   const int top_k = p.top_k ? p.top_k[row] : 0;
@@ -621,6 +660,7 @@ extern "C" int sb_sample(const void* logits, int dtype, int64_t ld, int rows, in
   // mixed settings: 66 us with 8 per row (two waves, whose phases overlap), 117 with 4, 80 with 16
   int cs = 1;
   while (cs < MAX_CS && p.segs >= cs * 2 * NW && static_cast<int64_t>(rows) * cs * 2 <= 7 * sb::num_sms()) cs *= 2;
+  p.sorted = static_cast<int64_t>(rows) * cs > CTAS * sb::num_sms() && (temperature || top_k || top_p || min_p);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == SB_F32) return launch_sample<float>(p, rows, cs, s);
   if (dtype == SB_F16) return launch_sample<__half>(p, rows, cs, s);

@@ -166,6 +166,24 @@ def test_sample_distribution(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(700, 1500), (150, 70001)])
+def test_sample_many_rows_of_all_kinds(cuda, rows, vocab):
+    """More rows than run at once, which are served in another order: each draws what it draws alone."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    logits = 3 * torch.randn(rows, vocab, generator=g, device="cuda")
+    kind = torch.arange(rows, device="cuda") % 7
+    one = torch.ones(rows, device="cuda")
+    args = dict(temperature=torch.where(kind == 0, 0 * one, 0.7 * one), top_p=torch.where(kind % 3 == 1, 0.8 * one, one),
+                min_p=torch.where(kind == 3, 0.05 * one, 0 * one), top_k=torch.where(kind >= 5, 20 * kind, 0 * kind).int())
+    seeds = torch.arange(rows, device="cuda") * 977 + 5
+    pos = torch.arange(rows, device="cuda", dtype=torch.int32)
+    got = kern.sample(logits, seeds, pos, **args)
+    for r in range(rows):
+        alone = kern.sample(logits[r:r + 1], seeds[r:r + 1], pos[r:r + 1], **{k: v[r:r + 1] for k, v in args.items()})
+        assert int(alone) == int(got[r]), r
+
+
+@pytest.mark.gpu
 def test_sample_strides(cuda):
     """Rows that start off a vector boundary, on another stream."""
     x, seeds, pos, u = _inputs(6, 5001, torch.float16, 1, cuda)
