@@ -787,25 +787,26 @@ def attn_prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan:
     if dtype is None or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError("q, k and v must all be f16 or all be bf16")
     nh, nkv, hd = plan.n_heads, plan.n_kv_heads, plan.head_dim
-    if q.shape != (plan.total_q, nh, hd) or q.stride(2) != 1:
+    q_shape, q_step, k_shape, k_step = q.shape, q.stride(), k.shape, k.stride()
+    if q_shape != (plan.total_q, nh, hd) or q_step[2] != 1:
         raise ValueError(f"q must be [{plan.total_q}, {nh}, {hd}] with unit stride in head_dim")
-    if k.shape != (plan.total_k, nkv, hd) or v.shape != k.shape or k.stride() != v.stride() or k.stride(2) != 1:
+    if k_shape != (plan.total_k, nkv, hd) or v.shape != k_shape or k_step != v.stride() or k_step[2] != 1:
         raise ValueError(f"k and v must be [{plan.total_k}, {nkv}, {hd}] with the same strides, unit in head_dim")
     if k.get_device() != gpu or v.get_device() != gpu or plan.gpu != gpu:
         raise ValueError(f"k, v and the plan must be on cuda:{gpu}")
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((plan.total_q, nh, hd))
-    elif out.dtype is not q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.get_device() != gpu:
+    elif out.dtype is not q.dtype or out.shape != q_shape or out.stride(2) != 1 or out.get_device() != gpu:
         raise ValueError("out must match q, with unit stride in head_dim")
-    _lib.call("sb_attn_prefill_packed", q.data_ptr(), _step(q, 0), _step(q, 1), k.data_ptr(), v.data_ptr(), _step(k, 0),
-              _step(k, 1), out.data_ptr(), _step(out, 0), _step(out, 1), dtype, plan.total_q, plan.total_k, nh, nkv, hd,
-              plan.window, scale, plan.tiles.data_ptr(), plan.n_tiles, _raw_stream(gpu))
+    _lib.call("sb_attn_prefill_packed", q.data_ptr(), *_steps(q_shape, q_step), k.data_ptr(), v.data_ptr(),
+              *_steps(k_shape, k_step), out.data_ptr(), *_steps(q_shape, out.stride()), dtype, q_shape[0], k_shape[0], nh,
+              nkv, hd, plan.window, scale, plan.tiles.data_ptr(), plan.n_tiles, _raw_stream(gpu))
     return out
 
 
-def _step(t: torch.Tensor, dim: int) -> int:
-    """Stride of a dimension; that of a dimension of one says nothing, so the rows' own width stands in."""
-    return t.stride(dim) if t.shape[dim] > 1 else t.shape[2]
+def _steps(shape, step) -> tuple[int, int]:
+    """Strides of tokens and heads; that of a dimension of one says nothing, so the rows' own width stands in."""
+    return step[0] if shape[0] > 1 else shape[2], step[1] if shape[1] > 1 else shape[2]
 
 
 def sample(logits: torch.Tensor, seeds: torch.Tensor, pos: torch.Tensor, temperature: torch.Tensor | None = None,
@@ -821,12 +822,13 @@ def sample(logits: torch.Tensor, seeds: torch.Tensor, pos: torch.Tensor, tempera
     dtype = _DT_ALL.get(logits.dtype)
     if dtype is None:
         raise TypeError(f"logits has dtype {logits.dtype}, expected f16, bf16 or f32")
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    shape, step = logits.shape, logits.stride()
+    if len(shape) != 2 or (step[1] != 1 and shape[1] > 1):
         raise ValueError("logits must be [rows, vocab] with unit column stride")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     if tokens is None:
         tokens = _empty(rows, dtype=_I32, device=logits.device)
-    _lib.call("sb_sample", logits.data_ptr(), dtype, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+    _lib.call("sb_sample", logits.data_ptr(), dtype, step[0] if rows > 1 else vocab, rows, vocab,
               _vec(seeds, "seeds", _I64, rows, gpu), _vec(pos, "pos", _I32, rows, gpu),
               _vec(temperature, "temperature", _F32T, rows, gpu), _vec(top_k, "top_k", _I32, rows, gpu),
               _vec(top_p, "top_p", _F32T, rows, gpu), _vec(min_p, "min_p", _F32T, rows, gpu), softcap,
