@@ -629,9 +629,10 @@ int sb_kv_append_paged(const sb_paged_kv* kv, const int32_t* page_table, int n_s
  * (pos[i] < 0) gives zeros.  q [b] rows of [n_heads][head_dim] q_stride elements
  * apart and out [b][n_heads][head_dim] are of the cache's type.
  * workspace: device, 16-byte aligned, at least
- * sb_attn_decode_paged_workspace_size bytes, zero before the first call; each
- * call leaves it ready for the next, of the same or of smaller shape.  Calls that may
- * overlap on the GPU need their own.
+ * sb_attn_decode_paged_workspace_size bytes (the same for every b >= 1), zero before
+ * the first call; each call leaves it ready for the next, of any batch, head counts
+ * and head_dim that it is large enough for.  Calls that may overlap on the GPU need
+ * their own.
  */
 int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_table, int max_pages, const int32_t* pos, int b,
                          const void* q, int64_t q_stride, int n_heads, int window, float scale, void* out,

@@ -79,8 +79,8 @@ struct DecodeParams {
   sbp::Pages pages;
   const int32_t* pos;
   unsigned int* group_count;  // [grid / JOIN + 1][2], zero between calls
-  unsigned int* count;        // [b * nkv * htiles], zero between calls
-  float* part;          // [grid][2][HT * (hd + 2)]
+  unsigned int* count;        // [grid], of the split segment that starts in that CTA; zero between calls
+  float* part;                // [grid][2][HT * (hd + 2)]
   int b, nkv, group, htiles, window;  // htiles: tiles of HT query heads per kv head
   float scale2;                       // scale * log2(e)
 };
@@ -126,14 +126,13 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
   __shared__ int sh_scan[W], sh_first[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int team = warp / HS, half = warp % HS;
-  const int heads_per_seq = p.nkv * p.htiles;
   sbd::griddep_launch_dependents();
   sbd::griddep_wait();
 
   // total blocks of all sequences, this CTA's run of them [r0, r1) and the sequence that holds r0: each
   // thread counts a few neighbouring sequences, whose loads are one latency (blocks of 16 keys or more of
   // a cache that fits a GPU number far below 2^31)
-  auto blocks_of = [&](int lo, int hi) { return (hi - lo + KB - 1) / KB * heads_per_seq; };
+  auto blocks_of = [&](int lo, int hi) { return (hi - lo + KB - 1) / KB * (p.nkv * p.htiles); };
   const int per = (p.b + W * 32 - 1) / (W * 32), b0 = threadIdx.x * per, b1 = min(b0 + per, p.b);
   int own = 0;
 #pragma unroll 4
@@ -182,8 +181,8 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
 
   for (int r = r0; r < r1;) {
     const int nblk = (hi - lo + KB - 1) / KB;
-    if (r >= seq_start + nblk * heads_per_seq) {
-      seq_start += nblk * heads_per_seq;
+    if (r >= seq_start + nblk * (p.nkv * p.htiles)) {
+      seq_start += nblk * (p.nkv * p.htiles);
       key_range(p, ++b, &lo, &hi);
       continue;
     }
@@ -486,7 +485,7 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
           }
         }
       };
-      unsigned int* cnt = p.count + static_cast<int64_t>(b) * heads_per_seq + hidx;
+      unsigned int* cnt = p.count + c0;  // only the last segment that starts in a CTA reaches past it
       if (c1 - c0 < JOIN) {
         if (last_of(cnt, c1 - c0 + 1)) join(c1 - c0 + 1, [&](int i) { return c0 + i; }, true);
       } else {
@@ -517,13 +516,11 @@ int head_tile(int group) { return group <= 8 ? 8 : 16; }
 // CTAs of one resident wave.
 int grid_of() { return 2 * sb::num_sms(); }
 
-// The workspace: counters of the groups and of the segments, then the partials.
+// The workspace: counters of the groups and of the CTAs, then the partials.  Where each lies and how many counters
+// there are depends on the GPU alone, so calls of any batch, head counts and head_dim follow each other on one
+// workspace that is large enough for them: none writes a partial over another's counters.
 size_t group_bytes(int grid) { return (static_cast<size_t>(grid) / JOIN + 1) * 8; }
-size_t counter_bytes(const sb_paged_kv* kv, int n_heads, int b) {
-  const int group = n_heads / kv->n_kv_heads, ht = head_tile(group);
-  const size_t n = static_cast<size_t>(b) * kv->n_kv_heads * ((group + ht - 1) / ht);
-  return (group_bytes(grid_of()) + n * 4 + 255) / 256 * 256;
-}
+size_t counter_bytes(int grid) { return (group_bytes(grid) + static_cast<size_t>(grid) * 4 + 255) / 256 * 256; }
 
 template <typename T, int HD, int HS, int NT>
 int launch_decode(const DecodeParams& p, int grid, cudaStream_t stream) {
@@ -556,8 +553,8 @@ int launch_decode_hd(int hd, int ht, const DecodeParams& p, int grid, cudaStream
 
 extern "C" size_t sb_attn_decode_paged_workspace_size(const sb_paged_kv* kv, int n_heads, int b) {
   if (!kv || kv->n_kv_heads < 1 || n_heads < 1 || n_heads % kv->n_kv_heads || b < 1) return 0;
-  const int ht = head_tile(n_heads / kv->n_kv_heads);
-  return counter_bytes(kv, n_heads, b) + static_cast<size_t>(grid_of()) * 2 * ht * (kv->head_dim + 2) * sizeof(float);
+  const int ht = head_tile(n_heads / kv->n_kv_heads), grid = grid_of();
+  return counter_bytes(grid) + static_cast<size_t>(grid) * 2 * ht * (kv->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_table, int max_pages, const int32_t* pos,
@@ -582,7 +579,7 @@ extern "C" int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_t
   const int grid = grid_of();
   p.group_count = static_cast<unsigned int*>(workspace);
   p.count = p.group_count + group_bytes(grid) / 4;
-  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + counter_bytes(kv, n_heads, b));
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + counter_bytes(grid));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return kv->dtype == SB_F16 ? launch_decode_hd<__half>(kv->head_dim, ht, p, grid, s)
                              : launch_decode_hd<__nv_bfloat16>(kv->head_dim, ht, p, grid, s);

@@ -711,8 +711,9 @@ def kv_append_paged(qkv: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
 
 
 def attn_decode_paged_workspace(cache: PagedKV, n_heads: int, batch: int) -> torch.Tensor:
-    """A zeroed workspace for :func:`attn_decode_paged` calls of up to ``batch`` sequences
-    that run one after another; calls that may overlap on the GPU need their own."""
+    """A zeroed workspace for :func:`attn_decode_paged` calls that run one after another, of up to
+    ``batch`` sequences in any order (and for caches of other shapes whose own workspace is
+    no larger); calls that may overlap on the GPU need their own."""
     n = int(_lib.load().sb_attn_decode_paged_workspace_size(cache.ptr, n_heads, batch))
     return torch.zeros(max(n, 16), dtype=torch.uint8, device=cache.device)
 
