@@ -43,6 +43,22 @@ class PagedRunner:
         self.H, self.nh, self.eps, self.vocab = cfg["hidden"], cfg["n_heads"], float(cfg["eps"]), cfg["vocab"]
         self.softcap = float(cfg.get("softcap") or 0.0)
         dev = dm.device
+        # all work runs on a stream of the runner's own, and so do the fills of its buffers; what the
+        # caller's stream still has to do (the model's weights) comes before
+        self.stream = torch.cuda.Stream(device=dev)
+        with self._own_stream():
+            self._allocate(specs, batch, n_pages, page_size)
+        self.free = list(range(n_pages))
+        self.lens, self.room = [0] * batch, [0] * batch
+        self.graph = None
+
+    def _own_stream(self):
+        """The runner's stream as the current one, behind all that the caller's stream has been given so far."""
+        self.stream.wait_stream(torch.cuda.current_stream(self.dm.device))
+        return torch.cuda.stream(self.stream)
+
+    def _allocate(self, specs, batch: int, n_pages: int, page_size: int) -> None:
+        dm, dev = self.dm, self.dm.device
         self.caches = []
         for sp in specs:  # a KV-shared layer holds its source layer's cache
             self.caches.append(kern.PagedKV.allocate(n_pages, page_size, 1, sp["hd"], torch.float16, dev)
@@ -54,20 +70,18 @@ class PagedRunner:
         self.temperature = torch.zeros(batch, device=dev)
         self.top_k, self.top_p, self.min_p = i32(batch), torch.ones(batch, device=dev), torch.zeros(batch, device=dev)
         self.seeds = torch.zeros(batch, dtype=torch.int64, device=dev)
-        self.free = list(range(n_pages))
-        self.lens, self.room = [0] * batch, [0] * batch
         # one workspace per shape of attention: the calls follow each other on one stream
         self.attn_ws = {sp["hd"]: kern.attn_decode_paged_workspace(c, self.nh, batch) for sp, c in zip(specs, self.caches)}
-        self.stream = torch.cuda.Stream(device=dev)
-        self.graph = None
 
     # ------------------------------------------------------------------ requests
     def set_sampling(self, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seeds=None) -> None:
         """Sampling settings, each a number for all sequences or one per sequence;
         temperature 0 is greedy.  They may change between steps."""
-        with torch.cuda.stream(self.stream):
+        with self._own_stream():
             for buf, v in ((self.temperature, temperature), (self.top_k, top_k), (self.top_p, top_p),
                            (self.min_p, min_p), (self.seeds, 0 if seeds is None else seeds)):
+                if isinstance(v, torch.Tensor) and v.is_cuda:
+                    v.record_stream(self.stream)  # its memory stays until this stream has read it
                 v = torch.as_tensor(v, dtype=buf.dtype)
                 if v.dim() and v.numel() != self.B:
                     raise ValueError(f"a setting must be one number or {self.B}")
@@ -150,7 +164,7 @@ class PagedRunner:
         if len(lens) != self.B or min(lens) < 1 or max(lens) + steps > self.dm.max_seq:
             raise ValueError(f"{self.B} prompts of 1 to {self.dm.max_seq - steps} tokens are wanted")
         dm, dev, T = self.dm, self.dm.device, sum(lens)
-        with torch.cuda.stream(self.stream):
+        with self._own_stream():
             self._reserve(lens, steps)
             host = torch.empty(3, T, dtype=torch.int32)
             host[0] = torch.cat([torch.as_tensor(list(p), dtype=torch.int32) for p in prompts])
@@ -216,8 +230,8 @@ class PagedRunner:
         for _ in range(steps):
             self.decode_step()
         self.lens = [n + steps for n in start]
-        torch.cuda.current_stream().wait_stream(self.stream)
-        h = self.history.cpu()
+        with torch.cuda.stream(self.stream):
+            h = self.history.cpu()
         return [h[b, n:n + steps].tolist() for b, n in enumerate(start)]
 
     def generate(self, prompts, steps: int, **sampling) -> list[list[int]]:
