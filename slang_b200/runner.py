@@ -279,6 +279,7 @@ class Runner:
         ws = max(_lib.load().sb_attn_decode_workspace_size(B, self.nh, sp["hd"], S) for sp in specs)
         self.attn_ws = torch.empty(max(1, ws // 4), dtype=torch.float32, device=dev)
         self.stream = torch.cuda.Stream(device=dev)
+        self.stream.wait_stream(torch.cuda.current_stream(dev))  # the buffers' fills and the weights come first
         if fused:
             self._fused_setup()
         self.graph = None
@@ -522,6 +523,8 @@ class Runner:
         if any(self._attn_route(sp, S) == "gemm" for sp in specs):
             ld = (S + 7) // 8 * 8
             pf["scores"], pf["p16"] = f32(S * nh * ld), f16(S * nh * ld)
+        # the buffers' memory may have work of the caller's stream still to come
+        self.stream.wait_stream(torch.cuda.current_stream(dev))
         self._pf = pf
         self._pgraphs.clear()  # captured prefills point at the old buffers
         return pf

@@ -50,3 +50,16 @@ def test_sampling_settings_from_a_busy_stream(cuda, model):
         mine[k].copy_(v)
     assert r.generate(PROMPTS, 8, **mine) == want
     torch.cuda.synchronize()
+
+
+def test_runner_made_behind_a_busy_stream(cuda, model):
+    def run():
+        r = runner.Runner(model, 1)
+        first = r.prefill(PROMPTS[0])
+        return [first] + r.decode(7)[0].tolist()
+
+    want = run()
+    torch.cuda.synchronize()
+    _busy(cuda)
+    assert run() == want
+    torch.cuda.synchronize()
