@@ -672,7 +672,7 @@ int sb_attn_prefill_packed(const void* q, int64_t q_token, int64_t q_head, const
  *   top_k[r]       (off: 0)   keep the k largest logits (k <= 0 or k >= vocab: all)
  *   top_p[r]       (off: 1)   of those keep each whose larger ones sum to less than
  *                             top_p of their total mass (>= 1: all, <= 0: the first)
- *   min_p[r]       (off: 0)   of those keep w_i >= min_p (the largest always stays)
+ *   min_p[r]       (off: 0)   of those keep w_i >= min_p (the first largest always stays: alone above 1, or NaN)
  * Equal logits rank by index, lowest first.  The kept token with the smallest
  * E_i / w_i is drawn (ties: lowest index), which is token i with probability
  * w_i / sum of the kept w; E_i = -log(1 - u_i), u_i = (q_i + 1/2) 2^-32 at most

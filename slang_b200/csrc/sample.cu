@@ -28,7 +28,7 @@
 //   top-p         one pass sums what ranks before the winner.  A token below (1 - p) / V of
 //                 the total is out from the start: all such tokens together
 //                 weigh less than 1 - p, so the prefix above them holds the nucleus.
-//   min-p         a token below w = min_p is out.
+//   min-p         a token below w = min_p is out (min_p <= 1 here: above it the largest is drawn).
 //   top-k         the k-th largest of the lanes' maxima is a lower bound of
 //                 the k-th largest value; what reaches it (a little more than
 //                 k tokens) is sorted by one CTA, which finishes the row alone.
@@ -174,6 +174,11 @@ __device__ Word reduce(Shared& sh, Word w, int cs, int& turn, unsigned* lower = 
   return warp_join(w);
 }
 
+// Settings that keep the largest logit alone (of equal ones the first).  No weight reaches a min_p above 1.
+__device__ __forceinline__ bool is_greedy(float temp, float top_p, float min_p, int top_k) {
+  return !(temp > 0.f) || top_p <= 0.f || !(min_p <= 1.f) || top_k == 1;
+}
+
 // The row of this cluster when the rows are more than one wave of CTAs: within NT neighbours those that take longest
 // come first (top-p without top-k, no filter, top-k, min-p, greedy; stable), so that the last ones to start are short.
 // 128 rows of 262144 with mixed settings: 64 us in place of 78; rows all of one kind pay 2 us, of 24 (greedy) to 105.
@@ -186,7 +191,7 @@ __device__ __forceinline__ int sorted_row(const SampleParams& p, Shared& sh) {
     const float temp = p.temperature ? p.temperature[r] : 1.f, top_p = p.top_p ? p.top_p[r] : 1.f;
     const float min_p = p.min_p ? p.min_p[r] : 0.f;
     const int top_k = p.top_k ? p.top_k[r] : 0;
-    if (!(temp > 0.f) || top_p <= 0.f || top_k == 1) kind = 4;
+    if (is_greedy(temp, top_p, min_p, top_k)) kind = 4;
     else if (top_k > 0) kind = 2;
     else if (min_p > 0.f) kind = 3;
     else kind = top_p < 1.f ? 0 : 1;
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
   const int64_t seed = p.seeds[row];
   const int pos = p.pos[row];
   const T* src = static_cast<const T*>(p.x) + row * p.ld;
-  const bool greedy = !(temp > 0.f) || top_p <= 0.f || top_k == 1;
+  const bool greedy = is_greedy(temp, top_p, min_p, top_k);
   const float inv = fmaxf(kLog2e / temp, 1e-37f);  // above zero, so that -inf stays -inf
   int turn = 0;
 

@@ -1,0 +1,48 @@
+"""GPU: sampling settings at and past the ends of their ranges."""
+import math
+
+import pytest
+import torch
+
+from slang_b200 import kernels as kern
+from tests.test_sample_gpu import reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows(cuda, rows, vocab, seed):
+    gen = torch.Generator(device=cuda).manual_seed(seed)
+    x = 2.5 * torch.randn(rows, vocab, generator=gen, device=cuda)
+    seeds = torch.randint(-2 ** 62, 2 ** 62, (rows,), generator=gen, device=cuda)
+    return x, seeds, torch.arange(rows, dtype=torch.int32, device=cuda)
+
+
+@pytest.mark.parametrize("vocab", [1, 700, 40000])
+@pytest.mark.parametrize("floor", [1.5, 1.0078125, 1e30, math.inf, math.nan])
+@pytest.mark.parametrize("rules", [{}, {"top_k": 5}, {"top_p": 0.7}, {"top_k": 2000, "top_p": 0.9}])
+def test_min_p_above_one_keeps_the_largest(cuda, vocab, floor, rules):
+    """No weight reaches a min_p above 1 (or one that is not a number): the largest logit, the first of
+    equal ones, always stays."""
+    x, seeds, pos = _rows(cuda, 24, vocab, 5)
+    x[8:16, ::7] = x[8:16].amax(1, keepdim=True)  # many equal ones, index 0 among them
+    x[16:, 0], x[16:, vocab // 2:] = -math.inf, x[16:].amax() + 1  # and an upper half of equal ones
+    kw = {k: torch.full((24,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device=cuda)
+          for k, v in rules.items()}
+    got = kern.sample(x, seeds, pos, min_p=torch.full((24,), floor, device=cuda), **kw)
+    want = [int((row == row.max()).nonzero()[0]) for row in x]
+    assert got.tolist() == want
+
+
+@pytest.mark.parametrize("rules", [{}, {"top_k": 3}, {"top_p": 0.4}])
+def test_min_p_of_one_keeps_equal_ones(cuda, rules):
+    """min_p of 1 keeps what weighs as much as the largest: the draw is among equal logits."""
+    n = 64
+    x = torch.tensor([[2.0, 1.0, 2.0, -1.0, 2.0, 0.0]], device=cuda).repeat(n, 1)
+    seeds, pos = torch.arange(n, device=cuda) * 7919 + 3, torch.zeros(n, dtype=torch.int32, device=cuda)
+    kw = {k: torch.full((n,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device=cuda)
+          for k, v in rules.items()}
+    got = kern.sample(x, seeds, pos, min_p=torch.ones(n, device=cuda), **kw).tolist()
+    names = {"top_p": "p", "top_k": "k"}
+    want = [reference(x[r].cpu().numpy(), int(seeds[r]), 0, floor=1.0, **{names[k]: v for k, v in rules.items()})[0]
+            for r in range(n)]
+    assert got == want and len(set(got)) > 1
