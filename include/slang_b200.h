@@ -671,7 +671,7 @@ int sb_attn_prefill_packed(const void* q, int64_t q_token, int64_t q_head, const
  *   temperature[r] (off: 1)   w_i = exp((x_i - max x) / T); T <= 0: the largest logit
  *   top_k[r]       (off: 0)   keep the k largest logits (k <= 0 or k >= vocab: all)
  *   top_p[r]       (off: 1)   of those keep each whose larger ones sum to less than
- *                             top_p of their total mass (>= 1: all, <= 0: the first)
+ *                             top_p of their total mass (>= 1 or NaN: all, <= 0: the first)
  *   min_p[r]       (off: 0)   of those keep w_i >= min_p (the first largest always stays: alone above 1, or NaN)
  * Equal logits rank by index, lowest first.  The kept token with the smallest
  * E_i / w_i is drawn (ties: lowest index), which is token i with probability

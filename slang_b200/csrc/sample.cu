@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
       for (unsigned r = r0; r < r1; ++r) {
         const float x = value_of(key[r]);
         const int idx = static_cast<int>(key[r] & 0xFFFFFFFFu);
-        if (x > -INFINITY && (top_p >= 1.f || static_cast<double>(before) < limit)) best.key = min(best.key, race(x, idx, word_of(idx)));
+        if (x > -INFINITY && (!(top_p < 1.f) || static_cast<double>(before) < limit)) best.key = min(best.key, race(x, idx, word_of(idx)));
         before += mass_of(z2_of(x));
       }
       int none = 0;

@@ -46,3 +46,11 @@ def test_min_p_of_one_keeps_equal_ones(cuda, rules):
     want = [reference(x[r].cpu().numpy(), int(seeds[r]), 0, floor=1.0, **{names[k]: v for k, v in rules.items()})[0]
             for r in range(n)]
     assert got == want and len(set(got)) > 1
+
+
+@pytest.mark.parametrize("top_k", [0, 4, 3000])
+def test_top_p_that_is_not_a_number_is_off(cuda, top_k):
+    x, seeds, pos = _rows(cuda, 16, 9000, 6)
+    k = torch.full((16,), top_k, dtype=torch.int32, device=cuda)
+    got = kern.sample(x, seeds, pos, top_k=k, top_p=torch.full((16,), math.nan, device=cuda))
+    assert torch.equal(got, kern.sample(x, seeds, pos, top_k=k))
