@@ -58,7 +58,9 @@ constexpr int BINS = 256;       // of maxima, 1/8 octave of w each
 constexpr int SORT = 1024;      // candidates of a top-k row that one CTA sorts
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLargest = 3.402823466e38f;  // bounds stay finite: -inf (banned, padding) is below them
-constexpr float kUnit = 2147483648.f;        // masses in units of 2^-31 of the largest token's
+// Masses in units of 2^-40 of the largest token's: a row's stay below 2^60, and 819200 tokens below a unit each
+// weigh less than 2^-20 of it.
+constexpr float kUnit = 1099511627776.f;
 
 struct SampleParams {
   const void* x;
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
     const uint32_t lo = idx & 1 ? r.y : r.x, hi = idx & 1 ? r.w : r.z;
     return idx & 2 ? hi : lo;
   };
-  auto mass_of = [&](float z2) { return static_cast<unsigned long long>(__float2uint_rn(ex2(z2) * kUnit)); };
+  auto mass_of = [&](float z2) { return __float2ull_rn(ex2(z2) * kUnit); };
   auto value_bits = [](uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); };
   auto value_of = [&](unsigned long long key) { return value_bits(~static_cast<uint32_t>(key >> 32)); };
   // a value below every x with log2 w >= c, whatever the rounding on either side
@@ -571,12 +573,15 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
       for (; may; may &= may - 1) enter(index_of(seg, __ffs(may) - 1));
     }
   };
-  // the mass of what ranks before (xl, il); lanes below it are not read again
+  // the mass of what ranks before (xl, il); lanes below it are not read again.  A lane's values of a segment are
+  // summed in f32, as in the segments' own masses, and rounded to units once.
   auto mass_all = [&] {
     visit(fmaxf(-kLargest, value_bits(xl)), [&](int seg, float (&v)[32]) {
+      float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (in(v[i], index_of(seg, i))) w.sum += mass_of(z2_of(v[i]));
+        if (in(v[i], index_of(seg, i))) sum += ex2(z2_of(v[i]));
+      w.sum += __float2ull_rn(sum * kUnit);
     });
   };
   if (top_p < 1.f) {  // the whole: of all tokens from the segments, of a top-k's by a pass

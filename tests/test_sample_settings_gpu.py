@@ -1,4 +1,4 @@
-"""GPU: sampling settings at and past the ends of their ranges."""
+"""GPU: sampling settings at and past the ends of their ranges, nuclei of very small weights."""
 import math
 
 import pytest
@@ -54,3 +54,26 @@ def test_top_p_that_is_not_a_number_is_off(cuda, top_k):
     k = torch.full((16,), top_k, dtype=torch.int32, device=cuda)
     got = kern.sample(x, seeds, pos, top_k=k, top_p=torch.full((16,), math.nan, device=cuda))
     assert torch.equal(got, kern.sample(x, seeds, pos, top_k=k))
+
+
+def test_nucleus_of_very_small_weights(cuda):
+    """One token weighs 1, 800000 others 2^-33 each, and top_p ends half way through those: what is
+    drawn of them lies in the first half.  (Their masses are lost to sums in units of 2^-31.)"""
+    vocab, rows, w = 800000, 100, 2.0 ** -33
+    x = torch.full((1, vocab), math.log(w), device=cuda)
+    x[0, 0] = 0.0
+    x = x.repeat(rows, 1)
+    w = math.exp(float(x[0, 1]))
+    total = 1 + (vocab - 1) * w
+    p = torch.full((rows,), (1 + 0.5 * vocab * w) / total, device=cuda)
+    # tokens 1 .. last are in; the sums resolve 2^-23 of the total, 1024 such tokens, and p 2^-24
+    last, slack = int((float(p[0]) * total - 1) / w) + 1, 2048
+    pos = torch.zeros(rows, dtype=torch.int32, device=cuda)
+    drawn = []
+    for call in range(1500):
+        seeds = torch.arange(rows, device=cuda) + call * rows
+        got = kern.sample(x, seeds, pos, top_p=p)
+        drawn.append(got[got != 0])
+    drawn = torch.cat(drawn).tolist()
+    # 150000 draws, each with a chance of 4.7e-5 of one of them: 7 expected, none with a chance of e^-7
+    assert drawn and max(drawn) <= last + slack, (last, drawn)
