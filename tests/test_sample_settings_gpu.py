@@ -1,11 +1,12 @@
-"""GPU: sampling settings at and past the ends of their ranges, nuclei of very small weights."""
+"""GPU: sampling settings at and past the ends of their ranges, the softcap, nuclei of very small weights."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from slang_b200 import kernels as kern
-from tests.test_sample_gpu import reference
+from tests.test_sample_gpu import RESOLVED, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,37 @@ def test_nucleus_of_very_small_weights(cuda):
     drawn = torch.cat(drawn).tolist()
     # 150000 draws, each with a chance of 4.7e-5 of one of them: 7 expected, none with a chance of e^-7
     assert drawn and max(drawn) <= last + slack, (last, drawn)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [1000, 50001])
+@pytest.mark.parametrize("softcap", [5.0, 30.0])
+def test_softcap(cuda, dtype, vocab, softcap):
+    """The draw is that of softcap * tanh(x / softcap), in every rule."""
+    rows = 48
+    x, seeds, pos = _rows(cuda, rows, vocab, vocab)
+    x = (0.24 * softcap * x).to(dtype)  # up to about 2.5 times the cap
+    x[1, ::3] = -math.inf
+    u = torch.rand(3, rows, generator=torch.Generator(device=cuda).manual_seed(1), device=cuda)
+    kind = torch.arange(rows, device=cuda) % 6
+    temp = torch.where(kind == 0, 0.0, 0.5 + u[0])
+    k = torch.where((kind == 2) | (kind == 4), 1 + (300 * u[1]).int(), 0).to(torch.int32)
+    p = torch.where((kind == 1) | (kind == 4), 0.3 + 0.6 * u[2], 1.0)
+    floor = torch.where((kind == 3) | (kind == 4), 0.2 * u[0], 0.0)
+    got = kern.sample(x, seeds, pos, temperature=temp, top_k=k, top_p=p, min_p=floor, softcap=softcap).tolist()
+    plain = kern.sample(x, seeds, pos, temperature=temp, top_k=k, top_p=p, min_p=floor).tolist()
+    checked = 0
+    for r in range(rows):
+        v = x[r].double().cpu().numpy()
+        capped = np.where(np.isinf(v), v, softcap * np.tanh(v / softcap))
+        args = [int(seeds[r]), int(pos[r]), float(temp[r]), int(k[r]), float(p[r]), float(floor[r])]
+        want, gap = reference(capped, *args)
+        # the cap is computed in f32, a few 2^-22 off: values closer than that may change places
+        top = np.sort(capped)[::-1]
+        edges = [0] if kind[r] == 0 else [int(k[r]) - 1] if k[r] > 0 else []
+        for at in edges:
+            gap = min(gap, math.inf if top[at] == top[at + 1] else top[at] - top[at + 1])
+        if gap > 4 * RESOLVED:  # 2^-14: steps of 2^-18 at 30, twice, over temperatures from 0.5
+            checked += 1
+            assert got[r] == want, (r, args)
+    assert checked >= 0.75 * rows and got != plain
