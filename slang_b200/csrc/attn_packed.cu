@@ -228,6 +228,13 @@ __device__ __forceinline__ float2 exp2_fma(uint64_t y) {
                      __int_as_float(__float_as_int(v.y) + (__float_as_int(k.y) << 23)));
 }
 
+// the larger, NaN if one of them is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // n low bits set, none below 0 and all from 32 on
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u; }
 
@@ -251,17 +258,24 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
       for (int e = 0; e < 32; ++e) sv[c][e] = seen & (1u << e) ? sv[c][e] : 0xFF800000u;  // -inf
     }
   }
+  // The polynomial below makes a number of anything: where it is used, the maximum keeps a NaN, and a warp with a query
+  // whose maximum is not finite takes all of the block's exponentials in the special-function unit.
+  constexpr bool kPoly = HD == 64;
+  auto larger = [](float a, float b) { return kPoly ? max_nan(a, b) : fmaxf(a, b); };
   float mx[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     mx[c] = __uint_as_float(sv[0][c]);
 #pragma unroll
-    for (int e = 4 + c; e < KB; e += 4) mx[c] = fmaxf(mx[c], __uint_as_float(sv[e >> 5][e & 31]));
+    for (int e = 4 + c; e < KB; e += 4) mx[c] = larger(mx[c], __uint_as_float(sv[e >> 5][e & 31]));
   }
-  const float mx2 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+  const float mx2 = larger(larger(mx[0], mx[1]), larger(mx[2], mx[3])) * scale2;
+  const bool odd = kPoly && whole && hi > 0 && !(fabsf(mx2) < INFINITY);  // hi: 0 where there is no query, but any value
+  bool any_odd = false;
   const bool start = m == -INFINITY;  // O is still zero in this row
   const bool rise = !start && mx2 > m + kRise;
-  if (__any_sync(0xFFFFFFFFu, rise)) {
+  if (__any_sync(0xFFFFFFFFu, rise || odd)) {
+    any_odd = kPoly && __any_sync(0xFFFFFFFFu, odd);
     // O += P V of the block before has to be complete before it is scaled
     if (!__all_sync(0xFFFFFFFFu, pv_before())) return false;
     sbd::tc_fence_after();
@@ -283,7 +297,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
   const uint64_t scale_2 = pack_f2(scale2, scale2), shift_2 = pack_f2(-mu, -mu);
   uint64_t sum[2] = {0, 0};  // pairs of zeros
   // POLY of 16 pairs of exponentials leave the special-function unit, 16 a cycle and SM, for the FMA pipe; not where
-  // a masked score has to give exactly 0.  At head_dim 64, bound by that unit, one prompt of 8000 tokens and 16 heads
+  // a masked score has to give exactly 0, nor beside scores that are not finite.  At head_dim 64, bound by that unit, one prompt of 8000 tokens and 16 heads
   // takes 242 us with 5 of 16, 247 with none and 258 with 9; at 128 and 256 none is best (6 prompts of 2000 tokens,
   // 32 heads of 128: 277 to 279 us with 0, 1 or 2, 283 with 6): there the issue slots are the scarcer ones.
   auto exps = [&](auto poly) {
@@ -307,7 +321,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
       sbd::tmem_st_32x32b_x16(tp + 16 * c, pk);
     }
   };
-  if (whole) exps(std::integral_constant<int, HD == 64 ? 5 : 0>{});
+  if (whole && !any_odd) exps(std::integral_constant<int, kPoly ? 5 : 0>{});
   else exps(std::integral_constant<int, 0>{});
   const float2 s0 = unpack_f2(sum[0]), s1 = unpack_f2(sum[1]);
   l += (s0.x + s0.y) + (s1.x + s1.y);
