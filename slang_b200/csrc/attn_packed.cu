@@ -55,7 +55,8 @@
 //        maximum) took 147 in place of 131, a third CTA does not fit tensor memory.
 //
 // S, O, m and l are f32; p is rounded to the input type for the second product
-// (its relative error is that of the output's own rounding).  Every wait is
+// (its relative error is that of the output's own rounding; f16 weights are lifted, see
+// kLift).  Every wait is
 // bounded (2 s): a stuck pipeline records SB_ERR_TIMEOUT and unwinds.
 #include <cudaTypedefs.h>
 
@@ -69,7 +70,7 @@ namespace {
 
 constexpr int QR = 128;  // query rows per tile
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRise = 8.f;  // log2 units: p stays below 2^8
+using sbp::kRise;
 
 // head_dim 64, one CTA
 struct Cfg64 {
@@ -293,7 +294,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
     l *= alpha;
   }
   if (start || rise) m = mx2;
-  const float mu = m == -INFINITY ? 0.f : m;
+  const float mu = (m == -INFINITY ? 0.f : m) - sbp::kLift<T>;
   const uint64_t scale_2 = pack_f2(scale2, scale2), shift_2 = pack_f2(-mu, -mu);
   uint64_t sum[2] = {0, 0};  // pairs of zeros
   // POLY of 16 pairs of exponentials leave the special-function unit, 16 a cycle and SM, for the FMA pipe; not where

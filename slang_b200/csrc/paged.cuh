@@ -5,6 +5,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace sbp {
@@ -32,6 +34,14 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+
+// Softmax weights p = 2^(s - m) rounded to T for the second product are held 2^kLift times as large, as are their sums.
+// m lies at most kRise below the largest score, so p < 2^8 and f16 has 2^7 to spare: its smallest weights are
+// 2^-31 of the one at m in place of 2^-24, which thousands of them beside one that dominates (an attention sink) would
+// lose.  bf16 has the range of f32.
+constexpr float kRise = 8.f;
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
 
 // Eight values at p + 8 * i as f32 (16-byte aligned; two vectors for f32).
 template <typename T>
