@@ -175,7 +175,10 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
     sh_first[0] = b, sh_first[1] = at, sh_first[2] = lo, sh_first[3] = hi;
   }
   __syncthreads();
-  int b = sh_first[0], seq_start = sh_first[1], lo = sh_first[2], hi = sh_first[3];  // seq_start: its first block
+  // The sequence in 64 bits where that saves spilled registers: 64 sequences of 4000 keys with 4 heads of 64 per kv head
+  // take 59.6 us in place of 64.0; with two tiles of heads it costs some (16 heads of 512: 83.4 in place of 80.2).
+  std::conditional_t<NT == 1, int64_t, int> b = sh_first[0];
+  int seq_start = sh_first[1], lo = sh_first[2], hi = sh_first[3];  // seq_start: its first block
   const T* kbase = static_cast<const T*>(p.pages.k);
   const T* vbase = static_cast<const T*>(p.pages.v);
   const int pmask = (1 << p.pages.shift) - 1;
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
     const int nblk = (hi - lo + KB - 1) / KB;
     if (r >= seq_start + nblk * (p.nkv * p.htiles)) {
       seq_start += nblk * (p.nkv * p.htiles);
-      key_range(p, ++b, &lo, &hi);
+      key_range(p, static_cast<int>(++b), &lo, &hi);
       continue;
     }
     const int hidx = (r - seq_start) / nblk;  // (kv head, head tile)
