@@ -49,7 +49,8 @@ class PagedRunner:
         with self._own_stream():
             self._allocate(specs, batch, n_pages, page_size)
         self.free = list(range(n_pages))
-        self.lens, self.room = [0] * batch, [0] * batch
+        # tokens of each sequence behind its prefill, decode steps since then and how many more there is room for
+        self.lens, self.taken, self.left = [0] * batch, 0, 0
         self.graph = None
 
     def _own_stream(self):
@@ -87,8 +88,10 @@ class PagedRunner:
                     raise ValueError(f"a setting must be one number or {self.B}")
                 buf.copy_(v.expand(self.B))
 
-    def _reserve(self, lens, extra: int) -> None:
-        """Pages for each sequence's prompt and ``extra`` more tokens; the last batch's go back."""
+    def _reserve(self, lens, extra: int) -> int:
+        """Pages for each sequence's prompt and ``extra`` more tokens; the last batch's go back.  Returns
+        the decode steps that there is room for: a step appends the token that the one before drew,
+        and its own goes into the history."""
         need = [-(-(n + extra) // self.page_size) for n in lens]
         if sum(need) > self.n_pages:
             raise ValueError(f"{sum(need)} pages needed, the caches have {self.n_pages}")
@@ -97,7 +100,8 @@ class PagedRunner:
         for b, n in enumerate(need):
             rows[b, :n] = torch.tensor([self.free.pop() for _ in range(n)], dtype=torch.int32)
         self.table.copy_(rows)
-        self.room = [n * self.page_size for n in need]
+        self.lens, self.taken, self.left = [n + 1 for n in lens], 0, 0
+        return min(min(p * self.page_size - n, self.dm.max_seq - n - 1) for p, n in zip(need, lens))
 
     # ------------------------------------------------------------------ layers
     def _layers(self, x: torch.Tensor, m: int, attend) -> torch.Tensor:
@@ -161,11 +165,13 @@ class PagedRunner:
         """Run the batch's prompts packed through the layers, with pages for ``steps`` tokens
         more each; returns the first token drawn for each."""
         lens = [len(p) for p in prompts]
+        if steps < 0:
+            raise ValueError("steps must not be negative")
         if len(lens) != self.B or min(lens) < 1 or max(lens) + steps > self.dm.max_seq:
             raise ValueError(f"{self.B} prompts of 1 to {self.dm.max_seq - steps} tokens are wanted")
         dm, dev, T = self.dm, self.dm.device, sum(lens)
         with self._own_stream():
-            self._reserve(lens, steps)
+            left = self._reserve(lens, steps)
             host = torch.empty(3, T, dtype=torch.int32)
             host[0] = torch.cat([torch.as_tensor(list(p), dtype=torch.int32) for p in prompts])
             host[1] = torch.cat([torch.arange(n, dtype=torch.int32) for n in lens])
@@ -192,7 +198,7 @@ class PagedRunner:
             self.pos.copy_(ends - 1)
             self._draw(out32[rows], out16[rows], self.pos)
             first = self.tok.tolist()
-        self.lens = [n + 1 for n in lens]
+        self.left = left
         return first
 
     def _step(self) -> None:
@@ -210,6 +216,8 @@ class PagedRunner:
 
     def decode_step(self) -> None:
         """One step for the whole batch; captured as a CUDA graph on first use."""
+        if self.left < 1:
+            raise ValueError("the sequences outgrow max_seq or the pages that prefill reserved for them")
         with torch.cuda.stream(self.stream):
             if self.graph is None:
                 saved = [t.clone() for t in (self.pos, self.cur, self.tok, self.history)]
@@ -221,21 +229,24 @@ class PagedRunner:
                 with torch.cuda.graph(self.graph, stream=self.stream):
                     self._step()
             self.graph.replay()
+        self.left -= 1
+        self.taken += 1
 
     def decode(self, steps: int) -> list[list[int]]:
         """``steps`` more tokens for every sequence (``prefill`` has to have reserved their pages)."""
-        start = self.lens
-        if max(start) + steps > self.dm.max_seq or any(n - 1 + steps > r for n, r in zip(start, self.room)):
-            raise ValueError("the sequences outgrow max_seq or the pages reserved for them")
+        start = [n + self.taken for n in self.lens]
+        if steps < 0 or steps > self.left:
+            raise ValueError(f"there is room for {self.left} more steps (pages that prefill reserved, max_seq)")
         for _ in range(steps):
             self.decode_step()
-        self.lens = [n + steps for n in start]
         with torch.cuda.stream(self.stream):
             h = self.history.cpu()
         return [h[b, n:n + steps].tolist() for b, n in enumerate(start)]
 
     def generate(self, prompts, steps: int, **sampling) -> list[list[int]]:
-        """``steps`` tokens for each prompt with the given sampling settings (``set_sampling``)."""
+        """``steps`` tokens (at least one) for each prompt with the given sampling settings (``set_sampling``)."""
+        if steps < 1:
+            raise ValueError("steps must be positive")
         self.set_sampling(**sampling)
         first = self.prefill(prompts, steps)
         rest = self.decode(steps - 1) if steps > 1 else [[] for _ in first]
