@@ -79,13 +79,16 @@ class PagedRunner:
         """Sampling settings, each a number for all sequences or one per sequence;
         temperature 0 is greedy.  They may change between steps."""
         with self._own_stream():
+            new = []
             for buf, v in ((self.temperature, temperature), (self.top_k, top_k), (self.top_p, top_p),
                            (self.min_p, min_p), (self.seeds, 0 if seeds is None else seeds)):
                 if isinstance(v, torch.Tensor) and v.is_cuda:
                     v.record_stream(self.stream)  # its memory stays until this stream has read it
                 v = torch.as_tensor(v, dtype=buf.dtype)
-                if v.dim() and v.numel() != self.B:
+                if v.dim() > 1 or (v.dim() and v.numel() != self.B):
                     raise ValueError(f"a setting must be one number or {self.B}")
+                new.append((buf, v))
+            for buf, v in new:
                 buf.copy_(v.expand(self.B))
 
     def _reserve(self, lens, extra: int) -> int:

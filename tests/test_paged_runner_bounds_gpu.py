@@ -63,3 +63,13 @@ def test_bad_step_counts(cuda, model):
     r.prefill(_prompts(9), steps=2)
     with pytest.raises(ValueError):
         r.decode(-1)
+
+
+def test_refused_settings_change_nothing(cuda, model):
+    r = paged.PagedRunner(model, 2, n_pages=8, page_size=4)
+    r.set_sampling(temperature=0.5, top_k=7)
+    for bad in (dict(temperature=0.9, top_p=[0.1, 0.2, 0.3]), dict(temperature=0.9, seeds=[[1], [2]])):
+        with pytest.raises(ValueError):
+            r.set_sampling(**bad)
+    torch.cuda.synchronize()
+    assert r.temperature.tolist() == [0.5, 0.5] and r.top_k.tolist() == [7, 7]
