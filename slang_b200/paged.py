@@ -173,10 +173,14 @@ class PagedRunner:
         if len(lens) != self.B or min(lens) < 1 or max(lens) + steps > self.dm.max_seq:
             raise ValueError(f"{self.B} prompts of 1 to {self.dm.max_seq - steps} tokens are wanted")
         dm, dev, T = self.dm, self.dm.device, sum(lens)
+        tokens = torch.cat([torch.as_tensor(list(p), dtype=torch.int64) for p in prompts])
+        rows = dm.embed_q.shape[0]
+        if int(tokens.min()) < 0 or int(tokens.max()) >= rows:  # they are looked up without a check
+            raise ValueError(f"tokens must lie in 0 .. {rows - 1}")
         with self._own_stream():
             left = self._reserve(lens, steps)
             host = torch.empty(3, T, dtype=torch.int32)
-            host[0] = torch.cat([torch.as_tensor(list(p), dtype=torch.int32) for p in prompts])
+            host[0] = tokens
             host[1] = torch.cat([torch.arange(n, dtype=torch.int32) for n in lens])
             host[2] = torch.repeat_interleave(torch.arange(self.B, dtype=torch.int32), torch.tensor(lens))
             tok, pos, seq = host.to(dev).unbind(0)

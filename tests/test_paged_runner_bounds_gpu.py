@@ -73,3 +73,14 @@ def test_refused_settings_change_nothing(cuda, model):
             r.set_sampling(**bad)
     torch.cuda.synchronize()
     assert r.temperature.tolist() == [0.5, 0.5] and r.top_k.tolist() == [7, 7]
+
+
+def test_tokens_outside_the_vocabulary(cuda, model):
+    """They would be read from past the embedding table: refused before anything is changed."""
+    r = paged.PagedRunner(model, 2, n_pages=8, page_size=4)
+    first = r.prefill(_prompts(6, 3), steps=4)
+    for bad in (2048, -1, 2 ** 31, 2 ** 40, -2 ** 31):
+        with pytest.raises(ValueError):
+            r.prefill([[1, 2, bad], [3]], steps=4)
+    again = paged.PagedRunner(model, 2, n_pages=8, page_size=4)
+    assert again.prefill(_prompts(6, 3), steps=4) == first and again.decode(3) == r.decode(3)
