@@ -627,7 +627,9 @@ int sb_kv_append_paged(const sb_paged_kv* kv, const int32_t* page_table, int n_s
  * q[i][h] . K) V over the cached keys at positions lo .. pos[i] of page-table
  * row i, lo = 0, or pos[i] + 1 - window when window > 0; a row without a key
  * (pos[i] < 0) gives zeros.  q [b] rows of [n_heads][head_dim] q_stride elements
- * apart and out [b][n_heads][head_dim] are of the cache's type.
+ * apart and out [b][n_heads][head_dim] are of the cache's type.  A table must hold
+ * fewer than 2^36 keys in all: b * max_pages * page_size * n_kv_heads, and that once for
+ * every 16 query heads of a kv head.
  * workspace: device, 16-byte aligned, at least
  * sb_attn_decode_paged_workspace_size bytes (the same for every b >= 1), zero before
  * the first call; each call leaves it ready for the next, of any batch, head counts

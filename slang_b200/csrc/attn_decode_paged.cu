@@ -105,6 +105,7 @@ struct Shape {
   static constexpr int TK = 16 * NS;       // keys per warp (team) and iteration
   static constexpr int TEAMS = W / HS;
   static constexpr int KB = TK * TEAMS;    // keys per block
+  static_assert(KB >= 32, "the entry point's bound on the number of blocks");
   static constexpr int HT = 8 * NT;
   static constexpr int PART = HT * (HD + 2);       // a partial: O [HT][HD], m [HT], l [HT]
   static constexpr int HP = HD + 4;                // a head's row in shared memory: neighbouring heads in other banks
@@ -131,8 +132,8 @@ __global__ void __launch_bounds__(W * 32, 2) attn_decode_paged_kernel(const Deco
   sbd::griddep_wait();
 
   // total blocks of all sequences, this CTA's run of them [r0, r1) and the sequence that holds r0: each
-  // thread counts a few neighbouring sequences, whose loads are one latency (blocks of 16 keys or more of
-  // a cache that fits a GPU number far below 2^31)
+  // thread counts a few neighbouring sequences, whose loads are one latency (the entry point has checked
+  // that they number below 2^31)
   auto blocks_of = [&](int lo, int hi) { return (hi - lo + KB - 1) / KB * (p.nkv * p.htiles); };
   const int per = (p.b + W * 32 - 1) / (W * 32), b0 = threadIdx.x * per, b1 = min(b0 + per, p.b);
   int own = 0;
@@ -580,6 +581,10 @@ extern "C" int sb_attn_decode_paged(const sb_paged_kv* kv, const int32_t* page_t
   const int group = n_heads / kv->n_kv_heads, ht = head_tile(group);
   p.q = q, p.q_stride = q_stride, p.out = out, p.pos = pos, p.b = b, p.nkv = kv->n_kv_heads, p.group = group;
   p.htiles = (group + ht - 1) / ht, p.window = window, p.scale2 = scale * kLog2e;
+  // what the table's rows can hold, in the kernel's 32-bit numbers of keys and of blocks (of 32 keys at least)
+  const int64_t held = static_cast<int64_t>(max_pages) * kv->page_size;
+  SB_CHECK_ARG(held <= (1ll << 31) - 4096 && (held / 32 + 1) * p.nkv * p.htiles < (1ll << 31) / b,
+               "sb_attn_decode_paged: a page table for %d sequences of %lld keys is too large", b, static_cast<long long>(held));
   const int grid = grid_of();
   p.group_count = static_cast<unsigned int*>(workspace);
   p.count = p.group_count + group_bytes(grid) / 4;

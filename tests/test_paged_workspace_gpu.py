@@ -1,9 +1,10 @@
-"""GPU: one decode workspace through calls of changing batch, head counts and head_dim."""
+"""GPU: one decode workspace through calls of changing batch, head counts and head_dim; the largest page tables."""
 import math
 
 import pytest
 import torch
 
+from slang_b200 import _lib
 from slang_b200 import kernels as kern
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +57,23 @@ def test_layers_of_other_shapes_share_a_workspace(cuda):
     for _ in range(3):
         for s, want in zip(states, fresh):
             assert torch.equal(_attend(s, ws), want)
+
+
+def test_page_tables_past_32_bits(cuda):
+    """Tables whose rows could hold more blocks of keys than 32 bits count are refused; one short of that
+    is served, whatever little of it is used."""
+    page = 1 << 20
+    none = torch.zeros(0, 1, page, 64, dtype=torch.float16, device=cuda)
+    cache = kern.PagedKV(none, none)
+
+    def attend(b, pages):
+        q = torch.ones(b, 8, 64, dtype=torch.float16, device=cuda)
+        table = torch.full((b, pages), -1, dtype=torch.int32, device=cuda)
+        return kern.attn_decode_paged(q, cache, table, torch.arange(b, dtype=torch.int32, device=cuda))
+
+    for b, pages in ((2, 2047), (32, 2047)):  # 32 * 2047 * 2^20 is 2^36 less 2^25
+        assert torch.all(attend(b, pages) == 0)
+    for b, pages in ((33, 2047), (65536, 1), (1, 2048)):
+        with pytest.raises(_lib.SlangError) as e:
+            attend(b, pages)
+        assert e.value.code == _lib.SB_ERR_ARG
