@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(NT, CTAS) sample_kernel(const SampleParams p) 
   const int pos = p.pos[row];
   const T* src = static_cast<const T*>(p.x) + row * p.ld;
   const bool greedy = is_greedy(temp, top_p, min_p, top_k);
-  const float inv = fmaxf(kLog2e / temp, 1e-37f);  // above zero, so that -inf stays -inf
+  const float inv = fmaxf(kLog2e / temp, 1e-45f);  // above zero, so that -inf stays -inf at any temperature
   int turn = 0;
 
   // This lane's values of a segment: v[4 j + e] is value seg * SEG + 128 j + 4 lane + e, -inf for NaN and past the end.

@@ -112,3 +112,19 @@ def test_softcap(cuda, dtype, vocab, softcap):
             checked += 1
             assert got[r] == want, (r, args)
     assert checked >= 0.75 * rows and got != plain
+
+
+@pytest.mark.parametrize("rules", [{"top_p": 0.3}, {"top_k": 100, "top_p": 0.5}, {"min_p": 0.5}, {}])
+def test_infinite_temperature(cuda, rules):
+    """Every finite logit weighs 1, however far apart they lie."""
+    rows, vocab = 32, 700
+    x, seeds, pos = _rows(cuda, rows, vocab, 8)
+    x = x * 1e37
+    x[:, ::5] = -math.inf
+    kw = {k: torch.full((rows,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device=cuda)
+          for k, v in rules.items()}
+    got = kern.sample(x, seeds, pos, temperature=torch.full((rows,), math.inf, device=cuda), **kw).tolist()
+    names = {"top_p": "p", "top_k": "k", "min_p": "floor"}
+    for r in range(rows):
+        want, gap = reference(x[r].cpu().numpy(), int(seeds[r]), int(pos[r]), 1e300, **{names[k]: v for k, v in rules.items()})
+        assert gap <= RESOLVED or got[r] == want, r
