@@ -201,40 +201,6 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^y on the FMA and integer pipes, for y up to about 100 (below -126: 2^-126): y = n + f with n the nearest
-// integer (Cody and Waite's reduction, n read off the low bits of y + 1.5 * 2^23) and 2^f, |f| <= 1/2, by a minimax
-// polynomial fitted for this interval: relative error 7.5e-5 (degree 3) for bf16, 2.6e-6 (degree 4) for f16,
-// below a seventh of what the rounding of p to its type does.
-template <typename T>
-__device__ __forceinline__ float2 exp2_fma(uint64_t y) {
-  constexpr float kMagic = 12582912.f;
-  const float2 c = unpack_f2(y);
-  y = pack_f2(fmaxf(c.x, -126.f), fmaxf(c.y, -126.f));
-  const uint64_t t = add_f2(y, pack_f2(kMagic, kMagic));
-  const uint64_t n = add_f2(t, pack_f2(-kMagic, -kMagic));
-  const uint64_t f = fma_f2(n, pack_f2(-1.f, -1.f), y);
-  uint64_t p;
-  if constexpr (std::is_same<T, __half>::value) {
-    p = fma_f2(f, pack_f2(0.009570102207362652f, 0.009570102207362652f), pack_f2(0.05591785907745361f, 0.05591785907745361f));
-    p = fma_f2(f, p, pack_f2(0.240247443318367f, 0.240247443318367f));
-    p = fma_f2(f, p, pack_f2(0.6931217908859253f, 0.6931217908859253f));
-    p = fma_f2(f, p, pack_f2(0.9999992847442627f, 0.9999992847442627f));
-  } else {
-    p = fma_f2(f, pack_f2(0.0551716685295105f, 0.0551716685295105f), pack_f2(0.2426111251115799f, 0.2426111251115799f));
-    p = fma_f2(f, p, pack_f2(0.6932609677314758f, 0.6932609677314758f));
-    p = fma_f2(f, p, pack_f2(0.9999280571937561f, 0.9999280571937561f));
-  }
-  const float2 v = unpack_f2(p), k = unpack_f2(t);
-  return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(k.x) << 23)),
-                     __int_as_float(__float_as_int(v.y) + (__float_as_int(k.y) << 23)));
-}
-
-// the larger, NaN if one of them is
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 
 // n low bits set, none below 0 and all from 32 on
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u; }
@@ -259,24 +225,17 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
       for (int e = 0; e < 32; ++e) sv[c][e] = seen & (1u << e) ? sv[c][e] : 0xFF800000u;  // -inf
     }
   }
-  // The polynomial below makes a number of anything: where it is used, the maximum keeps a NaN, and a warp with a query
-  // whose maximum is not finite takes all of the block's exponentials in the special-function unit.
-  constexpr bool kPoly = HD == 64;
-  auto larger = [](float a, float b) { return kPoly ? max_nan(a, b) : fmaxf(a, b); };
   float mx[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     mx[c] = __uint_as_float(sv[0][c]);
 #pragma unroll
-    for (int e = 4 + c; e < KB; e += 4) mx[c] = larger(mx[c], __uint_as_float(sv[e >> 5][e & 31]));
+    for (int e = 4 + c; e < KB; e += 4) mx[c] = fmaxf(mx[c], __uint_as_float(sv[e >> 5][e & 31]));
   }
-  const float mx2 = larger(larger(mx[0], mx[1]), larger(mx[2], mx[3])) * scale2;
-  const bool odd = kPoly && whole && hi > 0 && !(fabsf(mx2) < INFINITY);  // hi: 0 where there is no query, but any value
-  bool any_odd = false;
+  const float mx2 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
   const bool start = m == -INFINITY;  // O is still zero in this row
   const bool rise = !start && mx2 > m + kRise;
-  if (__any_sync(0xFFFFFFFFu, rise || odd)) {
-    any_odd = kPoly && __any_sync(0xFFFFFFFFu, odd);
+  if (__any_sync(0xFFFFFFFFu, rise)) {
     // O += P V of the block before has to be complete before it is scaled
     if (!__all_sync(0xFFFFFFFFu, pv_before())) return false;
     sbd::tc_fence_after();
@@ -297,33 +256,21 @@ __device__ __forceinline__ bool softmax_block(uint32_t ts, uint32_t tp, uint32_t
   const float mu = (m == -INFINITY ? 0.f : m) - sbp::kLift<T>;
   const uint64_t scale_2 = pack_f2(scale2, scale2), shift_2 = pack_f2(-mu, -mu);
   uint64_t sum[2] = {0, 0};  // pairs of zeros
-  // POLY of 16 pairs of exponentials leave the special-function unit, 16 a cycle and SM, for the FMA pipe; not where
-  // a masked score has to give exactly 0, nor beside scores that are not finite.  At head_dim 64, bound by that unit, one prompt of 8000 tokens and 16 heads
-  // takes 242 us with 5 of 16, 247 with none and 258 with 9; at 128 and 256 none is best (6 prompts of 2000 tokens,
-  // 32 heads of 128: 277 to 279 us with 0, 1 or 2, 283 with 6): there the issue slots are the scarcer ones.
-  auto exps = [&](auto poly) {
-    constexpr int POLY = decltype(poly)::value;
+  // All exponentials in the special-function unit, 16 a cycle and SM.  Some of them by a polynomial on the FMA pipe cost
+  // more issue slots than they save even at head_dim 64, and need a way of their own for scores that are not finite: one
+  // prompt of 8000 tokens and 16 heads takes 221 us with none, 228 with 3 of 16, 237 with 5 and 247 with 9.
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      uint32_t pk[16];
+  for (int c = 0; c < CH; ++c) {
+    uint32_t pk[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint64_t y = fma_f2(pack_f2(__uint_as_float(sv[c][2 * e]), __uint_as_float(sv[c][2 * e + 1])), scale_2, shift_2);
-        float2 p;
-        if ((e * POLY) % 16 + POLY >= 16) {  // spread evenly
-          p = exp2_fma<T>(y);
-        } else {
-          p = unpack_f2(y);
-          p = make_float2(ex2(p.x), ex2(p.y));
-        }
-        sum[e & 1] = add_f2(sum[e & 1], pack_f2(p.x, p.y));
-        pk[e] = sbp::pack2<T>(p.x, p.y);
-      }
-      sbd::tmem_st_32x32b_x16(tp + 16 * c, pk);
+    for (int e = 0; e < 16; ++e) {
+      float2 p = unpack_f2(fma_f2(pack_f2(__uint_as_float(sv[c][2 * e]), __uint_as_float(sv[c][2 * e + 1])), scale_2, shift_2));
+      p = make_float2(ex2(p.x), ex2(p.y));
+      sum[e & 1] = add_f2(sum[e & 1], pack_f2(p.x, p.y));
+      pk[e] = sbp::pack2<T>(p.x, p.y);
     }
-  };
-  if (whole && !any_odd) exps(std::integral_constant<int, kPoly ? 5 : 0>{});
-  else exps(std::integral_constant<int, 0>{});
+    sbd::tmem_st_32x32b_x16(tp + 16 * c, pk);
+  }
   const float2 s0 = unpack_f2(sum[0]), s1 = unpack_f2(sum[1]);
   l += (s0.x + s0.y) + (s1.x + s1.y);
   sbd::tmem_wait_st();
