@@ -651,8 +651,9 @@ size_t sb_attn_decode_paged_workspace_size(const sb_paged_kv* kv, int n_heads, i
  * k and v [t_k][n_kv_heads] and out [t_q][n_heads] rows of head_dim lie *_token and
  * *_head elements apart (multiples of 8, k and v alike).  What lies in rows of
  * other sequences, NaN included, changes nothing; a NaN or infinity in a value row
- * of the sequence itself may also reach queries before it (0 times it, in a block of
- * up to 128 keys), one in a key row does not.
+ * of the sequence itself may also reach queries that do not see it, those before it and
+ * those whose window begins behind it (0 times it, in a block of up to 128 keys); one
+ * in a key row reaches the queries that see it alone.
  * tiles: device copy of what sb_attn_packed_plan wrote for the same lengths, head
  * counts and head_dim (host arrays; tiles NULL: the count alone; kv_lens NULL: as
  * q_lens; 8 int32 per tile; `window` only orders them, longest first).  A plan
@@ -670,8 +671,10 @@ int sb_attn_prefill_packed(const void* q, int64_t q_token, int64_t q_head, const
  * stride ld; rows <= 65535, vocab <= 819200).  softcap > 0: logits are first capped,
  * x = softcap * tanh(x / softcap), -inf excepted (the model's final_logit_softcapping,
  * gemma4/reference.py:179).  Per row r, each setting a device array or NULL for "off":
- *   temperature[r] (off: 1)   w_i = exp((x_i - max x) / T); T <= 0: the largest logit
- *   top_k[r]       (off: 0)   keep the k largest logits (k <= 0 or k >= vocab: all)
+ *   temperature[r] (off: 1)   w_i = exp((x_i - max x) / T); T <= 0 or NaN: the largest logit
+ *   top_k[r]       (off: 0)   keep the k largest logits (k <= 0 or k >= vocab: all); a large
+ *                             k (some 870 and above of 262144 logits) or thousands of values
+ *                             equal to the k-th largest take some 25 times as long
  *   top_p[r]       (off: 1)   of those keep each whose larger ones sum to less than
  *                             top_p of their total mass (>= 1 or NaN: all, <= 0: the first)
  *   min_p[r]       (off: 0)   of those keep w_i >= min_p (the first largest always stays: alone above 1, or NaN)

@@ -29,11 +29,13 @@
 // kLift); m, l, S and O are f32.
 // m only rises when a score passes it by 2^8, so O is rarely rescaled.
 //
-// Measured: 96 sequences of 4096 keys on average (ragged, 32 heads of 128 over 8, bf16)
-// 270 us (1.61 GB, 6.0 TB/s, 0.93 of a copy's rate); one sequence of 130001 keys (8 heads
-// of 256 over one) 34 us, 21 of them its bytes: about 5 until the first keys arrive
-// (positions, page table, keys: each needs the one before), 2 to 3 for two
-// joins, 2 for the launch.  One sequence of 1091 keys 10.2 us: the same latencies.
+// Measured in a graph of such calls: 96 sequences of 4096 keys on average (ragged, 32 heads
+// of 128 over 8, bf16) 269 us (1.61 GB, 6.0 TB/s, 0.93 of a copy's rate); one sequence of
+// 130001 keys (8 heads of 256 over one) 35 us, 21 of them its bytes: about 5 until the first
+// keys arrive (positions, page table, keys: each needs the one before), 2 to 3 for two
+// joins, 2 for the launch.  One sequence of 1091 keys 10.7 us: the same latencies.  More than
+// 16 query heads per kv head read K and V once per 16: 64 sequences of 4000 keys with 48
+// heads of 128 over one take 78 us, with 32 over two 58 (twice the bytes, read once).
 #include <algorithm>
 
 #include "paged.cuh"
@@ -42,9 +44,9 @@ namespace {
 
 constexpr int W = 4;  // warps per CTA
 // Partials one CTA joins: more than the square root of the grid, so two levels suffice.  One sequence of 130001 keys
-// (8 heads of 256 over one): 34.1 us with 24, 34.9 with 32, 34.7 with 12.
+// (8 heads of 256 over one): 35.2 us with 24, 36.0 with 32, 35.9 with 12.
 constexpr int JOIN = 24;
-// Keys that a CTA has at least.  One sequence of 1091 keys (17 CTAs of 64): 10.2 us, 10.5 with 128, the same with 32.
+// Keys that a CTA has at least.  One sequence of 1091 keys (17 CTAs of 64): 10.9 us, 12.1 with 128, the same with 32.
 constexpr int MIN_KEYS = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 using sbp::kRise;

@@ -41,23 +41,28 @@
 //
 // Work per 128 x 128 block and head dim HD: 2 * 128 * 128 * HD multiply-adds = 8 HD
 // cycles at 4096 per cycle and SM, and 128 * 128 exponentials = 1024 cycles at 16:
-// tensor-bound at 256, even at 128, bound by the exponentials at 64.  Measured:
+// tensor-bound at 256, even at 128, bound by the exponentials at 64.  Measured (in graphs
+// of such calls where nothing else is said):
 //   256  one prompt of 15001 tokens, 8 heads over one: 2570 cycles per block of 128
-//        keys (2048 of MMA), 617 to 635 us = 1.45 to 1.49 PFLOP/s (0.88 to 0.90 of
-//        the cuBLAS rate) in a single call, 732 to 754 us in a row of them, when the power
-//        limit takes the clock to 1.6 GHz and below.
+//        keys (2048 of MMA), 720 to 728 us = 1.27 to 1.28 PFLOP/s (0.77 of the cuBLAS rate,
+//        0.92 of the sustained one), when the power limit takes the clock to 1.6 GHz and
+//        below; 687 us in calls 30 ms apart, some 20 of them the launch.
 //   128  8 prompts, 8003 tokens, 32 heads over 8: 1710 cycles per block of 64 keys with
 //        two CTAs on an SM (512 each of MMA, 512 each of exponentials): 860 in the
 //        exponentials, 300 for the scores, 150 for the maximum, 100 each for
-//        reading, for handing the scores back and for P.  118 us = 730 TFLOP/s;
-//        bound by that chain, with the tensor pipe and the special-function unit 43 %
+//        reading, for handing the scores back and for P.  105 us = 820 TFLOP/s (122 us in
+//        a row of calls from the host); bound by that chain, with the tensor pipe and the special-function unit 43 %
 //        busy each.  Two threads per row (half the chain, one exchange of the
-//        maximum) took 147 in place of 131, a third CTA does not fit tensor memory.
+//        maximum) took an eighth longer, a third CTA does not fit tensor memory.
+//    64  one prompt of 8000 tokens, 16 heads: 218 us in f16, 216 in bf16 = 600 TFLOP/s
+//        (110 us of exponentials, 79 of MMA at the cuBLAS rate); 8 prompts, 8003 tokens,
+//        16 heads over 4: 51.5 us.
+// With a window of 512, 4 prompts of 2000 tokens: 50 us (8 heads of 256 over one), 94 (32 of
+// 128 over 8); 8 times 128 tokens behind a cached prefix to 4096 (32 of 128 over 8): 79 us.
 //
 // S, O, m and l are f32; p is rounded to the input type for the second product
 // (its relative error is that of the output's own rounding; f16 weights are lifted, see
-// kLift).  Every wait is
-// bounded (2 s): a stuck pipeline records SB_ERR_TIMEOUT and unwinds.
+// kLift).  Every wait is bounded (2 s): a stuck pipeline records SB_ERR_TIMEOUT and unwinds.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -349,8 +354,8 @@ __device__ __forceinline__ Row row_of(const PackedParams& p, const Tile& tl, int
 // What a CTA or a pair does at a time: a plan's tile and a kv head.  It stays and takes one item after another, there
 // and back over the plan (`units` of them do): the tiles come in falling order of their keys, so the sums are about the
 // same.  Each role walks the items by itself, so the loads and scores of one run ahead into the softmax and output of
-// the one before; the rings and the barriers' phases carry on.  Against a CTA or pair per item: 8 packed prompts of
-// 32 x 128 heads, 8003 tokens, take 113 us in place of 133; of 16 x 64 heads, 59 in place of 66 (the launch included).
+// the one before; the rings and the barriers' phases carry on.  Against a CTA or pair per item 8 packed prompts of
+// 32 x 128 heads, 8003 tokens, take 15 % less time, of 16 x 64 heads 11 %.
 struct Item {
   Tile tl;
   int kv;

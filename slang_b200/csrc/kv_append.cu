@@ -10,9 +10,10 @@
 // rotation pairs, v and v + r / 8 (past the rotated part any two), so a pair
 // shares its angles, nothing is exchanged between lanes but the norm's sum, and
 // every load and store is a full vector whatever rot is.  A head takes
-// head_dim / 16 lanes, a warp holds 512 / head_dim heads.  Measured: 16133 packed
-// tokens of 48 x 128 bf16 values 74 to 78 us (397 MB, 5.1 to 5.4 TB/s, 0.80 to 0.84 of
-// a copy's rate); in a graph one token 2.2 us, 256 tokens 3.1 us.
+// head_dim / 16 lanes, a warp holds 512 / head_dim heads.  Measured in a graph of such
+// calls: 16133 packed tokens of 48 x 128 bf16 values 74 us into pages laid out token by
+// token, 78 head by head (397 MB, 5.4 and 5.1 TB/s, 0.84 and 0.79 of a copy's rate), 89
+// with k_out and v_out too (463 MB); one token 2.2 us, 256 tokens 3.0.
 #include "paged.cuh"
 
 namespace {
@@ -147,8 +148,8 @@ int launch_append_r(AppendParams& p, int pieces, cudaStream_t stream) {
 
 // A piece per warp while they fit two full waves (the shortest chain of loads);
 // beyond that three, which keep more bytes in flight.  16133 tokens of 48 heads of
-// 128 in bf16 (398 MB): 86 us with one piece, 78 with two, 70.5 with three (5.6
-// TB/s), 73 with four, whose registers leave one block less per SM.
+// 128 in bf16, pages laid out head by head: 115 us with one piece, 87 with two, 78
+// with three, 84 with four, whose registers leave one block less per SM.
 template <int HD, typename S, typename D>
 int launch_append(AppendParams& p, cudaStream_t stream) {
   constexpr int HPW = 512 / HD;

@@ -35,13 +35,20 @@
 // Masses are added as integers, those of a segment in one order, so neither the
 // order of arrival nor the number of CTAs shows in the result.
 //
-// One row of 262144 f32 logits with top-p takes 11.5 us: 2.2 for the pass, 2.8
-// for the random words on the row's 16 SMs, the rest three joins of its CTAs.  128
-// such rows with mixed settings take 64 us (2.1 TB/s): greedy rows alone 26 (5.1
-// TB/s), min-p 36, top-k 61, no filter 63, top-p 110.  The random words bound the
-// last two: twenty 32 x 32 -> 64 products per four tokens, 16 a cycle and SM, are
-// 37 us for 33.5 million tokens.  (High words through f64 multiply-adds rounded
-// down are exact too and took 64 in place of 59 without a filter.)
+// One row of 262144 f32 logits with top-p takes 11.5 us where the first winner stands:
+// 2.2 for the pass, 2.8 for the random words on the row's 16 SMs, the rest three joins
+// of its CTAs; 14 to 16 on average over rows that race again.  128 such rows with mixed
+// settings take 61 to 65 us by their draws (2.1 TB/s): greedy rows alone 26 (5.1 TB/s),
+// min-p 37, top-k of 20 to 200 61, no filter 64, top-p 92 to 101; mixed with the softcap,
+// whose tanhf is taken of every value that is read, 120 to 132.  The random words bound
+// the rows without a filter and with top-p: twenty 32 x 32 -> 64 products per four
+// tokens, 16 a cycle and SM, are 37 us for 33.5 million tokens.  (High words through f64
+// multiply-adds rounded down are exact too and took 8 % longer without a filter.)
+//
+// Rows whose top-k has more than 1024 candidates (k near 870 and above of 262144 such
+// logits, or thousands of equal values) are searched bit by bit, some 50 passes each:
+// 128 rows with k = 1100 take 1750 us, with k = 850, where a few rows are among them, 95 to
+// 480.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -183,7 +190,8 @@ __device__ __forceinline__ bool is_greedy(float temp, float top_p, float min_p, 
 
 // The row of this cluster when the rows are more than one wave of CTAs: within NT neighbours those that take longest
 // come first (top-p without top-k, no filter, top-k, min-p, greedy; stable), so that the last ones to start are short.
-// 128 rows of 262144 with mixed settings: 64 us in place of 78; rows all of one kind pay 2 us, of 24 (greedy) to 105.
+// Rows of 262144 with mixed settings: 128 of them 63.6 us in place of 66.4, with the softcap 122 in place of 141, 256 of
+// them 101 in place of 111; rows all of one kind pay 2 us, of 25 (greedy) to 100.
 __device__ __forceinline__ int sorted_row(const SampleParams& p, Shared& sh) {
   constexpr int KINDS = 6;  // the last: past the last row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -666,8 +674,10 @@ extern "C" int sb_sample(const void* logits, int dtype, int64_t ld, int rows, in
   p.vec = sb::aligned(logits, 4 * size) && (rows == 1 || ld % 4 == 0);
   p.segs = (vocab + SEG - 1) / SEG;
   p.softcap = softcap;
-  // CTAs per row: as many as make about seven per SM in all, while each warp has a segment.  128 rows of 262144 with
-  // mixed settings: 66 us with 8 per row (two waves, whose phases overlap), 117 with 4, 80 with 16
+  // CTAs per row: as many as make about seven per SM in all, while each warp has a segment.  Rows of 262144 with mixed
+  // settings: 64 of them 46 us with 16 per row (the rule's), 51 with 4; 128 of them 64 with 8 (the rule's, two waves,
+  // whose phases overlap), 85 with 4, 75 with 16; 256 of them 101 with 4 (the rule's), 93 with 8, 140 with 16.  The bound
+  // is met by powers of two just so: 130 rows get 4 and take 76 to 96 by their draws, where 8 took 66.
   int cs = 1;
   while (cs < MAX_CS && p.segs >= cs * 2 * NW && static_cast<int64_t>(rows) * cs * 2 <= 7 * sb::num_sms()) cs *= 2;
   p.sorted = static_cast<int64_t>(rows) * cs > CTAS * sb::num_sms() && (temperature || top_k || top_p || min_p);
