@@ -26,7 +26,11 @@ _F16, _F32 = _lib.SB_F16, _lib.SB_F32
 class PagedRunner:
     """State of up to ``batch`` sequences of ``dm`` over ``n_pages`` pages of ``page_size``
     tokens per layer.  Layers may differ in head_dim (64, 128 or 256), share another
-    layer's K/V and attend over a sliding window; per-layer embeddings are not served."""
+    layer's K/V and attend over a sliding window; per-layer embeddings are not served.
+
+    The batch is fixed from ``prefill`` to the end.  Up to ``GEMV_ROWS`` sequences are
+    sampled from f32 logits, more from f16 ones, so a request may draw another token in
+    a larger batch.  All work runs on the runner's own stream, behind the caller's."""
 
     GEMV_ROWS = 8  # up to this many rows the lm_head is the GEMV with f32 logits, above it the GEMM with f16 ones
 
